@@ -62,9 +62,10 @@ extern "C" {
 #define TG_ERR_DEVICE_STATUS -5  /* a kernel reported a data error (see below)    */
 #define TG_ERR_COLLECTIVE    -6  /* a collective missed its deadline; the communicator was aborted */
 
-/* ---- dtypes of the logits --------------------------------------------------- */
+/* ---- dtypes of the logits and caches --------------------------------------------------- */
 #define TG_DTYPE_F32   0
 #define TG_DTYPE_BF16  1
+#define TG_DTYPE_F16   2  /* caches only */
 
 /* ---- per-row sampling parameters (32 bytes, POD) ---------------------------
  * temperature <= 0 selects greedy.  top_k <= 0 or >= vocab disables top-k.
@@ -384,6 +385,186 @@ int32_t tg_grammar_state_row(const tg_grammar_state* s, int32_t* row, int32_t* i
 /* The host table (rows x ceil(vocab/32) words, row-major) to upload as
  * tg_sample's mask_table; valid until the next tg_grammar_state_row. */
 int32_t tg_grammar_table(tg_grammar* g, const uint32_t** words, int32_t* rows);
+
+/* ---------------------------------------------------------------------------
+ * Paged key/value cache: what a decoder keeps between the calls of tg_sample,
+ * tg_spec_verify and tg_beam_select.  No counterpart in the reference, whose
+ * cache is one sequence's contiguous array (its KVCache).
+ *
+ * Keys and values live in two pools [layers, num_pages, kv_heads, page_size,
+ * head_dim] that the caller owns; the handle owns the bookkeeping, all of it in
+ * device memory: per sequence slot a length, a number of pages and a row of page
+ * ids (-1 past that number), per page the number of rows that hold it.  Every call
+ * is asynchronous on `stream`, reads its row arguments from device memory,
+ * allocates nothing and never waits for the host, so a decode step whose lengths
+ * are decided on the device (tg_cache_accept) needs no round trip and can be
+ * captured in a CUDA graph.  Results do not depend on timing: a call that needs
+ * pages takes the lowest-numbered free ones, row after row.
+ *
+ * A call's `seqs` hold slots in [0, max_seqs), each at most once (tg_cache_fork's
+ * `src` may repeat).  A row that cannot be served is left as it was and sets a
+ * bit of the handle's status word (tg_cache_device_status):
+ *   bit 0: a slot outside [0, max_seqs), or twice in a call that forbids it
+ *   bit 1: not enough free pages (extend: rows are served in order until one
+ *          does not fit; that row and the later ones that need pages get none)
+ *   bit 2: a length past max_pages_per_seq pages, or a negative count or length
+ *   bit 3: keys and values past the pages reserved by tg_cache_extend (not stored),
+ *          or an advance past them
+ *   bit 4: a bounded wait of tg_tree_attention gave up (its output is unreliable)
+ *   bit 5: a tree whose node count is outside [0, nodes]
+ * Threading and streams: as tg_sampler, one handle serves one stream at a time. */
+#define TG_MAX_TREE_NODES 64
+
+typedef struct tg_cache tg_cache;
+
+typedef struct tg_cache_config {
+  int32_t layers;
+  int32_t kv_heads;
+  int32_t head_dim;           /* a multiple of 8, 8..128                          */
+  int32_t page_size;          /* tokens per page: a power of two, 8..256          */
+  int32_t num_pages;
+  int32_t max_seqs;           /* sequence slots                                   */
+  int32_t max_pages_per_seq;
+  int32_t dtype;              /* TG_DTYPE_BF16 or TG_DTYPE_F16                    */
+} tg_cache_config;
+
+/* Device addresses of the bookkeeping, to read (int32): lens [max_seqs], counts
+ * [max_seqs] (pages held), tables [max_seqs, max_pages_per_seq], refs [num_pages]. */
+typedef struct tg_cache_state {
+  const int32_t* lens;
+  const int32_t* counts;
+  const int32_t* tables;
+  const int32_t* refs;
+} tg_cache_state;
+
+/* k_pool, v_pool: device memory, 16-byte aligned, owned by the caller and kept
+ * while the handle lives.  Every slot starts empty. */
+int32_t tg_cache_create(int32_t device, const tg_cache_config* config, void* k_pool, void* v_pool,
+                        tg_cache** out);
+int32_t tg_cache_destroy(tg_cache* c);
+int32_t tg_cache_get_state(tg_cache* c, tg_cache_state* out);
+
+/* Status bits since the last call; synchronizes the device and clears them. */
+int32_t tg_cache_device_status(tg_cache* c, uint32_t* out_bits);
+
+/* Reserves pages so that row i can store counts[i] tokens past its length.  Where
+ * those would start in a page that other rows hold too, the row gets a copy of
+ * its part of that page, in every layer (of several such rows in one call that
+ * are the page's only holders, the first keeps the page).  seqs, counts: [n]. */
+int32_t tg_cache_extend(tg_cache* c, int32_t n, const int32_t* seqs, const int32_t* counts, void* stream);
+
+/* Slot dst[i] becomes a copy of slot src[i] as it was before the call (src[i] = -1:
+ * empty), sharing its pages; pages that dst[i] alone held are freed.  All rows at
+ * once: src may repeat, and src and dst may overlap, as when a beam search's
+ * parents replace the beams.  dst's slots are distinct.  Tokens reserved but not
+ * committed are not taken along. */
+int32_t tg_cache_fork(tg_cache* c, int32_t n, const int32_t* src, const int32_t* dst, void* stream);
+
+/* Sets row i's length back to lens[i] (NULL: to 0) and frees its pages past it,
+ * reserved ones included. */
+int32_t tg_cache_truncate(tg_cache* c, int32_t n, const int32_t* seqs, const int32_t* lens, void* stream);
+
+/* Advances row i's length by counts[i] tokens, already stored in reserved pages. */
+int32_t tg_cache_commit(tg_cache* c, int32_t n, const int32_t* seqs, const int32_t* counts, void* stream);
+
+/* Stores tokens' keys and values in one layer at row i's positions length ..
+ * length + counts[i] - 1 (counts NULL: `tokens` for every row); the length stays
+ * (tg_cache_commit).  k, v: [n, tokens, kv_heads, head_dim] of the cache's dtype with
+ * the given strides in elements (row, token, head); the last dimension is contiguous. */
+int32_t tg_cache_append(tg_cache* c, int32_t layer, int32_t n, const int32_t* seqs, const int32_t* counts,
+                        int32_t tokens, const void* k, int64_t k_row, int64_t k_token, int64_t k_head,
+                        const void* v, int64_t v_row, int64_t v_token, int64_t v_head, void* stream);
+
+/* Attention of each row's drafted nodes over its cached tokens and over the nodes
+ * themselves, in one layer; stores the nodes' keys and values at the row's positions
+ * length + node (reserved by tg_cache_extend; the length stays).
+ *   nodes     nodes per row in the arrays, 1..TG_MAX_TREE_NODES
+ *   n_nodes   [n] nodes of each row (NULL: all); the others' outputs are 0 and
+ *             nothing of them is read
+ *   masks     [n, nodes] uint64: bit j of node i set = node i sees node j (its
+ *             ancestors and itself, as the caller says; NULL: j <= i, a chain or
+ *             a single token)
+ *   q         [n, nodes, q_heads, head_dim], k, v [n, nodes, kv_heads, head_dim] of the
+ *             cache's dtype; strides in elements (row, node, head)
+ *   out       [n, nodes, q_heads, head_dim] contiguous, of the cache's dtype
+ *   out_lse   [n, nodes, q_heads] float: log of the sum of exp(score) (NULL: none)
+ * q_heads is a multiple of kv_heads; query head h reads key head h / (q_heads /
+ * kv_heads).  score = scale * q.k; softmax and sums in 32 bits, the weights rounded
+ * to the cache's dtype for the product with the values.  A node that sees
+ * nothing has output 0 and out_lse -inf.  A node's key or value influences only the
+ * nodes that see it, infinities and NaN included. */
+int32_t tg_tree_attention(tg_cache* c, int32_t layer, int32_t n, const int32_t* seqs, int32_t nodes,
+                          const int32_t* n_nodes, const uint64_t* masks, int32_t q_heads,
+                          const void* q, int64_t q_row, int64_t q_node, int64_t q_head,
+                          const void* k, int64_t k_row, int64_t k_node, int64_t k_head,
+                          const void* v, int64_t v_row, int64_t v_node, int64_t v_head,
+                          float scale, void* out, float* out_lse, void* stream);
+
+/* Settles a step over drafted trees.  Walks each tree from node 0 (the root, whose
+ * token was accepted before): ids[node] is the token that the target model gives
+ * after that node (tg_sample over all nodes' logits); the lowest-numbered child
+ * with that token is taken next, until there is none.  The taken nodes' keys and
+ * values, in every layer, move to positions length, length + 1, ...; the length
+ * grows by their number and the pages past it are freed.
+ *   parents   [n, nodes] int32: a node's parent (before the node; ignored for node 0)
+ *   tokens    [n, nodes] int32: the drafted tokens (ignored for node 0)
+ *   ids       [n, nodes] int32
+ *   n_nodes   [n] (NULL: all)
+ *   out_ids   [n, nodes] int32: the step's new tokens, ids along the path (the
+ *             accepted ones, then the target's own); -1 past out_n
+ *   out_n     [n] int32: their number, also the number of nodes taken
+ * Needs the nodes' positions reserved (tg_cache_extend) and stored. */
+int32_t tg_cache_accept(tg_cache* c, int32_t n, const int32_t* seqs, int32_t nodes, const int32_t* n_nodes,
+                        const int32_t* parents, const int32_t* tokens, const int32_t* ids, int32_t* out_ids,
+                        int32_t* out_n, void* stream);
+
+/* masks[i] of tg_tree_attention from parents: bit i, and the bits of i's ancestors.
+ * parents [n, nodes] as above; nodes past n_nodes (NULL: all) get 0. */
+int32_t tg_tree_masks(int32_t n, int32_t nodes, const int32_t* n_nodes, const int32_t* parents,
+                      uint64_t* masks, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Beam search: the selection of the next beams over beams and vocabulary, with
+ * the reordering of their histories (tg_cache_fork reorders the caches).  The
+ * reference has no beam search.
+ *
+ * For beam w of batch row b, row r = b * beams + w:
+ *   x      = logits[r] (bf16 widened); a clear mask bit, or NaN: -inf; +inf: FLT_MAX
+ *   lse    = max x + log(sum exp(x - max x)), rounded to fp32
+ *   score  = fl(scores[r] + fl(x - lse)), for a finished beam scores[r] for the
+ *            token pad_id alone; NaN counts as -inf
+ * The `beams` best (score, then lowest w * vocab + token) with score > -inf are the
+ * row's next beams in that order; fewer: parent -1, token -1, score -inf, finished. */
+#define TG_MAX_BEAMS 32
+
+typedef struct tg_beam tg_beam;
+
+/* A handle for up to max_batch rows of `beams` beams; owns the workspace (one
+ * stream at a time).  status bits: 0: a state id outside [0, num_states) (its row
+ * is unmasked), 1: a history length outside [0, history_stride] (clamped). */
+int32_t tg_beam_create(int32_t device, int32_t vocab, int32_t beams, int32_t max_batch, tg_beam** out);
+int32_t tg_beam_destroy(tg_beam* h);
+int32_t tg_beam_device_status(tg_beam* h, uint32_t* out_bits);
+
+/* Device pointers; asynchronous on `stream`, allocates nothing.
+ *   logits     [batch * beams, row_stride] of dtype (TG_DTYPE_F32 or TG_DTYPE_BF16)
+ *   scores     [batch, beams] float
+ *   finished   [batch, beams] int32, non-zero = finished (NULL: none)
+ *   mask_table, num_states, state_id [batch * beams]: as tg_sample (NULL: no masks)
+ *   eos_id     a beam that takes it is finished (-1: none); pad_id in [0, vocab)
+ *   history    [batch * beams, history_stride] int32, history_len [batch * beams]
+ *              (NULL: no histories), as tg_sample reads them
+ *   out_parent, out_token [batch, beams] int32; out_score float; out_finished int32
+ *              (may be NULL)
+ *   out_history [batch * beams, history_stride], out_history_len: the parent's
+ *              history, then the token unless the parent was finished or its
+ *              history is full; -1 past the length.  Not the input arrays. */
+int32_t tg_beam_select(tg_beam* h, const void* logits, int32_t dtype, int64_t row_stride, int32_t batch,
+                       const float* scores, const int32_t* finished, const uint32_t* mask_table,
+                       int32_t num_states, const int32_t* state_id, int32_t eos_id, int32_t pad_id,
+                       const int32_t* history, const int32_t* history_len, int32_t history_stride,
+                       int32_t* out_parent, int32_t* out_token, float* out_score, int32_t* out_finished,
+                       int32_t* out_history, int32_t* out_history_len, void* stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */

@@ -22,10 +22,13 @@ TG_ERR_DEVICE_STATUS = -5
 TG_ERR_COLLECTIVE = -6
 TG_DTYPE_F32 = 0
 TG_DTYPE_BF16 = 1
+TG_DTYPE_F16 = 2
 TG_MAX_VOCAB = 1 << 20
 TG_MAX_HISTORY = 4096
 TG_STATIC_SPEC_MAX_ROWS = 8192
 TG_SHARD_CAP = 1280
+TG_MAX_TREE_NODES = 64
+TG_MAX_BEAMS = 32
 TG_GRAMMAR_JSON_SCHEMA = 0
 TG_GRAMMAR_TOOL_TAGS = 1
 SHARD_RECORD_BYTES = 16 + 8 * TG_SHARD_CAP
@@ -44,7 +47,21 @@ EXPORTED = ["tg_abi_version", "tg_last_error_string", "tg_sampler_create", "tg_s
             "tg_grammar_state_create", "tg_grammar_state_destroy", "tg_grammar_accept_bytes",
             "tg_grammar_kind", "tg_grammar_state_clone",
             "tg_grammar_commit", "tg_grammar_is_complete", "tg_grammar_mask",
-            "tg_grammar_state_row", "tg_grammar_table"]
+            "tg_grammar_state_row", "tg_grammar_table",
+            "tg_cache_create", "tg_cache_destroy", "tg_cache_get_state", "tg_cache_device_status", "tg_cache_extend",
+            "tg_cache_fork", "tg_cache_truncate", "tg_cache_commit", "tg_cache_append", "tg_tree_attention", "tg_cache_accept",
+            "tg_tree_masks", "tg_beam_create", "tg_beam_destroy", "tg_beam_device_status", "tg_beam_select"]
+
+
+class CacheConfig(ctypes.Structure):
+    """tg_cache_config."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("layers", "kv_heads", "head_dim", "page_size", "num_pages", "max_seqs",
+                                              "max_pages_per_seq", "dtype")]
+
+
+class CacheState(ctypes.Structure):
+    """tg_cache_state: device addresses."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("lens", "counts", "tables", "refs")]
 
 
 class TGError(RuntimeError):
@@ -119,6 +136,27 @@ def load(path: str = LIB_PATH):
     L.tg_grammar_state_row.argtypes = [vp, ctypes.POINTER(i32), ctypes.POINTER(i32)]
     L.tg_grammar_table.argtypes = [vp, ctypes.POINTER(ctypes.POINTER(ctypes.c_uint32)),
                                    ctypes.POINTER(i32)]
+    L.tg_cache_create.argtypes = [i32, ctypes.POINTER(CacheConfig), vp, vp, ctypes.POINTER(vp)]
+    L.tg_cache_destroy.argtypes = [vp]
+    L.tg_cache_get_state.argtypes = [vp, ctypes.POINTER(CacheState)]
+    L.tg_cache_device_status.argtypes = [vp, ctypes.POINTER(ctypes.c_uint32)]
+    L.tg_cache_extend.argtypes = [vp, i32, vp, vp, vp]
+    L.tg_cache_fork.argtypes = [vp, i32, vp, vp, vp]
+    L.tg_cache_truncate.argtypes = [vp, i32, vp, vp, vp]
+    L.tg_cache_commit.argtypes = [vp, i32, vp, vp, vp]
+    L.tg_cache_append.argtypes = [vp, i32, i32, vp, vp, i32, vp, i64, i64, i64, vp, i64, i64, i64, vp]
+    L.tg_tree_attention.argtypes = [vp, i32, i32, vp, i32, vp, vp, i32, vp, i64, i64, i64, vp, i64, i64, i64,
+                                    vp, i64, i64, i64, ctypes.c_float, vp, vp, vp]
+    L.tg_cache_accept.argtypes = [vp, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp]
+    L.tg_tree_masks.argtypes = [i32, i32, vp, vp, vp, vp]
+    L.tg_beam_create.argtypes = [i32, i32, i32, i32, ctypes.POINTER(vp)]
+    L.tg_beam_destroy.argtypes = [vp]
+    L.tg_beam_device_status.argtypes = [vp, ctypes.POINTER(ctypes.c_uint32)]
+    L.tg_beam_select.argtypes = [vp, vp, i32, i64, i32, vp, vp, vp, i32, vp, i32, i32, vp, vp, i32, vp, vp, vp, vp,
+                                 vp, vp, vp]
+    for name in EXPORTED:
+        if name.startswith(("tg_cache_", "tg_tree_", "tg_beam_")):
+            getattr(L, name).restype = i32
     for name in ("tg_grammar_create", "tg_grammar_destroy", "tg_grammar_state_create",
                  "tg_grammar_kind", "tg_grammar_state_clone",
                  "tg_grammar_state_destroy", "tg_grammar_accept_bytes", "tg_grammar_commit",

@@ -3,6 +3,8 @@ from __future__ import annotations
 
 import os
 import subprocess
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -11,12 +13,13 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 # --fmad=false: the sampling semantics are defined op by op; no contraction.
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "--fmad=false",
-         "-std=c++17", "-Xcompiler", "-fPIC", "-shared", "-diag-suppress", "177,128"]
+         "-std=c++17", "-Xcompiler", "-fPIC", "-diag-suppress", "177,128"]
+UNITS = ["tgsample.cu", "tg_grammar.cpp", "tg_cache.cu", "tg_tree.cu", "tg_beam.cu"]
 
 
 def sources() -> list[str]:
     return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC)
-                  if f.endswith((".cu", ".cuh", ".cpp")))
+                  if f.endswith((".cu", ".cuh", ".cpp", ".h")))
 
 
 def needs_build() -> bool:
@@ -28,12 +31,19 @@ def needs_build() -> bool:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
+    """Compiles the translation units side by side and links the library."""
     if force or needs_build():
-        cmd = [NVCC, *FLAGS, "-o", LIB, os.path.join(CSRC, "tgsample.cu"),
-               os.path.join(CSRC, "tg_grammar.cpp")]
-        if verbose:
-            cmd.insert(1, "-Xptxas=-v")
-        subprocess.run(cmd, check=True)
+        with tempfile.TemporaryDirectory() as tmp:
+            def compile_unit(unit: str) -> str:
+                obj = os.path.join(tmp, unit + ".o")
+                cmd = [NVCC, *FLAGS, "-c", "-o", obj, os.path.join(CSRC, unit)]
+                if verbose:
+                    cmd.insert(1, "-Xptxas=-v")
+                subprocess.run(cmd, check=True)
+                return obj
+            with ThreadPoolExecutor() as pool:
+                objs = list(pool.map(compile_unit, UNITS))
+            subprocess.run([NVCC, *FLAGS, "-shared", "-o", LIB, *objs], check=True)
     return LIB
 
 

@@ -1,0 +1,230 @@
+"""Paged key/value cache and the attention of drafted trees over it (tg_cache_*, tg_tree_*).
+
+What a decoder keeps between the calls of the sampler: `PagedCache` holds the keys
+and values of many sequences in pages that beams share, and all of its
+bookkeeping lives on the device, so a step whose lengths are decided there (a tree's
+accepted path) needs no round trip to the host.  The reference keeps one
+sequence's contiguous cache per layer; it has no counterpart of pages, forks or trees.
+
+A speculative step:  extend -> tree_attention (every layer) -> Sampler.sample over the
+nodes' logits -> accept.  A beam step:  BeamSearch.select -> fork -> extend ->
+tree_attention (every layer, one node) -> commit.
+
+Device arrays are torch CUDA tensors; every call goes through libtgsample.so on the
+current stream (or `stream`).
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+from . import _lib
+from ._lib import check
+from .sampler import _ptr, _stream_ptr
+
+try:
+    import torch
+except ImportError:  # pragma: no cover - the host API needs torch for device memory
+    torch = None
+
+
+class _Handle:
+    """Destroys a tg_cache when the cache and every view of its state are gone."""
+
+    def __init__(self, lib, ptr):
+        self.lib, self.ptr = lib, ptr
+
+    def __del__(self):
+        try:
+            self.lib.tg_cache_destroy(self.ptr)
+        except Exception:  # noqa: BLE001
+            pass
+
+
+class _DeviceInts:
+    """An int32 array that a handle owns, for torch.as_tensor: the tensor keeps the handle alive."""
+
+    def __init__(self, handle: _Handle, ptr: int, shape):
+        self.handle = handle
+        self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": "<i4", "data": (ptr, False), "version": 2}
+
+
+def _rows(t, name: str, n: int | None = None, device: int | None = None):
+    """An int32 contiguous CUDA vector of n entries (None: not given)."""
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or not t.is_cuda:
+        raise ValueError(f"{name} must be a contiguous int32 CUDA vector")
+    if (n is not None and t.shape[0] != n) or (device is not None and t.device.index != device):
+        raise ValueError(f"{name} must have {n} entries on device {device}")
+    return t
+
+
+def _tree(t, name: str, shape, device: int, dtype=None):
+    if t.dtype != (dtype or torch.int32) or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device.index != device:
+        raise ValueError(f"{name} must be a contiguous {dtype or torch.int32} tensor of shape {tuple(shape)} on device {device}")
+    return t
+
+
+def tree_masks(parents, n_nodes=None, *, out=None, stream=None):
+    """tg_tree_masks: int64 [n, nodes] bit sets (a node and its ancestors) from int32 parents [n, nodes]."""
+    n, nodes = parents.shape
+    dev = parents.device.index
+    if dev is None:
+        raise ValueError("parents must be a CUDA tensor")
+    _tree(parents, "parents", (n, nodes), dev)
+    _rows(n_nodes, "n_nodes", n, dev)
+    if out is None:
+        out = torch.empty((n, nodes), dtype=torch.int64, device=parents.device)
+    _tree(out, "out", (n, nodes), dev, torch.int64)
+    with torch.cuda.device(dev):
+        check(_lib.load().tg_tree_masks(n, nodes, _ptr(n_nodes), _ptr(parents), _ptr(out), _stream_ptr(stream)))
+    return out
+
+
+class PagedCache:
+    """A tg_cache handle and its pools k, v [layers, pages, kv_heads, page_size, head_dim].
+
+    lens, counts, tables and refs are views of the handle's device state, to read:
+    lengths and page counts by slot, page ids by slot (-1 past the count), holders by page.
+    """
+
+    def __init__(self, layers: int, kv_heads: int, head_dim: int, page_size: int, num_pages: int, max_seqs: int,
+                 max_pages_per_seq: int, *, dtype=None, device: int = 0, k=None, v=None):
+        dtype = torch.bfloat16 if dtype is None else dtype
+        code = {torch.bfloat16: _lib.TG_DTYPE_BF16, torch.float16: _lib.TG_DTYPE_F16}.get(dtype)
+        if code is None:
+            raise TypeError(f"a cache holds bfloat16 or float16, got {dtype}")
+        shape = (layers, num_pages, kv_heads, page_size, head_dim)
+        self._L = _lib.load()
+        self._h = None
+        self.device = int(device)
+        self.dtype = dtype
+        self.layers, self.kv_heads, self.head_dim, self.page_size = int(layers), int(kv_heads), int(head_dim), int(page_size)
+        self.num_pages, self.max_seqs, self.max_pages_per_seq = int(num_pages), int(max_seqs), int(max_pages_per_seq)
+        if min(shape) <= 0:
+            raise ValueError(f"the pools' shape {shape} must be positive")
+        where = torch.device("cuda", self.device)
+        self.k = torch.empty(shape, dtype=dtype, device=where) if k is None else k
+        self.v = torch.empty(shape, dtype=dtype, device=where) if v is None else v
+        for name, t in (("k", self.k), ("v", self.v)):
+            if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous() or t.device != where:
+                raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {where}")
+        cfg = _lib.CacheConfig(self.layers, self.kv_heads, self.head_dim, self.page_size, self.num_pages, self.max_seqs,
+                               self.max_pages_per_seq, code)
+        h = ctypes.c_void_p()
+        check(self._L.tg_cache_create(self.device, ctypes.byref(cfg), _ptr(self.k), _ptr(self.v), ctypes.byref(h)))
+        self._owner, self._h = _Handle(self._L, h), h
+        st = _lib.CacheState()
+        check(self._L.tg_cache_get_state(self._h, ctypes.byref(st)))
+        view = lambda p, *dims: torch.as_tensor(_DeviceInts(self._owner, p, dims), device=where)  # noqa: E731
+        self.lens = view(st.lens, self.max_seqs)
+        self.counts = view(st.counts, self.max_seqs)
+        self.tables = view(st.tables, self.max_seqs, self.max_pages_per_seq)
+        self.refs = view(st.refs, self.num_pages)
+
+    @property
+    def handle(self):
+        return self._h
+
+    def close(self) -> None:
+        """Lets go of the handle and the pools; views of the state that the caller holds keep the handle."""
+        self._h = self._owner = self.k = self.v = self.lens = self.counts = self.tables = self.refs = None
+
+    def device_status(self) -> int:
+        """Status bits since the last call (synchronizes; see tgsample.h)."""
+        bits = ctypes.c_uint32(0)
+        check(self._L.tg_cache_device_status(self._h, ctypes.byref(bits)))
+        return bits.value
+
+    def extend(self, seqs, counts, *, stream=None) -> None:
+        """Pages for counts[i] tokens past slot seqs[i]'s length; a shared last page is copied first."""
+        n = _rows(seqs, "seqs", None, self.device).shape[0]
+        _rows(counts, "counts", n, self.device)
+        check(self._L.tg_cache_extend(self._h, n, _ptr(seqs), _ptr(counts), _stream_ptr(stream)))
+
+    def fork(self, src, dst, *, stream=None) -> None:
+        """Slots dst[i] become copies of slots src[i] (-1: empty), all at once, sharing pages."""
+        n = _rows(src, "src", None, self.device).shape[0]
+        _rows(dst, "dst", n, self.device)
+        check(self._L.tg_cache_fork(self._h, n, _ptr(src), _ptr(dst), _stream_ptr(stream)))
+
+    def truncate(self, seqs, lens, *, stream=None) -> None:
+        """Sets lengths back to lens[i]; pages past them are freed."""
+        n = _rows(seqs, "seqs", None, self.device).shape[0]
+        _rows(lens, "lens", n, self.device)
+        check(self._L.tg_cache_truncate(self._h, n, _ptr(seqs), _ptr(lens), _stream_ptr(stream)))
+
+    def free(self, seqs, *, stream=None) -> None:
+        """Empties slots."""
+        n = _rows(seqs, "seqs", None, self.device).shape[0]
+        check(self._L.tg_cache_truncate(self._h, n, _ptr(seqs), None, _stream_ptr(stream)))
+
+    def commit(self, seqs, counts, *, stream=None) -> None:
+        """Advances lengths by counts[i] stored tokens."""
+        n = _rows(seqs, "seqs", None, self.device).shape[0]
+        _rows(counts, "counts", n, self.device)
+        check(self._L.tg_cache_commit(self._h, n, _ptr(seqs), _ptr(counts), _stream_ptr(stream)))
+
+    def _tokens(self, t, name: str, n: int, tokens: int, heads: int):
+        if t.dtype != self.dtype or tuple(t.shape) != (n, tokens, heads, self.head_dim) or t.device.index != self.device:
+            raise ValueError(f"{name} must be a {self.dtype} tensor of shape {(n, tokens, heads, self.head_dim)} on device {self.device}")
+        st = t.stride()
+        if st[3] != 1:
+            raise ValueError(f"{name}: the last dimension must be contiguous")
+        return st
+
+    def append(self, layer: int, seqs, k, v, counts=None, *, stream=None) -> None:
+        """Stores keys and values [n, tokens, kv_heads, head_dim] of one layer past the lengths (reserve with
+        extend, advance with commit)."""
+        n, tokens = _rows(seqs, "seqs", None, self.device).shape[0], k.shape[1]
+        ks, vs = self._tokens(k, "k", n, tokens, self.kv_heads), self._tokens(v, "v", n, tokens, self.kv_heads)
+        _rows(counts, "counts", n, self.device)
+        check(self._L.tg_cache_append(self._h, layer, n, _ptr(seqs), _ptr(counts), tokens, _ptr(k), ks[0], ks[1], ks[2],
+                                      _ptr(v), vs[0], vs[1], vs[2], _stream_ptr(stream)))
+
+    def tree_attention(self, layer: int, seqs, q, k, v, masks=None, *, n_nodes=None, scale: float | None = None, out=None,
+                       want_lse: bool = False, lse=None, stream=None):
+        """tg_tree_attention: q [n, nodes, q_heads, head_dim] over the slots' cached tokens and the nodes' own k, v
+        [n, nodes, kv_heads, head_dim], which are also stored past the lengths.  masks: int64 [n, nodes] bit sets
+        (tree_masks; None: a chain).  Returns out, or (out, lse) with want_lse or lse given."""
+        n = _rows(seqs, "seqs", None, self.device).shape[0]
+        if q.dim() != 4:
+            raise ValueError("q must be [n, nodes, q_heads, head_dim]")
+        nodes, heads = q.shape[1], q.shape[2]
+        qs = self._tokens(q, "q", n, nodes, heads)
+        ks, vs = self._tokens(k, "k", n, nodes, self.kv_heads), self._tokens(v, "v", n, nodes, self.kv_heads)
+        if masks is not None:
+            _tree(masks, "masks", (n, nodes), self.device, torch.int64)
+        _rows(n_nodes, "n_nodes", n, self.device)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        else:
+            _tree(out, "out", q.shape, self.device, self.dtype)
+        if lse is not None:
+            _tree(lse, "lse", q.shape[:3], self.device, torch.float32)
+        elif want_lse:
+            lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+        check(self._L.tg_tree_attention(self._h, layer, n, _ptr(seqs), nodes, _ptr(n_nodes), _ptr(masks), heads,
+                                        _ptr(q), qs[0], qs[1], qs[2], _ptr(k), ks[0], ks[1], ks[2], _ptr(v), vs[0], vs[1], vs[2],
+                                        1.0 / math.sqrt(self.head_dim) if scale is None else scale, _ptr(out), _ptr(lse),
+                                        _stream_ptr(stream)))
+        return out if lse is None else (out, lse)
+
+    def accept(self, seqs, parents, tokens, ids, *, n_nodes=None, out_ids=None, out_n=None, stream=None):
+        """tg_cache_accept: walks each tree (parents, drafted tokens [n, nodes]) with the target's ids [n, nodes] and
+        keeps the accepted path in the cache.  Returns (out_ids int32 [n, nodes], out_n int32 [n])."""
+        n = _rows(seqs, "seqs", None, self.device).shape[0]
+        shape = (n, parents.shape[1])
+        for name, t in (("parents", parents), ("tokens", tokens), ("ids", ids)):
+            _tree(t, name, shape, self.device)
+        _rows(n_nodes, "n_nodes", n, self.device)
+        if out_ids is None:
+            out_ids = torch.empty(shape, dtype=torch.int32, device=ids.device)
+        if out_n is None:
+            out_n = torch.empty(n, dtype=torch.int32, device=ids.device)
+        _tree(out_ids, "out_ids", shape, self.device)
+        _rows(out_n, "out_n", n, self.device)
+        check(self._L.tg_cache_accept(self._h, n, _ptr(seqs), shape[1], _ptr(n_nodes), _ptr(parents), _ptr(tokens), _ptr(ids),
+                                      _ptr(out_ids), _ptr(out_n), _stream_ptr(stream)))
+        return out_ids, out_n

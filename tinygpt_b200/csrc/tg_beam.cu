@@ -1,0 +1,677 @@
+// tg_beam.cu -- beam search's selection over beams and vocabulary.
+//
+// Two launches.  scan_kernel streams the logits once: a block takes a part of a row,
+// sums exp(x - max) and finds the part's `beams` largest logits.  merge_kernel takes a
+// batch row: lse from its parts, score = (x - lse) + scores[beam] for the parts'
+// candidates, the `beams` best of them, and the histories.
+//
+// The candidates of a part cost the stream almost nothing: each thread keeps the
+// maximum of every 4 vectors it reads in shared memory.  The (beams + 4)-th largest of
+// the threads' own maxima bounds the part's (beams + 4)-th largest logit from below, so
+// only the few groups that reach it (about beams + 4 of thousands) are read again.
+//
+// Order is by score in fp32, then index, while a part's list is cut by logit.  The two
+// differ only where rounding gives two different logits one score; merge_kernel looks
+// for that at every list's cut and then, as for rows with NaN or +inf or with more ties
+// than a list holds, finds the row's list from the logits themselves (row_exact).
+//
+// Bound: HBM bytes (each logit once) for many rows, launch and reduction latency for
+// few.
+#include "tg_host.h"
+
+#include <cuda_bf16.h>
+
+#include <cfloat>
+#include <cmath>
+#include <new>
+
+namespace tg {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kVecs = 4;         // 16-byte vectors of a group
+constexpr int kMaxGroups = 32;   // groups of a thread in a part
+constexpr int kListMax = 1024;   // candidates of a part before its cut
+constexpr int kExtra = 4;        // candidates past `beams`: the first one cut is then known exactly
+constexpr int kParts = 1184;     // blocks that fill the GPU: 148 SMs x 8
+constexpr float kLog2e = 1.44269504f;
+
+constexpr uint32_t kBadState = 1, kBadHistory = 2;
+
+struct PartHead {
+  float t, l;     // sum over the part of 2^(x log2e - t)
+  float cut;      // the largest logit left out of the list (-inf: none)
+  int32_t count;  // entries of the list; -1: the row needs row_exact
+};
+
+struct Candidate {
+  float x;
+  int32_t id;
+};
+
+struct BeamArgs {
+  const void* logits;
+  int64_t row_stride;
+  int32_t vocab, beams, batch, parts, num_states, mask_words, eos_id, pad_id, history_stride;
+  const float* scores;
+  const int32_t* finished;
+  const uint32_t* mask_table;
+  const int32_t* state_id;
+  const int32_t* history;
+  const int32_t* history_len;
+  int32_t *out_parent, *out_token, *out_finished, *out_history, *out_history_len;
+  float* out_score;
+  PartHead* heads;         // [rows, parts]
+  Candidate* candidates;   // [rows, parts, beams]
+  uint32_t* status;
+};
+
+__device__ __forceinline__ void after_previous_work() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A row adds no candidates of its own when its beam is finished or dead.
+__device__ __forceinline__ bool row_scores(const BeamArgs& a, int row) {
+  const float s = a.scores[row];
+  return s > -INFINITY && !(a.finished && a.finished[row]);
+}
+
+__device__ __forceinline__ const uint32_t* row_mask(const BeamArgs& a, int row) {
+  if (!a.state_id) return nullptr;
+  const int s = a.state_id[row];
+  return s < 0 || s >= a.num_states ? nullptr : a.mask_table + static_cast<size_t>(s) * a.mask_words;
+}
+
+__device__ __forceinline__ bool allowed(const uint32_t* mask, int v) { return !mask || (mask[v >> 5] >> (v & 31) & 1); }
+
+template <int DT>
+struct Elem;
+template <>
+struct Elem<TG_DTYPE_F32> {
+  static constexpr int kPer = 4;
+  using T = float;
+  static __device__ __forceinline__ float get(const float* p) { return __ldg(p); }
+  static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
+    x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
+  }
+  static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+};
+template <>
+struct Elem<TG_DTYPE_BF16> {
+  static constexpr int kPer = 8;
+  using T = uint16_t;
+  static __device__ __forceinline__ float get(const uint16_t* p) { return __uint_as_float(static_cast<uint32_t>(__ldg(p)) << 16); }
+  static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+};
+
+__device__ __forceinline__ uint4 load_stream(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+// The bits of `kPer` tokens from token v on (v + kPer <= vocab).
+template <int kPer>
+__device__ __forceinline__ uint32_t mask_bits(const uint32_t* mask, int v) {
+  const uint32_t lo = __ldg(mask + (v >> 5));
+  const uint32_t hi = (v & 31) + kPer > 32 ? __ldg(mask + (v >> 5) + 1) : 0;
+  return __funnelshift_r(lo, hi, v & 31);
+}
+
+// sum 2^(x log2e - t), rescaled when a group exceeds t: t is a rounded x log2e, so
+// every term is at most about 1, and lse = t / log2e + ln(sum) has no error from the
+// rounding of t.
+struct Sum {
+  float t = -INFINITY, l = 0.0f;
+  template <int N>
+  __device__ __forceinline__ void add(const float* x, float top) {
+    const float at = top * kLog2e;
+    if (at > t) {
+      l *= exp2_fast(t - at);
+      t = at;
+    }
+    if (top > -INFINITY) {
+      float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        s0 += exp2_fast(__fmaf_rn(x[i], kLog2e, -t));
+        s1 += exp2_fast(__fmaf_rn(x[i + 1], kLog2e, -t));
+      }
+      l += s0 + s1;
+    }
+  }
+  __device__ __forceinline__ void merge(float t2, float l2) {
+    if (t2 == -INFINITY) return;
+    if (t2 > t) {
+      l = l * exp2_fast(t - t2) + l2;
+      t = t2;
+    } else {
+      l += l2 * exp2_fast(t2 - t);
+    }
+  }
+};
+
+__device__ __forceinline__ bool before(float xa, int ia, float xb, int ib) { return xa > xb || (xa == xb && ia < ib); }
+
+template <int DT, bool kMasked>
+__global__ void __launch_bounds__(kThreads, 4) scan_kernel(BeamArgs a) {
+  using E = Elem<DT>;
+  constexpr int kPer = E::kPer;
+  __shared__ float group_max[kMaxGroups + 1][kThreads];
+  __shared__ float thread_max[kThreads];
+  __shared__ Candidate list[kListMax];
+  __shared__ float warp_t[kThreads / 32], warp_l[kThreads / 32];
+  __shared__ int n_list;
+  __shared__ float bound;
+  const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
+  after_previous_work();
+  if (!row_scores(a, row)) return;
+  const uint32_t* mask = kMasked ? row_mask(a, row) : nullptr;
+  const typename E::T* p = static_cast<const typename E::T*>(a.logits) + row * a.row_stride;
+  // the row's 16-byte-aligned middle in equal parts; the first part also has the
+  // elements before it, the last those after it
+  const int head = min(static_cast<int>((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / static_cast<int>(sizeof(typename E::T)), a.vocab);
+  const int vecs = (a.vocab - head) / kPer;
+  const int per = (vecs + a.parts - 1) / a.parts;
+  const int v0 = min(part * per, vecs), v1 = min(v0 + per, vecs);
+  const uint4* pv = reinterpret_cast<const uint4*>(p + head);
+  const int groups = (v1 - v0 + kThreads * kVecs - 1) / (kThreads * kVecs);
+
+  Sum sum;
+  float most = -INFINITY;
+  // the odd elements: one per thread, kept as a group of their own
+  int odd = -1;
+  if (part == 0 && tid < head) odd = tid;
+  if (part == a.parts - 1 && tid >= 32) {
+    const int v = head + vecs * kPer + tid - 32;
+    if (v < a.vocab) odd = v;
+  }
+  float odd_x = -INFINITY;
+  if (odd >= 0 && allowed(mask, odd)) {
+    odd_x = fmaxf(E::get(p + odd), -INFINITY);  // NaN: -inf
+    const float raw = E::get(p + odd);
+    const float two[2] = {raw, -INFINITY};
+    sum.add<2>(two, odd_x);
+  }
+  group_max[groups][tid] = odd_x;
+  most = odd_x;
+
+  const auto fetch = [&](int g, uint4* d) {
+#pragma unroll
+    for (int u = 0; u < kVecs; u++) {
+      const int i = v0 + (g * kVecs + u) * kThreads + tid;
+      d[u] = i < v1 ? load_stream(pv + i) : E::nothing();
+    }
+  };
+  const auto values = [&](int g, int u, const uint4& d, float* x) {
+    E::unpack(d, x);
+    if (kMasked && mask) {
+      const int i = v0 + (g * kVecs + u) * kThreads + tid;
+      const uint32_t bits = i < v1 ? mask_bits<kPer>(mask, head + i * kPer) : 0;
+#pragma unroll
+      for (int e = 0; e < kPer; e++) x[e] = bits >> e & 1 ? x[e] : -INFINITY;
+    }
+  };
+  uint4 next[kVecs];
+  if (groups > 0) fetch(0, next);
+  for (int g = 0; g < groups; g++) {
+    uint4 now[kVecs];
+#pragma unroll
+    for (int u = 0; u < kVecs; u++) now[u] = next[u];
+    if (g + 1 < groups) fetch(g + 1, next);
+    float top = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kVecs; u++) {
+      float x[kPer];
+      values(g, u, now[u], x);
+      float m = x[0];
+#pragma unroll
+      for (int e = 1; e < kPer; e++) m = fmaxf(m, x[e]);
+      top = fmaxf(top, m);
+    }
+#pragma unroll
+    for (int u = 0; u < kVecs; u++) {
+      float x[kPer];
+      values(g, u, now[u], x);
+      sum.add<kPer>(x, top);
+    }
+    group_max[g][tid] = top;
+    most = fmaxf(most, top);
+  }
+  // the part's sum
+  float t = sum.t, l = sum.l;
+  for (int d = 16; d; d >>= 1) {
+    const float t2 = __shfl_xor_sync(~0u, t, d), l2 = __shfl_xor_sync(~0u, l, d);
+    Sum s;
+    s.t = t, s.l = l;
+    s.merge(t2, l2);
+    t = s.t, l = s.l;
+  }
+  if ((tid & 31) == 0) warp_t[tid >> 5] = t, warp_l[tid >> 5] = l;
+  thread_max[tid] = most;
+  if (tid == 0) {
+    n_list = 0;
+    bound = -INFINITY;
+  }
+  __syncthreads();
+  // the (beams + kExtra)-th largest thread maximum: each thread counts those before its own
+  int rank = 0;
+  for (int i = 0; i < kThreads; i += 4) {
+    const float4 o = *reinterpret_cast<const float4*>(&thread_max[i]);
+    rank += before(o.x, i, most, tid) + before(o.y, i + 1, most, tid) + before(o.z, i + 2, most, tid) + before(o.w, i + 3, most, tid);
+  }
+  if (rank == a.beams + kExtra - 1) bound = most;
+  __syncthreads();
+  const float low = bound;
+  const auto put = [&](float x, int id) {
+    const int at = atomicAdd(&n_list, 1);
+    if (at < kListMax) list[at] = Candidate{x, id};
+  };
+  if (most >= low && most > -INFINITY) {
+    for (int g = 0; g < groups; g++) {
+      const float top = group_max[g][tid];
+      if (!(top >= low && top > -INFINITY)) continue;
+      uint4 d[kVecs];
+      fetch(g, d);
+#pragma unroll
+      for (int u = 0; u < kVecs; u++) {
+        float x[kPer];
+        values(g, u, d[u], x);
+        const int id = head + (v0 + (g * kVecs + u) * kThreads + tid) * kPer;
+#pragma unroll
+        for (int e = 0; e < kPer; e++)
+          if (x[e] >= low && x[e] > -INFINITY) put(x[e], id + e);
+      }
+    }
+    if (odd_x >= low && odd_x > -INFINITY) put(odd_x, odd);
+  }
+  __syncthreads();
+  const int n = n_list, kept = min(n, a.beams);
+  const int64_t at = static_cast<int64_t>(row) * a.parts + part;
+  if (n <= kListMax) {
+    for (int i = tid; i < n; i += kThreads) {
+      const Candidate c = list[i];
+      int r = 0;
+      for (int j = 0; j < n; j++) r += before(list[j].x, list[j].id, c.x, c.id);
+      if (r < a.beams) a.candidates[at * a.beams + r] = c;
+      if (r == a.beams) a.heads[at].cut = c.x;
+    }
+    if (tid == 0 && n <= a.beams) a.heads[at].cut = -INFINITY;
+  }
+  if (tid == 0) {
+    Sum s;
+    s.t = warp_t[0], s.l = warp_l[0];
+    for (int w = 1; w < kThreads / 32; w++) s.merge(warp_t[w], warp_l[w]);
+    a.heads[at].t = s.t;
+    a.heads[at].l = s.l;
+    // NaN, +inf or logits beyond the range of x log2e in the part: its sum is not finite
+    a.heads[at].count = n <= kListMax && s.l < INFINITY && s.t < INFINITY ? kept : -1;
+  }
+}
+
+// 64-bit keys in the order of the result: score, then the lower index.
+__device__ __forceinline__ uint64_t key_of(float s, uint32_t index) {
+  const uint32_t b = __float_as_uint(s);
+  const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
+  return static_cast<uint64_t>(o) << 32 | (0xffffffffu - index);
+}
+__device__ __forceinline__ float score_of(uint64_t key) {
+  const uint32_t o = static_cast<uint32_t>(key >> 32);
+  return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ uint32_t index_of(uint64_t key) { return 0xffffffffu - static_cast<uint32_t>(key); }
+
+// -0 and +0 are one score.
+__device__ __forceinline__ float score(float x, float lse, float beam) { return ((x - lse) + beam) + 0.0f; }
+
+// The block's largest key; every thread gets it.
+__device__ uint64_t block_max(uint64_t k, uint64_t* warp_keys) {
+  for (int d = 16; d; d >>= 1) {
+    const uint64_t o = __shfl_xor_sync(~0u, k, d);
+    k = o > k ? o : k;
+  }
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) warp_keys[threadIdx.x >> 5] = k;
+  __syncthreads();
+  uint64_t best = 0;
+  for (int w = 0; w < kThreads / 32; w++) best = warp_keys[w] > best ? warp_keys[w] : best;
+  return best;
+}
+
+template <int DT>
+__device__ __forceinline__ float logit(const typename Elem<DT>::T* p, const uint32_t* mask, int v) {
+  if (!allowed(mask, v)) return -INFINITY;
+  return fminf(fmaxf(Elem<DT>::get(p + v), -INFINITY), FLT_MAX);  // NaN: -inf, +inf: the largest finite value
+}
+
+// A row's lse and its `beams` best keys from the logits, by `beams` + 2 passes of the
+// block over the row: what the lists cannot settle.
+template <int DT>
+__device__ void row_exact(const BeamArgs& a, int row, int w, float* lse_out, uint64_t* keys, uint64_t* warp_keys) {
+  const typename Elem<DT>::T* p = static_cast<const typename Elem<DT>::T*>(a.logits) + row * a.row_stride;
+  const uint32_t* mask = row_mask(a, row);
+  const int tid = threadIdx.x;
+  float top = -INFINITY;
+  for (int v = tid; v < a.vocab; v += kThreads) top = fmaxf(top, logit<DT>(p, mask, v));
+  top = score_of(block_max(key_of(top, 0), warp_keys));
+  double sum = 0.0;
+  if (top > -INFINITY)
+    for (int v = tid; v < a.vocab; v += kThreads) sum += exp(static_cast<double>(logit<DT>(p, mask, v)) - static_cast<double>(top));
+  // the block's sum, in a fixed order
+  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+  __syncthreads();
+  if ((tid & 31) == 0) warp_keys[tid >> 5] = __double_as_longlong(sum);
+  __syncthreads();
+  sum = 0.0;
+  for (int i = 0; i < kThreads / 32; i++) sum += __longlong_as_double(warp_keys[i]);
+  const float lse = static_cast<float>(static_cast<double>(top) + log(sum));
+  const float beam = a.scores[row];
+  uint64_t prev = ~0ull;
+  for (int r = 0; r < a.beams; r++) {
+    uint64_t best = 0;
+    if (top > -INFINITY)
+      for (int v = tid; v < a.vocab; v += kThreads) {
+        const float x = logit<DT>(p, mask, v);
+        if (x == -INFINITY) continue;
+        const float s = score(x, lse, beam);
+        if (!(s > -INFINITY)) continue;
+        const uint64_t k = key_of(s, static_cast<uint32_t>(w) * a.vocab + v);
+        if (k < prev && k > best) best = k;
+      }
+    best = block_max(best, warp_keys);
+    if (tid == 0) keys[r] = best;
+    prev = best;
+    if (best == 0) {  // no more: the same for every thread
+      for (int i = r + 1 + tid; i < a.beams; i += kThreads) keys[i] = 0;
+      break;
+    }
+  }
+  if (tid == 0) *lse_out = lse;
+  __syncthreads();
+}
+
+// Key 0: no candidate.
+template <int DT>
+__global__ void __launch_bounds__(kThreads) merge_kernel(BeamArgs a) {
+  extern __shared__ uint64_t keys[];  // [beams, parts, beams]
+  __shared__ uint64_t warp_keys[kThreads / 32], best[TG_MAX_BEAMS];
+  __shared__ float lse[TG_MAX_BEAMS];
+  __shared__ int exact[TG_MAX_BEAMS];  // 1: the row needs row_exact, 2: it had it
+  const int b = blockIdx.x, tid = threadIdx.x, W = a.beams, P = a.parts, row0 = b * W;
+  after_previous_work();
+  const int per_row = P * W, total = W * per_row;
+  // lse of each row: a thread merges a row's parts in order, in 64 bits
+  if (tid < W) {
+    const int row = row0 + tid;
+    int ex = 0;
+    double top = -INFINITY, sum = 0.0;
+    if (row_scores(a, row)) {
+      if (a.state_id && a.state_id[row] >= a.num_states) atomicOr(a.status, kBadState);
+      const PartHead* h = a.heads + static_cast<int64_t>(row) * P;
+      for (int p = 0; p < P; p++) {
+        if (h[p].count < 0) ex = 1;
+        top = fmax(top, static_cast<double>(h[p].t));
+      }
+      for (int p = 0; p < P; p++)
+        if (h[p].t > -INFINITY) sum += static_cast<double>(h[p].l) * exp2(static_cast<double>(h[p].t) - top);
+    }
+    lse[tid] = top > -INFINITY ? static_cast<float>(top / static_cast<double>(kLog2e) + log(sum)) : -INFINITY;
+    exact[tid] = ex;
+  }
+  __syncthreads();
+  for (int i = tid; i < total; i += kThreads) {
+    const int w = i / per_row, p = i % per_row / W, r = i % W, row = row0 + w;
+    uint64_t k = 0;
+    if (row_scores(a, row)) {
+      const int64_t at = static_cast<int64_t>(row) * P + p;
+      if (r < a.heads[at].count) {
+        const Candidate c = a.candidates[at * W + r];
+        const float s = score(c.x, lse[w], a.scores[row]);
+        if (s > -INFINITY) k = key_of(s, static_cast<uint32_t>(w) * a.vocab + c.id);
+      }
+    } else if (i % per_row == 0 && a.scores[row] > -INFINITY) {  // finished: it stays as it is
+      k = key_of(a.scores[row] + 0.0f, static_cast<uint32_t>(w) * a.vocab + a.pad_id);
+    }
+    keys[i] = k;
+  }
+  __syncthreads();
+  for (bool again = true; again;) {
+    again = false;
+    for (int w = 0; w < W; w++)
+      if (exact[w] == 1) {  // the same for every thread
+        for (int i = W + tid; i < per_row; i += kThreads) keys[w * per_row + i] = 0;
+        row_exact<DT>(a, row0 + w, w, &lse[w], keys + w * per_row, warp_keys);
+        if (tid == 0) exact[w] = 2;
+        __syncthreads();
+      }
+    uint64_t prev = ~0ull;
+    for (int r = 0; r < W; r++) {
+      uint64_t k = 0;
+      for (int i = tid; i < total; i += kThreads) {
+        const uint64_t o = keys[i];
+        if (o < prev && o > k) k = o;
+      }
+      k = block_max(k, warp_keys);
+      if (tid == 0) best[r] = k;
+      prev = k;
+    }
+    __syncthreads();
+    // A logit that a list left out matters only if it has the score of one that the
+    // list kept with a larger logit, and that score reaches the selection.
+    const uint64_t last = best[W - 1];
+    for (int i = tid; i < W * P; i += kThreads) {
+      const int w = i / P, row = row0 + w;
+      if (exact[w] || !row_scores(a, row)) continue;
+      const int64_t at = static_cast<int64_t>(row) * P + i % P;
+      const PartHead h = a.heads[at];
+      if (h.cut == -INFINITY || h.count <= 0) continue;
+      // the list's kept logits with the cut one's score, if any, are at its end
+      const float s = score(h.cut, lse[w], a.scores[row]);
+      if (!(s > -INFINITY) || (last != 0 && s < score_of(last))) continue;
+      for (int r = h.count - 1; r >= 0; r--) {
+        const Candidate c = a.candidates[at * W + r];
+        if (score(c.x, lse[w], a.scores[row]) != s) break;
+        if (c.x != h.cut) {
+          exact[w] = 1;
+          break;
+        }
+      }
+    }
+    __syncthreads();
+    for (int w = 0; w < W; w++) again |= exact[w] == 1;
+    __syncthreads();
+  }
+  if (tid < W) {
+    const uint64_t k = best[tid];
+    const uint32_t index = index_of(k);
+    const int parent = k ? static_cast<int>(index / a.vocab) : -1, token = k ? static_cast<int>(index % a.vocab) : -1;
+    const int at = row0 + tid;
+    a.out_parent[at] = parent;
+    a.out_token[at] = token;
+    a.out_score[at] = k ? score_of(k) : -INFINITY;
+    const bool was = k && a.finished && a.finished[row0 + parent];
+    if (a.out_finished) a.out_finished[at] = !k || was || (a.eos_id >= 0 && token == a.eos_id);
+  }
+  if (!a.history) return;
+  for (int w = 0; w < W; w++) {
+    const uint64_t k = best[w];
+    const uint32_t index = index_of(k);
+    const int parent = k ? static_cast<int>(index / a.vocab) : 0, token = static_cast<int>(index % a.vocab);
+    const int32_t* from = a.history + static_cast<int64_t>(row0 + parent) * a.history_stride;
+    int32_t* to = a.out_history + static_cast<int64_t>(row0 + w) * a.history_stride;
+    int len = k ? a.history_len[row0 + parent] : 0;
+    if (len < 0 || len > a.history_stride) {
+      if (tid == 0) atomicOr(a.status, kBadHistory);
+      len = min(max(len, 0), a.history_stride);
+    }
+    const bool grow = k && len < a.history_stride && !(a.finished && a.finished[row0 + parent]);
+    for (int j = tid; j < a.history_stride; j += kThreads) to[j] = j < len ? from[j] : (j == len && grow ? token : -1);
+    if (tid == 0) a.out_history_len[row0 + w] = len + grow;
+  }
+}
+
+// Parts of a row: enough blocks to fill the GPU, none with less than one group per
+// thread, and no more groups than a block keeps.
+int parts_of(int vocab, int per, int rows) {
+  const int step = kThreads * kVecs * per;  // elements of one group of every thread
+  const int most = (vocab + step - 1) / step, least = (most + kMaxGroups - 1) / kMaxGroups;
+  int p = kParts / rows;
+  if (p > most) p = most;
+  if (p < least) p = least;
+  return p < 1 ? 1 : p;
+}
+
+}  // namespace
+}  // namespace tg
+
+struct tg_beam {
+  int device = 0;
+  int vocab = 0;
+  int beams = 0;
+  int max_batch = 0;
+  size_t slots = 0;  // (row, part) pairs that the workspace holds
+  tg::PartHead* heads = nullptr;
+  tg::Candidate* candidates = nullptr;
+  uint32_t* status = nullptr;
+};
+
+using tg::set_error;
+
+extern "C" {
+
+int32_t tg_beam_destroy(tg_beam* h) {
+  if (!h) return TG_OK;
+  {
+    tg::CurrentDevice g(h->device);
+    if (h->heads) cudaFree(h->heads);
+  }
+  delete h;
+  return TG_OK;
+}
+
+int32_t tg_beam_create(int32_t device, int32_t vocab, int32_t beams, int32_t max_batch, tg_beam** out) {
+  if (!out) return set_error(TG_ERR_INVALID_ARG, "out is NULL");
+  *out = nullptr;
+  if (vocab <= 0 || vocab > TG_MAX_VOCAB) return set_error(TG_ERR_UNSUPPORTED, "vocab outside [1, TG_MAX_VOCAB]");
+  if (beams <= 0 || beams > TG_MAX_BEAMS) return set_error(TG_ERR_UNSUPPORTED, "beams outside [1, TG_MAX_BEAMS]");
+  if (max_batch <= 0) return set_error(TG_ERR_INVALID_ARG, "max_batch must be positive");
+  if (max_batch > 65535 / beams) return set_error(TG_ERR_UNSUPPORTED, "max_batch * beams beyond 65535");
+  int ndev = 0;
+  if (cudaGetDeviceCount(&ndev) != cudaSuccess || device < 0 || device >= ndev) return set_error(TG_ERR_NO_DEVICE, "CUDA device not present");
+  tg::CurrentDevice g(device);
+  tg_beam* h = new (std::nothrow) tg_beam();
+  if (!h) return set_error(TG_ERR_CUDA, "out of host memory");
+  h->device = device;
+  h->vocab = vocab;
+  h->beams = beams;
+  h->max_batch = max_batch;
+  const size_t rows = static_cast<size_t>(max_batch) * beams;
+  const size_t least = tg::parts_of(vocab, 4, tg::kParts * 2);  // the parts of a row when rows are many
+  h->slots = rows * least > tg::kParts + rows ? rows * least : tg::kParts + rows;
+  char* base = nullptr;
+  const size_t list_bytes = h->slots * beams * sizeof(tg::Candidate);
+  cudaError_t e = cudaMalloc(&base, h->slots * sizeof(tg::PartHead) + list_bytes + 4);
+  if (e == cudaSuccess) {
+    h->heads = reinterpret_cast<tg::PartHead*>(base);
+    h->candidates = reinterpret_cast<tg::Candidate*>(base + h->slots * sizeof(tg::PartHead));
+    h->status = reinterpret_cast<uint32_t*>(base + h->slots * sizeof(tg::PartHead) + list_bytes);
+    e = cudaMemset(h->status, 0, 4);
+  }
+  const int smem = TG_MAX_BEAMS * 1024 * 8 > 200 * 1024 ? 200 * 1024 : TG_MAX_BEAMS * 1024 * 8;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(tg::merge_kernel<TG_DTYPE_F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(tg::merge_kernel<TG_DTYPE_BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) e = cudaDeviceSynchronize();  // calls may come on any stream
+  if (e != cudaSuccess) {
+    tg_beam_destroy(h);
+    return tg::set_cuda_error(e, "tg_beam_create");
+  }
+  *out = h;
+  return TG_OK;
+}
+
+int32_t tg_beam_device_status(tg_beam* h, uint32_t* out_bits) {
+  if (!h || !out_bits) return set_error(TG_ERR_INVALID_ARG, "NULL argument");
+  tg::CurrentDevice g(h->device);
+  TG_TRY(cudaDeviceSynchronize());
+  TG_TRY(cudaMemcpy(out_bits, h->status, 4, cudaMemcpyDeviceToHost));
+  TG_TRY(cudaMemset(h->status, 0, 4));
+  TG_TRY(cudaDeviceSynchronize());
+  return TG_OK;
+}
+
+int32_t tg_beam_select(tg_beam* h, const void* logits, int32_t dtype, int64_t row_stride, int32_t batch, const float* scores,
+                       const int32_t* finished, const uint32_t* mask_table, int32_t num_states, const int32_t* state_id,
+                       int32_t eos_id, int32_t pad_id, const int32_t* history, const int32_t* history_len,
+                       int32_t history_stride, int32_t* out_parent, int32_t* out_token, float* out_score,
+                       int32_t* out_finished, int32_t* out_history, int32_t* out_history_len, void* stream) {
+  if (!h) return set_error(TG_ERR_INVALID_ARG, "beam handle is NULL");
+  if (dtype != TG_DTYPE_F32 && dtype != TG_DTYPE_BF16) return set_error(TG_ERR_INVALID_ARG, "dtype must be TG_DTYPE_F32 or TG_DTYPE_BF16");
+  if (batch < 0 || batch > h->max_batch) return set_error(TG_ERR_INVALID_ARG, "batch outside [0, max_batch]");
+  if (batch == 0) return TG_OK;
+  if (!logits || !scores || !out_parent || !out_token || !out_score)
+    return set_error(TG_ERR_INVALID_ARG, "logits, scores, out_parent, out_token and out_score are required");
+  if (row_stride < h->vocab) return set_error(TG_ERR_INVALID_ARG, "row_stride < vocab");
+  if (state_id && (!mask_table || num_states <= 0)) return set_error(TG_ERR_INVALID_ARG, "state_id given without mask_table / num_states");
+  if (eos_id < -1 || eos_id >= h->vocab || pad_id < 0 || pad_id >= h->vocab) return set_error(TG_ERR_INVALID_ARG, "eos_id outside [-1, vocab) or pad_id outside [0, vocab)");
+  if (history && (!history_len || !out_history || !out_history_len || history_stride <= 0))
+    return set_error(TG_ERR_INVALID_ARG, "history given without history_len, history_stride, out_history and out_history_len");
+  if (history && (history == out_history || history_len == out_history_len)) return set_error(TG_ERR_INVALID_ARG, "out_history must not be history");
+  const uintptr_t es = dtype == TG_DTYPE_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(logits) % es) return set_error(TG_ERR_INVALID_ARG, "logits is not aligned to its elements");
+  tg::CurrentDevice g(h->device);
+  tg::BeamArgs a{};
+  a.logits = logits;
+  a.row_stride = row_stride;
+  a.vocab = h->vocab;
+  a.beams = h->beams;
+  a.batch = batch;
+  a.parts = tg::parts_of(h->vocab, dtype == TG_DTYPE_F32 ? 4 : 8, batch * h->beams);
+  a.num_states = num_states;
+  a.mask_words = (h->vocab + 31) / 32;
+  a.eos_id = eos_id;
+  a.pad_id = pad_id;
+  a.history_stride = history_stride;
+  a.scores = scores;
+  a.finished = finished;
+  a.mask_table = mask_table;
+  a.state_id = state_id;
+  a.history = history;
+  a.history_len = history_len;
+  a.out_parent = out_parent;
+  a.out_token = out_token;
+  a.out_score = out_score;
+  a.out_finished = out_finished;
+  a.out_history = out_history;
+  a.out_history_len = out_history_len;
+  a.heads = h->heads;
+  a.candidates = h->candidates;
+  a.status = h->status;
+  // the merge holds beams x parts x beams keys in shared memory
+  const size_t most = 200 * 1024 / 8 / (static_cast<size_t>(h->beams) * h->beams);
+  if (static_cast<size_t>(a.parts) > most) a.parts = static_cast<int>(most);
+  const size_t smem = static_cast<size_t>(a.beams) * a.parts * a.beams * 8;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const dim3 grid(a.parts, batch * h->beams);
+  if (dtype == TG_DTYPE_F32) {
+    TG_TRY(tg::launch_after(state_id ? tg::scan_kernel<TG_DTYPE_F32, true> : tg::scan_kernel<TG_DTYPE_F32, false>, grid, tg::kThreads, 0, st, 1, a));
+    TG_TRY(tg::launch_after(tg::merge_kernel<TG_DTYPE_F32>, dim3(batch), tg::kThreads, smem, st, 1, a));
+  } else {
+    TG_TRY(tg::launch_after(state_id ? tg::scan_kernel<TG_DTYPE_BF16, true> : tg::scan_kernel<TG_DTYPE_BF16, false>, grid, tg::kThreads, 0, st, 1, a));
+    TG_TRY(tg::launch_after(tg::merge_kernel<TG_DTYPE_BF16>, dim3(batch), tg::kThreads, smem, st, 1, a));
+  }
+  return TG_OK;
+}
+
+}  // extern "C"

@@ -21,6 +21,7 @@
 #include "tg_fused.cuh"
 #include "tg_theta.cuh"
 #include "tg_spec.cuh"
+#include "tg_host.h"
 
 namespace {
 
@@ -102,6 +103,16 @@ cudaError_t static_scratch(int dev, void** out) {
 }
 
 }  // namespace
+
+namespace tg {
+int32_t set_error(int32_t code, const char* msg) noexcept {
+  try {
+    g_last_error = msg;
+  } catch (...) {  // no memory for the message: the code alone
+  }
+  return code;
+}
+}  // namespace tg
 
 struct tg_sampler {
   int device = 0;
