@@ -1,4 +1,33 @@
 // tg_tree.cu -- attention of drafted nodes over a paged cache (tg_tree_attention).
+//
+//   s_ij = scale q_i . k_j over the cached tokens and the nodes that i sees,
+//   o_i = sum_j 2^(c s_ij - t_i) v_j / sum_j 2^(c s_ij - t_i),  c = scale log2 e
+// in one pass over the keys with a running bound t_i of the row's maximum.
+//
+// Rows.  All query heads of a key head and all nodes read the same keys, so they form
+// the rows of one matrix: row = node * group + head in group.  A work item is (sequence,
+// key head, block of rows); its tiles are the nodes themselves (up to 64 keys, tile 0)
+// and 128 cached tokens each.  Keys and values are read once per item; a single
+// token with 4 heads per key head uses 4 of a tile's 128 rows, which costs nothing while
+// the bytes bound the time (128 rows need 1050 tensor cycles a tile, its 64 KB 2800).
+//
+// Split.  The tiles of all items, in order, are cut into equal runs, one per block, one
+// block per SM: any mix of lengths is balanced to a tile.  An item that is cut
+// leaves (t, sum, unnormalised o) of its runs in a workspace, and join_kernel puts
+// them together in the order of the runs: the result does not depend on timing.
+//
+// A block.  Warp 8 brings pages with tiled TMA into a ring of 128-byte-swizzled slots;
+// warp 9 issues tcgen05.mma: S = Q K^T into TMEM, and O += P V with P read from TMEM;
+// two groups of four warps turn S into P, a thread per row, so no row needs a
+// shuffle.  The two groups work on two S buffers: on two blocks of 128 rows of the same
+// tile when the item has more than 128 rows (kWide), else on alternate tiles of
+// the same rows, joined at the item's end.  While one group exponentiates, the tensor
+// cores work for the other.
+//
+// Rounding: S, the sums and O are fp32; P is rounded to the cache's type for the tensor
+// cores (the products with V take 16-bit operands), relative 2^-8 (bf16) or 2^-11
+// (f16) of a weight, and the output once.  t moves only when a row's maximum exceeds it
+// by more than 8, so P stays below 2^8 and O is rarely rescaled.
 #include "tg_cache.h"
 
 #include <cuda_bf16.h>
@@ -9,93 +38,862 @@
 namespace tg {
 namespace {
 
-__device__ __forceinline__ void after_previous_work() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+constexpr int kThreads = 320;    // 8 softmax warps, a loading warp, an issuing warp
+constexpr int kTile = 128;       // cached tokens of a tile, rows of a row block
+constexpr int kTreeTile = TG_MAX_TREE_NODES;
+constexpr int kWaitLimit = 1 << 21;  // polls of at most about a microsecond
+constexpr float kSlack = 8.0f;   // log2 of how far P may exceed 1
+constexpr float kLog2e = 1.44269504f;
 
 struct Rows {  // [n, nodes, heads, head_dim]: strides in elements
-  const void* p;
+  const uint16_t* p;
   int64_t row, node, head;
 };
 
 struct TreeArgs {
-  int32_t layer, n, nodes, q_heads;
+  int32_t layer, n, nodes, q_heads, group, blocks, min_tiles, vec;  // vec: all rows are 16-byte aligned
   const int32_t* seqs;
   const int32_t* n_nodes;
   const uint64_t* masks;
   Rows q, k, v;
   float scale;
-  void* out;
+  uint16_t* out;
   float* out_lse;
+  int64_t* starts;  // [n + 2] first tile of each sequence, all tiles, tiles of a run
+  float* partial;   // [blocks of the grid, 2, rows, padded dim + 2]
 };
 
-constexpr int kThreads = 128;
+// ---- PTX -----------------------------------------------------------------------------
 
-// A block per (row, node, query head); a warp per key, lanes over the head's
-// dimensions; each warp with its own running maximum and sum.
-template <class T>
-__global__ void __launch_bounds__(kThreads) tree_kernel(CacheView c, TreeArgs a) {
-  __shared__ float wm[4], wl[4], wo[4][128];
-  const int h = blockIdx.x, i = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  after_previous_work();
-  const int D = c.head_dim, kvh = h / (a.q_heads / c.kv_heads);
-  T* out = static_cast<T*>(a.out) + ((static_cast<int64_t>(b) * a.nodes + i) * a.q_heads + h) * D;
-  const int64_t at = (static_cast<int64_t>(b) * a.nodes + i) * a.q_heads + h;
-  const int s = a.seqs[b], given = a.n_nodes ? a.n_nodes[b] : a.nodes;
-  const bool bad = given < 0 || given > a.nodes;
-  const int count = bad ? 0 : given;
-  if (bad && threadIdx.x == 0) atomicOr(c.status, kBadTree);
-  if (s < 0 || s >= c.max_seqs || i >= count) {
-    for (int d = threadIdx.x; d < D; d += kThreads) out[d] = T(0.0f);
-    if (threadIdx.x == 0 && a.out_lse) a.out_lse[at] = -INFINITY;
+__device__ __forceinline__ void after_previous_work() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
+__device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_poll(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(1000u)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ void tma_load(uint32_t to, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(to), "l"(map), "r"(bar), "r"(x), "r"(y),
+      "r"(z), "r"(w)
+      : "memory");
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tmem_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+#define TG_R32(v, o) \
+  "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7]), "=r"(v[o + 8]), "=r"(v[o + 9]), \
+      "=r"(v[o + 10]), "=r"(v[o + 11]), "=r"(v[o + 12]), "=r"(v[o + 13]), "=r"(v[o + 14]), "=r"(v[o + 15]), "=r"(v[o + 16]), "=r"(v[o + 17]), "=r"(v[o + 18]), \
+      "=r"(v[o + 19]), "=r"(v[o + 20]), "=r"(v[o + 21]), "=r"(v[o + 22]), "=r"(v[o + 23]), "=r"(v[o + 24]), "=r"(v[o + 25]), "=r"(v[o + 26]), "=r"(v[o + 27]), \
+      "=r"(v[o + 28]), "=r"(v[o + 29]), "=r"(v[o + 30]), "=r"(v[o + 31])
+#define TG_I32(v, o) \
+  "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7]), "r"(v[o + 8]), "r"(v[o + 9]), \
+      "r"(v[o + 10]), "r"(v[o + 11]), "r"(v[o + 12]), "r"(v[o + 13]), "r"(v[o + 14]), "r"(v[o + 15]), "r"(v[o + 16]), "r"(v[o + 17]), "r"(v[o + 18]), \
+      "r"(v[o + 19]), "r"(v[o + 20]), "r"(v[o + 21]), "r"(v[o + 22]), "r"(v[o + 23]), "r"(v[o + 24]), "r"(v[o + 25]), "r"(v[o + 26]), "r"(v[o + 27]), \
+      "r"(v[o + 28]), "r"(v[o + 29]), "r"(v[o + 30]), "r"(v[o + 31])
+#define TG_REGS32 \
+  "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}"
+
+// 32 columns of this warp's 32 lanes, a lane per thread.
+__device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 " TG_REGS32 ", [%32];" : TG_R32(v, 0) : "r"(at));
+}
+__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], " TG_REGS32 ";" ::TG_I32(v, 0), "r"(at) : "memory");
+}
+
+// Shared-memory matrix descriptor, 128-byte swizzle: start, leading and stride byte
+// offsets in 16-byte units, version 1, layout 2.  K-major operands: stride = 8 rows;
+// the N-major V: leading = the next 64 columns, stride = 8 keys.
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t leading, uint32_t stride) {
+  return static_cast<uint64_t>((addr & 0x3ffff) >> 4) | static_cast<uint64_t>(leading >> 4) << 16 | static_cast<uint64_t>(stride >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+// Instruction descriptor: fp32 result, 16-bit operands (0: f16, 1: bf16), M = 128.
+__device__ __forceinline__ constexpr uint32_t instruction(int bf16, int n, int n_major_b) {
+  return 1u << 4 | static_cast<uint32_t>(bf16) << 7 | static_cast<uint32_t>(bf16) << 10 | static_cast<uint32_t>(n_major_b) << 16 | static_cast<uint32_t>(n >> 3) << 17 |
+         static_cast<uint32_t>(kTile >> 4) << 24;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add)
+               : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add)
+               : "memory");
+}
+
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  uint32_t r;
+  if (kBf16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <bool kBf16>
+__device__ __forceinline__ bool not_finite(uint16_t x) {
+  return kBf16 ? (x & 0x7f80) == 0x7f80 : (x & 0x7c00) == 0x7c00;
+}
+template <bool kBf16>
+__device__ __forceinline__ float widen(uint16_t x) {
+  return kBf16 ? __uint_as_float(static_cast<uint32_t>(x) << 16) : __half2float(__ushort_as_half(x));
+}
+
+// ---- the division of the work ---------------------------------------------------------
+
+// A sequence's part of the work.
+struct Seq {
+  int slot, len, nodes;  // nodes 0 where the row cannot be served
+  int ctx;               // tiles of cached tokens
+  int active;            // row blocks with rows
+  int per_head;          // tiles of a key head
+  uint32_t bad;
+};
+
+template <int kRows>
+__device__ __forceinline__ Seq sequence(const CacheView& c, const TreeArgs& a, int b) {
+  Seq q;
+  q.slot = __ldg(a.seqs + b);
+  q.nodes = a.n_nodes ? __ldg(a.n_nodes + b) : a.nodes;
+  q.bad = 0;
+  if (q.nodes < 0 || q.nodes > a.nodes) q.bad |= kBadTree;
+  if (q.slot < 0 || q.slot >= c.max_seqs) q.bad |= kBadSlot;
+  if (q.bad) q.nodes = 0;
+  q.len = q.bad ? 0 : __ldg(c.lens + q.slot);
+  q.ctx = (q.len + kTile - 1) / kTile;
+  q.active = (q.nodes * a.group + kRows - 1) / kRows;
+  q.per_head = q.active * (q.ctx + 1) + (a.blocks - q.active);
+  return q;
+}
+
+// A run of tiles of one item.
+template <int kRows>
+struct Walk {
+  int64_t left;  // tiles of the block's run from this segment on
+  int64_t off;   // this segment's first tile in the sequence's tiles
+  int b, head, block;
+  int t0, t1, tiles;  // [t0, t1) of the item's tiles
+  bool first, last;   // the run's first, last segment
+  Seq q;
+
+  __device__ void start(const CacheView& c, const TreeArgs& a, int b0, int64_t off0, int64_t count) {
+    b = b0, off = off0, left = count, first = true;
+    q = sequence<kRows>(c, a, b);
+    place();
+  }
+  __device__ void place() {
+    head = static_cast<int>(off / q.per_head);
+    int r = static_cast<int>(off % q.per_head);
+    const int full = q.active * (q.ctx + 1);
+    if (r < full) {
+      tiles = q.ctx + 1;
+      block = r / tiles;
+      t0 = r % tiles;
+    } else {
+      tiles = 1;
+      block = q.active + r - full;
+      t0 = 0;
+    }
+    const int64_t rest = tiles - t0;
+    t1 = t0 + static_cast<int>(rest < left ? rest : left);
+    last = left <= rest;
+  }
+  __device__ bool next(const CacheView& c, const TreeArgs& a) {
+    const int n = t1 - t0;
+    if (last) return false;
+    left -= n;
+    off += n;
+    first = false;
+    if (off == static_cast<int64_t>(q.per_head) * c.kv_heads) {
+      off = 0;
+      b++;
+      q = sequence<kRows>(c, a, b);
+    }
+    place();
+    return true;
+  }
+  __device__ int context_tiles() const { return t1 - max(t0, 1); }
+};
+
+// ---- shared memory ----------------------------------------------------------------------
+
+template <int kDim, bool kWide>
+struct Layout {
+  static constexpr int kBlocks = kDim / 64;                 // 64-column blocks of a row
+  static constexpr int kSlot = kTile * kDim * 2;            // 128 keys or values
+  static constexpr int kQ = (kWide ? 2 : 1) * kTile * kDim * 2;
+  static constexpr int kTree = kTreeTile * kDim * 2;        // the nodes' keys, and as much for their values
+  static constexpr int kSlots = kDim == 128 ? (kWide ? 4 : 5) : 10;
+  static constexpr int kRing = 0, kQAt = kSlots * kSlot, kTreeK = kQAt + kQ, kTreeV = kTreeK + kTree, kBytes = kTreeV + kTree;
+  static constexpr int kRows = kWide ? 2 * kTile : kTile;
+};
+
+struct Control {
+  uint64_t full[10], empty[10], q_full, s_full[2], p_full[2], done, meet, drain;
+  uint64_t odd[3];  // nodes with a value that is not finite, by segment modulo 3
+  float sums[2][2][kTile];  // join of the two groups: t and sum of each row
+  int64_t scan[kThreads / 32 + 1];
+  int64_t run_at, run_off;
+  int32_t run_b, give_up;
+  uint32_t tmem;
+};
+constexpr int kControl = 3072;  // its share of shared memory, in front of the 1024-byte-aligned tiles
+static_assert(sizeof(Control) <= kControl, "the control block outgrew its space");
+
+// Waits for a phase; all 32 lanes get the same answer.  False: the block gives up (this
+// wait or another took too long).
+__device__ __forceinline__ bool wait(Control* ctl, uint64_t* bar, uint32_t parity) {
+  const uint32_t at = smem_addr(bar);
+  for (int i = 0; i < kWaitLimit; i++) {
+    if (__all_sync(~0u, bar_poll(at, parity))) return true;
+    if (__any_sync(~0u, *reinterpret_cast<volatile int32_t*>(&ctl->give_up))) return false;
+  }
+  *reinterpret_cast<volatile int32_t*>(&ctl->give_up) = 1;
+  return false;
+}
+
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) bar_arrive(smem_addr(bar));
+}
+
+// 8 elements of a row from column `col` on, zeros past the head's dimension.
+__device__ __forceinline__ uint4 load8(const uint16_t* row, int col, int dim, bool vec) {
+  uint4 x = make_uint4(0, 0, 0, 0);
+  if (col < dim) {
+    if (vec) {
+      x = __ldg(reinterpret_cast<const uint4*>(row + col));
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) w[i] = __ldg(row + col + 2 * i) | static_cast<uint32_t>(__ldg(row + col + 2 * i + 1)) << 16;
+      x = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  return x;
+}
+
+// The factor of a part (t, sum) of a row in the whole: nothing where the part saw
+// nothing; NaN where all that it saw were NaN.
+__device__ __forceinline__ float weight(float t, float sum, float t_all) { return t == -INFINITY ? sum : exp2_fast(t - t_all); }
+
+template <int kDim, bool kWide, bool kBf16>
+__global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+  using L = Layout<kDim, kWide>;
+  constexpr int kRows = L::kRows, kChunks = kDim / 8;
+  extern __shared__ __align__(1024) uint8_t raw[];
+  Control& ctl = *reinterpret_cast<Control*>(raw);
+  uint8_t* smem = raw + kControl;
+  const uint32_t base = smem_addr(smem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (base & 1023) {  // the swizzle needs it; shared memory starts on such a boundary
+    if (tid == 0) atomicOr(c.status, kGaveUp);
     return;
   }
-  const int len = c.lens[s];
-  const uint64_t mask = a.masks ? a.masks[static_cast<int64_t>(b) * a.nodes + i] : (i == 63 ? ~0ull : (2ull << i) - 1);
-  const T* q = static_cast<const T*>(a.q.p) + b * a.q.row + i * a.q.node + h * a.q.head;
-  float qr[4], o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0;
-  for (int e = 0; e < 4; e++) qr[e] = lane + 32 * e < D ? float(q[lane + 32 * e]) : 0.0f;
-  for (int j = warp; j < len + count; j += 4) {
-    const T *k, *v;
-    if (j < len) {
-      const int64_t page = c.tables[static_cast<size_t>(s) * c.width + (j >> c.page_log2)] + static_cast<int64_t>(a.layer) * c.num_pages;
-      const int64_t off = (((page * c.kv_heads + kvh) << c.page_log2) + (j & (c.page_size - 1))) * D;
-      k = reinterpret_cast<const T*>(c.k) + off;
-      v = reinterpret_cast<const T*>(c.v) + off;
-    } else {
-      if (!(mask >> (j - len) & 1)) continue;
-      k = static_cast<const T*>(a.k.p) + b * a.k.row + (j - len) * a.k.node + kvh * a.k.head;
-      v = static_cast<const T*>(a.v.p) + b * a.v.row + (j - len) * a.v.node + kvh * a.v.head;
+
+  if (tid == 0) {
+    for (int i = 0; i < L::kSlots; i++) {
+      bar_init(smem_addr(&ctl.full[i]), 1);
+      bar_init(smem_addr(&ctl.empty[i]), 1);
     }
-    float dot = 0;
-    for (int e = 0; e < 4; e++)
-      if (lane + 32 * e < D) dot = fmaf(qr[e], float(k[lane + 32 * e]), dot);
-    for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(~0u, dot, d);
-    dot *= a.scale;
-    const float nm = fmaxf(m, dot), f = expf(m - nm), p = expf(dot - nm);
-    m = nm;
-    l = l * f + p;
-    for (int e = 0; e < 4; e++)
-      if (lane + 32 * e < D) o[e] = o[e] * f + p * float(v[lane + 32 * e]);
+    bar_init(smem_addr(&ctl.q_full), 8);
+    for (int i = 0; i < 2; i++) {
+      bar_init(smem_addr(&ctl.s_full[i]), 1);
+      bar_init(smem_addr(&ctl.p_full[i]), 4);
+    }
+    bar_init(smem_addr(&ctl.done), 1);
+    bar_init(smem_addr(&ctl.meet), 8);
+    bar_init(smem_addr(&ctl.drain), 1);
+    ctl.odd[0] = ctl.odd[1] = ctl.odd[2] = 0;
+    ctl.give_up = 0;
+    ctl.run_b = -1;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (lane == 0) wm[warp] = m, wl[warp] = l;
-  for (int e = 0; e < 4; e++) wo[warp][lane + 32 * e] = o[e];
+  if (warp == 9) {  // all 512 columns: shared memory allows one block per SM
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&ctl.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (warp == 8 && lane == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map));
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map));
+  }
+  after_previous_work();
+
+  // this block's run: each thread adds up some sequences' tiles, the one whose sum
+  // reaches the run's first tile finds its place
+  {
+    const int per = (a.n + kThreads - 1) / kThreads, b0 = min(tid * per, a.n), b1 = min(b0 + per, a.n);
+    int64_t mine = 0;
+    uint32_t bad = 0;
+    for (int b = b0; b < b1; b++) {
+      const Seq q = sequence<kRows>(c, a, b);
+      mine += static_cast<int64_t>(q.per_head) * c.kv_heads;
+      bad |= q.bad;
+    }
+    int64_t inc = mine;
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t y = __shfl_up_sync(~0u, inc, d);
+      if (lane >= d) inc += y;
+    }
+    if (lane == 31) ctl.scan[warp] = inc;
+    tmem_before();
+    __syncthreads();
+    tmem_after();
+    int64_t before = 0, total = 0;
+    for (int w = 0; w < kThreads / 32; w++) {
+      if (w < warp) before += ctl.scan[w];
+      total += ctl.scan[w];
+    }
+    int64_t at = before + inc - mine;
+    int64_t run = (total + gridDim.x - 1) / gridDim.x;
+    if (run < a.min_tiles) run = a.min_tiles;
+    const int64_t first = run * blockIdx.x;
+    if (blockIdx.x == 0) {
+      if (bad) atomicOr(c.status, bad);
+      if (tid == 0) a.starts[a.n] = total, a.starts[a.n + 1] = run;
+    }
+    if (first < total && first >= at && first < at + mine || blockIdx.x == 0) {
+      for (int b = b0; b < b1; b++) {
+        const Seq q = sequence<kRows>(c, a, b);
+        const int64_t n = static_cast<int64_t>(q.per_head) * c.kv_heads;
+        if (blockIdx.x == 0) a.starts[b] = at;
+        if (first >= at && first < at + n) {
+          ctl.run_b = b;
+          ctl.run_off = first - at;
+          ctl.run_at = run < total - first ? run : total - first;
+        }
+        at += n;
+      }
+    }
+    __syncthreads();
+  }
+  const uint32_t tmem = ctl.tmem;
+  const bool work = ctl.run_b >= 0;
+
+  if (work && warp == 8) {
+    // ---- loading warp: a lane per page of a tile
+    Walk<kRows> w;
+    w.start(c, a, ctl.run_b, ctl.run_off, ctl.run_at);
+    const int box = min(c.page_size, kTile);  // tokens of a page in a tile
+    uint32_t loaded = 0;
+    bool ok = true;
+    do {
+      for (int t = max(w.t0, 1); ok && t < w.t1; t++) {
+        const int token = (t - 1) * kTile, here = min(kTile, w.q.len - token), n = (here + box - 1) / box;
+        int page = 0;
+        if (lane < n) page = __ldg(c.tables + static_cast<size_t>(w.q.slot) * c.width + ((token + lane * box) >> c.page_log2));
+        const int z = a.layer * c.num_pages + page, y = (token + lane * box) & (c.page_size - 1);
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++) {
+          const uint32_t slot = loaded % L::kSlots, turn = loaded / L::kSlots;
+          if (turn > 0 && !wait(&ctl, &ctl.empty[slot], (turn - 1) & 1)) {
+            ok = false;
+            break;
+          }
+          const uint32_t bar = smem_addr(&ctl.full[slot]), to = base + L::kRing + slot * L::kSlot;
+          if (lane == 0) bar_expect(bar, n * box * L::kBlocks * 128);
+          __syncwarp();
+          if (lane < n) {
+#pragma unroll
+            for (int x = 0; x < L::kBlocks; x++)
+              tma_load(to + x * (kTile * 128) + lane * box * 128, kv ? &v_map : &k_map, bar, x * 64, y, w.head, z);
+          }
+          loaded++;
+        }
+      }
+    } while (ok && w.next(c, a));
+    // on giving up, no copy may still be under way when the block ends
+    if (*reinterpret_cast<volatile int32_t*>(&ctl.give_up)) {
+      const uint32_t from = loaded > L::kSlots ? loaded - L::kSlots : 0;
+      for (uint32_t i = from; i < loaded; i++) {
+        const uint32_t at = smem_addr(&ctl.full[i % L::kSlots]);
+        for (int poll = 0; poll < kWaitLimit && !__all_sync(~0u, bar_poll(at, (i / L::kSlots) & 1)); poll++) {
+        }
+      }
+    }
+  } else if (work && warp == 9) {
+    // ---- issuing warp: S = Q K^T two steps ahead of O += P V
+    Walk<kRows> w;
+    w.start(c, a, ctl.run_b, ctl.run_off, ctl.run_at);
+    constexpr uint32_t s_wide = instruction(kBf16, kTile, 0), s_tree = instruction(kBf16, kTreeTile, 0), o_inst = instruction(kBf16, kDim, 1);
+    uint32_t loaded = 0;              // ring entries before this segment
+    uint32_t segment = 0, p_turn[2] = {0, 0};
+    bool ok = true;
+    do {
+      const int n = (w.t1 - w.t0) * (kWide ? 2 : 1), ctx0 = max(w.t0, 1);
+      ok = wait(&ctl, &ctl.q_full, segment & 1);
+      const auto tile_of = [&](int j) { return w.t0 + (kWide ? j >> 1 : j); };
+      const auto scores = [&](int j) {
+        const int t = tile_of(j), s = j & 1;
+        const uint32_t d = tmem + s * kTile, q = base + L::kQAt + (kWide ? s * (kTile * kDim * 2) : 0);
+        uint32_t k = base + L::kTreeK, rows = kTreeTile, inst = s_tree;
+        if (t > 0) {
+          const uint32_t e = loaded + 2 * (t - ctx0), slot = e % L::kSlots;
+          if (!wait(&ctl, &ctl.full[slot], (e / L::kSlots) & 1)) return false;
+          k = base + L::kRing + slot * L::kSlot, rows = kTile, inst = s_wide;
+          tmem_after();
+        }
+        if (lane == 0) {
+#pragma unroll
+          for (int i = 0; i < kDim / 16; i++) {
+            const uint32_t qa = q + (i >> 2) * (kTile * 128) + (i & 3) * 32, ka = k + (i >> 2) * (rows * 128) + (i & 3) * 32;
+            mma_ss(d, operand(qa, 16, 1024), operand(ka, 16, 1024), inst, i > 0);
+          }
+          tmem_commit(smem_addr(&ctl.s_full[s]));
+          if (t > 0 && (!kWide || s == 1)) tmem_commit(smem_addr(&ctl.empty[(loaded + 2 * (t - ctx0)) % L::kSlots]));
+        }
+        __syncwarp();
+        return true;
+      };
+      tmem_after();
+      for (int j = 0; ok && j < min(n, 2); j++) ok = scores(j);
+      for (int j = 0; ok && j < n; j++) {
+        const int t = tile_of(j), s = j & 1;
+        uint32_t v = base + L::kTreeV, rows = kTreeTile, slot = 0;
+        int keys = w.q.nodes;
+        if (t > 0) {
+          const uint32_t e = loaded + 2 * (t - ctx0) + 1;
+          slot = e % L::kSlots;
+          ok = wait(&ctl, &ctl.full[slot], (e / L::kSlots) & 1);
+          v = base + L::kRing + slot * L::kSlot, rows = kTile;
+          keys = min(kTile, w.q.len - (t - 1) * kTile);
+        }
+        ok = ok && wait(&ctl, &ctl.p_full[s], p_turn[s] & 1);
+        if (!ok) break;
+        p_turn[s]++;
+        tmem_after();
+        if (lane == 0) {
+          const uint32_t d = tmem + 2 * kTile + s * kDim, p = tmem + s * kTile;
+          const int steps = max(1, (keys + 15) / 16);
+          for (int i = 0; i < steps; i++)
+            mma_ts(d, p + i * 8, operand(v + i * 2048, rows * 128, 1024), o_inst, j >= 2 || i > 0);
+          if (t > 0 && (!kWide || s == 1)) tmem_commit(smem_addr(&ctl.empty[slot]));
+          if (j == n - 1) tmem_commit(smem_addr(&ctl.done));
+        }
+        __syncwarp();
+        if (j + 2 < n) ok = scores(j + 2);
+      }
+      loaded += 2 * w.context_tiles();
+      segment++;
+    } while (ok && w.next(c, a));
+    if (!ok) {  // what was issued ends before the block does
+      if (lane == 0) tmem_commit(smem_addr(&ctl.drain));
+      __syncwarp();
+      const uint32_t at = smem_addr(&ctl.drain);
+      for (int poll = 0; poll < kWaitLimit && !__all_sync(~0u, bar_poll(at, 0)); poll++) {
+      }
+    }
+  } else if (work) {
+    // ---- softmax warps: a thread per row
+    Walk<kRows> w;
+    w.start(c, a, ctl.run_b, ctl.run_off, ctl.run_at);
+    const int g = warp >> 2, row = tid & (kTile - 1);       // group, row of its row block
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
+    const uint32_t s_at = tmem + lanes + g * kTile, o_at = tmem + lanes + 2 * kTile + g * kDim;
+    const float cs = fmaxf(fabsf(a.scale) * kLog2e, 1.17549435e-38f);  // not 0: a masked -inf stays -inf
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0;  // scale's sign goes into Q
+    uint32_t loaded = 0, segment = 0, s_turn = 0, meets = 0;
+    bool ok = true;
+    do {
+      const int rows0 = w.block * kRows, rows = min(kRows, w.q.nodes * a.group - rows0);  // rows that are there
+      // Q, and with tile 0 the nodes' keys and values, which also go to the cache
+      if (rows > 0) {
+        for (int i = tid; i < rows * kChunks; i += 256) {
+          const int r = i / kChunks, ch = i % kChunks, node = (rows0 + r) / a.group, h = w.head * a.group + (rows0 + r) % a.group;
+          uint4 x = load8(a.q.p + w.b * a.q.row + node * a.q.node + h * a.q.head, ch * 8, c.head_dim, a.vec);
+          x.x ^= flip, x.y ^= flip, x.z ^= flip, x.w ^= flip;
+          const int rr = r & (kTile - 1);
+          *reinterpret_cast<uint4*>(smem + L::kQAt + (r / kTile) * (kTile * kDim * 2) + (ch >> 3) * (kTile * 128) + rr * 128 + ((ch ^ rr) & 7) * 16) = x;
+        }
+      }
+      if (tid == 0) ctl.odd[(segment + 1) % 3] = 0;
+      if (w.t0 == 0) {
+        const int room = w.q.nodes > 0 ? (__ldg(c.counts + w.q.slot) << c.page_log2) - w.q.len : 0;
+        const int keep = w.block == 0 ? min(w.q.nodes, room) : 0;
+        if (tid == 0 && w.block == 0 && w.head == 0 && w.q.nodes > room) atomicOr(c.status, kNotReserved);
+        for (int i = tid; i < kTreeTile * kChunks; i += 256) {
+          const int j = i / kChunks, ch = i % kChunks;
+          uint4 x = make_uint4(0, 0, 0, 0), y = x;
+          if (j < w.q.nodes) {
+            x = load8(a.k.p + w.b * a.k.row + j * a.k.node + w.head * a.k.head, ch * 8, c.head_dim, a.vec);
+            y = load8(a.v.p + w.b * a.v.row + j * a.v.node + w.head * a.v.head, ch * 8, c.head_dim, a.vec);
+            if (j < keep && ch * 8 < c.head_dim) {
+              const int pos = w.q.len + j;
+              const int64_t page = c.tables[static_cast<size_t>(w.q.slot) * c.width + (pos >> c.page_log2)] + static_cast<int64_t>(a.layer) * c.num_pages;
+              const int64_t at = (((page * c.kv_heads + w.head) << c.page_log2) + (pos & (c.page_size - 1))) * c.head_dim * 2 + ch * 16;
+              *reinterpret_cast<uint4*>(c.k + at) = x;
+              *reinterpret_cast<uint4*>(c.v + at) = y;
+            }
+            // a value that is not finite would reach every row as 0 * inf: it is taken
+            // out here and added to the rows that see it at the end
+            uint32_t ws[4] = {y.x, y.y, y.z, y.w};
+            bool odd = false;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              if (not_finite<kBf16>(ws[e] & 0xffff)) ws[e] &= 0xffff0000u, odd = true;
+              if (not_finite<kBf16>(ws[e] >> 16)) ws[e] &= 0xffffu, odd = true;
+            }
+            if (odd) {
+              atomicOr(reinterpret_cast<unsigned long long*>(&ctl.odd[segment % 3]), 1ull << j);
+              y = make_uint4(ws[0], ws[1], ws[2], ws[3]);
+            }
+          }
+          const int at = (ch >> 3) * (kTreeTile * 128) + j * 128 + ((ch ^ j) & 7) * 16;
+          *reinterpret_cast<uint4*>(smem + L::kTreeK + at) = x;
+          *reinterpret_cast<uint4*>(smem + L::kTreeV + at) = y;
+        }
+      }
+      fence_async();
+      warp_arrive(&ctl.q_full);
+
+      const int r = row + (kWide ? g * kTile : 0);
+      const bool mine = r < rows, any = (r & ~31) < rows;  // this row, this warp's rows are there
+      const int node = mine ? (rows0 + r) / a.group : 0, h = w.head * a.group + (mine ? (rows0 + r) % a.group : 0);
+      uint64_t sees = 0;
+      if (mine && w.t0 == 0) {
+        sees = a.masks ? __ldg(reinterpret_cast<const unsigned long long*>(a.masks) + static_cast<int64_t>(w.b) * a.nodes + node) : ~0ull >> (63 - node);
+        if (w.q.nodes < 64) sees &= (1ull << w.q.nodes) - 1;
+      }
+      float t_ref = -INFINITY, sum = 0.0f;
+      const int step = kWide ? 1 : 2;
+      for (int t = w.t0 + (kWide ? 0 : g); ok && t < w.t1; t += step) {
+        ok = wait(&ctl, &ctl.s_full[g], s_turn & 1);
+        if (!ok) break;
+        s_turn++;
+        tmem_after();
+        const int keys = t > 0 ? min(kTile, w.q.len - (t - 1) * kTile) : kTreeTile;
+        if (any) {
+          float top = -INFINITY;
+          uint32_t v[kTile];
+#pragma unroll
+          for (int i = 0; i < kTile; i += 32)
+            if (i < 64 || t > 0) tmem_load32(s_at + i, v + i);
+          tmem_wait_ld();
+          if (t == 0) {
+#pragma unroll
+            for (int i = 0; i < 64; i++) v[i] = sees >> i & 1 ? v[i] : 0xff800000u;
+#pragma unroll
+            for (int i = 64; i < kTile; i++) v[i] = 0xff800000u;
+          } else if (keys < kTile) {
+#pragma unroll
+            for (int i = 0; i < kTile; i++) v[i] = i < keys ? v[i] : 0xff800000u;
+          }
+          float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < kTile; i += 4) {
+            m0 = fmaxf(m0, __uint_as_float(v[i]));
+            m1 = fmaxf(m1, __uint_as_float(v[i + 1]));
+            m2 = fmaxf(m2, __uint_as_float(v[i + 2]));
+            m3 = fmaxf(m3, __uint_as_float(v[i + 3]));
+          }
+          top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * cs;
+          const bool begun = t >= w.t0 + step;  // O holds something
+          const bool move = top > t_ref + kSlack;
+          if (__any_sync(~0u, move)) {
+            const float f = move ? exp2_fast(t_ref - top) : 1.0f;
+            if (move) t_ref = top;
+            sum *= f;
+            if (begun) {
+#pragma unroll 1
+              for (int i = 0; i < kDim; i += 32) {
+                uint32_t o[32];
+                tmem_load32(o_at + i, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tmem_store32(o_at + i, o);
+              }
+            }
+          }
+          const float t_use = t_ref == -INFINITY ? 0.0f : t_ref;
+          float a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kTile; i += 64) {
+            uint32_t p[32];
+#pragma unroll
+            for (int e = 0; e < 64; e += 4) {
+              const float p0 = exp2_fast(__fmaf_rn(__uint_as_float(v[i + e]), cs, -t_use));
+              const float p1 = exp2_fast(__fmaf_rn(__uint_as_float(v[i + e + 1]), cs, -t_use));
+              const float p2 = exp2_fast(__fmaf_rn(__uint_as_float(v[i + e + 2]), cs, -t_use));
+              const float p3 = exp2_fast(__fmaf_rn(__uint_as_float(v[i + e + 3]), cs, -t_use));
+              a0 += p0, a1 += p1, a2 += p2, a3 += p3;
+              p[e / 2] = pack<kBf16>(p0, p1);
+              p[e / 2 + 1] = pack<kBf16>(p2, p3);
+            }
+            if (i == 0 || t > 0) tmem_store32(s_at + i / 2, p);
+          }
+          sum += (a0 + a1) + (a2 + a3);
+          tmem_wait_st();
+        }
+        if (t > 0 && keys < kTile) {
+          // the rows of V past the sequence's end that the last 16-key step reads are
+          // not its tokens: zeros in their place
+          const uint32_t e = loaded + 2 * (t - max(w.t0, 1)) + 1, slot = e % L::kSlots;
+          ok = wait(&ctl, &ctl.full[slot], (e / L::kSlots) & 1);
+          if (!ok) break;
+          const int end = (keys + 15) & ~15;
+          for (int i = row; i < (end - keys) * kChunks; i += kTile) {
+            const int j = keys + i / kChunks, ch = i % kChunks;
+            *reinterpret_cast<uint4*>(smem + L::kRing + slot * L::kSlot + (ch >> 3) * (kTile * 128) + j * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_async();
+        }
+        tmem_before();
+        warp_arrive(&ctl.p_full[g]);
+      }
+      ok = ok && wait(&ctl, &ctl.done, segment & 1);
+      if (!ok) break;
+      tmem_after();
+      loaded += 2 * w.context_tiles();
+
+      // ---- the segment's end: join the groups, write the rows or leave them to be joined
+      constexpr int kMine = kWide ? kDim : kDim / 2;  // columns that this thread writes
+      const int col0 = kWide ? 0 : g * kMine;
+      const bool whole = w.t0 == 0 && w.t1 == w.tiles;
+      const bool two = !kWide && w.t1 - w.t0 > 1;     // both groups had tiles
+      float f_mine = 1.0f, f_other = 0.0f;
+      const float* other = nullptr;
+      if (!kWide) {
+        // each group hands the other its half of the columns, [column][row]; the space of
+        // Q and the tree is free until the next segment
+        float* give = reinterpret_cast<float*>(smem + L::kQAt) + (g ^ 1) * (kMine * kTile);
+        other = reinterpret_cast<const float*>(smem + L::kQAt) + g * (kMine * kTile);
+        ctl.sums[g][0][row] = t_ref;
+        ctl.sums[g][1][row] = sum;
+        if (any && (two || g == 0)) {
+#pragma unroll 1
+          for (int i = 0; i < kMine; i += 32) {
+            uint32_t o[32];
+            __syncwarp();
+            tmem_load32(o_at + (g ^ 1) * kMine + i, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; e++) give[(i + e) * kTile + row] = __uint_as_float(o[e]);
+          }
+        }
+        warp_arrive(&ctl.meet);
+        ok = wait(&ctl, &ctl.meet, meets++ & 1);
+        if (!ok) break;
+        const float t2 = ctl.sums[g ^ 1][0][row], sum2 = ctl.sums[g ^ 1][1][row];
+        const float t_all = fmaxf(t_ref, t2);
+        f_mine = weight(t_ref, sum, t_all);
+        f_other = weight(t2, sum2, t_all);
+        // in group order in both groups, so that both write the same sum
+        sum = g == 0 ? sum * f_mine + sum2 * f_other : sum2 * f_other + sum * f_mine;
+        t_ref = t_all;
+      }
+      if (any) {
+        const int64_t at = (static_cast<int64_t>(w.b) * a.nodes + node) * a.q_heads + h;
+        const uint64_t odd = w.t0 == 0 ? ctl.odd[segment % 3] & sees : 0;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        float* part = a.partial + ((static_cast<int64_t>(blockIdx.x) * 2 + (w.first ? 0 : 1)) * kRows + r) * (kDim + 2);
+#pragma unroll 1
+        for (int i = 0; i < kMine; i += 32) {
+          uint32_t o[32];
+          const int col = col0 + i;
+          __syncwarp();
+          if (kWide || two || g == 0) {
+            tmem_load32(o_at + col, o);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e++) o[e] = 0;
+          }
+          float x[32];
+#pragma unroll
+          for (int e = 0; e < 32; e++) x[e] = __uint_as_float(o[e]);
+          if (!kWide) {
+#pragma unroll
+            for (int e = 0; e < 32; e++) {
+              const float y = (two || g == 1) ? other[(i + e) * kTile + row] : 0.0f;
+              // a factor of 0 must not meet what an unused accumulator holds
+              x[e] = (f_mine == 0.0f ? 0.0f : x[e] * f_mine) + (f_other == 0.0f ? 0.0f : y * f_other);
+            }
+          }
+          if (odd) {  // rare: the values that were taken out
+            for (uint64_t m = odd; m; m &= m - 1) {
+              const int j = __ffsll(m) - 1;
+              const uint16_t* vr = a.v.p + w.b * a.v.row + j * a.v.node + w.head * a.v.head;
+#pragma unroll
+              for (int e = 0; e < 32; e++)
+                if (col + e < c.head_dim && not_finite<kBf16>(vr[col + e])) x[e] += widen<kBf16>(vr[col + e]);
+            }
+          }
+          if (mine) {
+            if (whole) {
+              uint4* out = reinterpret_cast<uint4*>(a.out + at * c.head_dim + col);
+#pragma unroll
+              for (int e = 0; e < 32; e += 8)
+                if (col + e < c.head_dim)
+                  out[e / 8] = make_uint4(pack<kBf16>(x[e] * inv, x[e + 1] * inv), pack<kBf16>(x[e + 2] * inv, x[e + 3] * inv), pack<kBf16>(x[e + 4] * inv, x[e + 5] * inv),
+                                          pack<kBf16>(x[e + 6] * inv, x[e + 7] * inv));
+            } else {
+              float2* to = reinterpret_cast<float2*>(part + col);
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) to[e / 2] = make_float2(x[e], x[e + 1]);
+            }
+          }
+        }
+        if (mine && (kWide || g == 0)) {
+          if (!whole) *reinterpret_cast<float2*>(part + kDim) = make_float2(t_ref, sum);
+          else if (a.out_lse) a.out_lse[at] = sum == 0.0f ? -INFINITY : static_cast<float>(static_cast<double>(t_ref) * 0.6931471805599453 + log(static_cast<double>(sum)));
+        }
+      }
+      if (w.t0 == 0) {  // rows of nodes that are not there: zeros
+        const int have = max(rows, 0), want = min(kRows, a.nodes * a.group - rows0);
+        for (int i = tid; i < (want - have) * (c.head_dim / 8); i += 256) {
+          const int q = rows0 + have + i / (c.head_dim / 8);
+          const int64_t at = (static_cast<int64_t>(w.b) * a.nodes + q / a.group) * a.q_heads + w.head * a.group + q % a.group;
+          reinterpret_cast<uint4*>(a.out + at * c.head_dim)[i % (c.head_dim / 8)] = make_uint4(0, 0, 0, 0);
+          if (i % (c.head_dim / 8) == 0 && a.out_lse) a.out_lse[at] = -INFINITY;
+        }
+      }
+      tmem_before();  // O has been read before the next segment's first product writes it
+      if (!kWide) {   // and the space of Q before the next segment's Q
+        warp_arrive(&ctl.meet);
+        ok = wait(&ctl, &ctl.meet, meets++ & 1);
+      }
+      segment++;
+    } while (ok && w.next(c, a));
+  }
+  __syncwarp();
+  tmem_before();
   __syncthreads();
-  float top = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
-  float total = 0, f[4];
-  for (int w = 0; w < 4; w++) {
-    f[w] = wm[w] == -INFINITY ? 0.0f : expf(wm[w] - top);
-    total += wl[w] * f[w];
+  if (tid == 0 && ctl.give_up) atomicOr(c.status, kGaveUp);
+  if (warp == 9) {
+    tmem_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }
-  for (int d = threadIdx.x; d < D; d += kThreads) {
-    float x = 0;
-    for (int w = 0; w < 4; w++) x += f[w] == 0.0f ? 0.0f : f[w] * wo[w][d];
-    out[d] = T(total == 0.0f ? 0.0f : x / total);
-  }
-  if (threadIdx.x == 0 && a.out_lse) a.out_lse[at] = total == 0.0f ? -INFINITY : top + logf(total);
 }
+
+// Joins the rows of items that runs cut.  Block x is the cut between runs x and x + 1;
+// the first cut inside an item does the item, a warp per row.
+template <int kDim, bool kWide, bool kBf16>
+__global__ void __launch_bounds__(256) join_kernel(CacheView c, TreeArgs a) {
+  constexpr int kRows = Layout<kDim, kWide>::kRows, kPer = kDim / 32;
+  after_previous_work();
+  const int64_t total = a.starts[a.n], run = a.starts[a.n + 1], cut = run * (blockIdx.x + 1);
+  if (cut >= total) return;
+  int lo = 0, hi = a.n - 1;  // the sequence that holds the cut
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.starts[mid] <= cut) lo = mid; else hi = mid - 1;
+  }
+  Walk<kRows> w;
+  w.start(c, a, lo, cut - a.starts[lo], 1);
+  const int64_t begin = cut - w.t0, end = begin + w.tiles;  // the item's tiles
+  if (w.t0 == 0 || cut - run > begin) return;               // not inside an item, or not the first cut in it
+  const int64_t first = begin / run, last = (end - 1) / run;
+  const int rows0 = w.block * kRows, rows = min(kRows, w.q.nodes * a.group - rows0);
+  const int lane = threadIdx.x & 31;
+  for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 8) {
+    // the item is the second segment of its first run unless the run starts with it
+    const auto part = [&](int64_t x) { return a.partial + ((x * 2 + (x == first && begin % run != 0 ? 1 : 0)) * kRows + r) * (kDim + 2); };
+    float t = -INFINITY;
+    for (int64_t x = first + lane; x <= last; x += 32) t = fmaxf(t, __ldcg(part(x) + kDim));
+    for (int d = 16; d; d >>= 1) t = fmaxf(t, __shfl_xor_sync(~0u, t, d));
+    float sum = 0.0f, o[kPer] = {};
+    for (int64_t x = first; x <= last; x++) {
+      const float* p = part(x);
+      const float2 ts = __ldcg(reinterpret_cast<const float2*>(p + kDim));
+      const float f = weight(ts.x, ts.y, t);
+      sum += f == 0.0f ? 0.0f : f * ts.y;
+#pragma unroll
+      for (int e = 0; e < kPer; e += 2) {
+        const float2 y = __ldcg(reinterpret_cast<const float2*>(p + lane * 2 + e * 32));
+        o[e] += f == 0.0f ? 0.0f : f * y.x;
+        o[e + 1] += f == 0.0f ? 0.0f : f * y.y;
+      }
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int q = rows0 + r;
+    const int64_t at = (static_cast<int64_t>(w.b) * a.nodes + q / a.group) * a.q_heads + w.head * a.group + q % a.group;
+#pragma unroll
+    for (int e = 0; e < kPer; e += 2) {
+      const int col = lane * 2 + e * 32;
+      if (col < c.head_dim) *reinterpret_cast<uint32_t*>(a.out + at * c.head_dim + col) = pack<kBf16>(o[e] * inv, o[e + 1] * inv);
+    }
+    if (lane == 0 && a.out_lse) a.out_lse[at] = sum == 0.0f ? -INFINITY : static_cast<float>(static_cast<double>(t) * 0.6931471805599453 + log(static_cast<double>(sum)));
+  }
+}
+
+template <int kDim, bool kWide>
+constexpr size_t block_smem() { return kControl + Layout<kDim, kWide>::kBytes; }
+
+template <int kDim, bool kWide, bool kBf16>
+cudaError_t allow_smem() {
+  return cudaFuncSetAttribute(tree_kernel<kDim, kWide, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(block_smem<kDim, kWide>()));
+}
+
+template <int kDim, bool kWide, bool kBf16>
+cudaError_t launch(tg_cache* c, const TreeArgs& a, cudaStream_t st) {
+  cudaError_t e = launch_after(tree_kernel<kDim, kWide, kBf16>, dim3(c->sms), kThreads, block_smem<kDim, kWide>(), st, 1, c->view, a, c->k_map, c->v_map);
+  const int rows = a.nodes * a.group < Layout<kDim, kWide>::kRows ? a.nodes * a.group : Layout<kDim, kWide>::kRows;
+  if (e == cudaSuccess) e = launch_after(join_kernel<kDim, kWide, kBf16>, dim3(c->sms - 1, (rows + 15) / 16), 256, 0, st, 1, c->view, a);
+  return e;
+}
+
+template <int kDim>
+cudaError_t launch_dim(tg_cache* c, const TreeArgs& a, bool wide, cudaStream_t st) {
+  const bool bf16 = c->dtype == TG_DTYPE_BF16;
+  if (wide) return bf16 ? launch<kDim, true, true>(c, a, st) : launch<kDim, true, false>(c, a, st);
+  return bf16 ? launch<kDim, false, true>(c, a, st) : launch<kDim, false, false>(c, a, st);
+}
+
+// Starts of the sequences, then the partial rows of every block's two cut items.
+constexpr size_t kStartBytes = (65535 + 2 + 64) * sizeof(int64_t);
+constexpr size_t partial_bytes(int sms) { return static_cast<size_t>(sms) * 2 * 2 * kTile * (128 + 2) * sizeof(float); }
 
 }  // namespace
 
-int32_t tree_setup(tg_cache*) noexcept { return TG_OK; }
+int32_t tree_setup(tg_cache* c) noexcept {
+  typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                               CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  void* fn = nullptr;
+  cudaDriverEntryPointQueryResult found;
+  TG_TRY(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found));
+  if (found != cudaDriverEntryPointSuccess || !fn) return set_error(TG_ERR_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
+  const CacheView& v = c->view;
+  const cuuint64_t d = v.head_dim, ps = v.page_size, heads = v.kv_heads;
+  const cuuint64_t dims[4] = {d, ps, heads, static_cast<cuuint64_t>(v.num_pages) * v.layers};
+  const cuuint64_t strides[3] = {d * 2, d * 2 * ps, d * 2 * ps * heads};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(ps < kTile ? ps : kTile), 1, 1}, ones[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 2; i++) {
+    const CUresult r = reinterpret_cast<EncodeFn>(fn)(i ? &c->v_map : &c->k_map, c->dtype == TG_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                                                      i ? v.v : v.k, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(TG_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+  }
+  TG_TRY((allow_smem<64, false, false>()));
+  TG_TRY((allow_smem<64, false, true>()));
+  TG_TRY((allow_smem<64, true, false>()));
+  TG_TRY((allow_smem<64, true, true>()));
+  TG_TRY((allow_smem<128, false, false>()));
+  TG_TRY((allow_smem<128, false, true>()));
+  TG_TRY((allow_smem<128, true, false>()));
+  TG_TRY((allow_smem<128, true, true>()));
+  TG_TRY(cudaMalloc(&c->partial, kStartBytes + partial_bytes(c->sms)));
+  return TG_OK;
+}
 
 }  // namespace tg
 
@@ -112,17 +910,37 @@ int32_t tg_tree_attention(tg_cache* c, int32_t layer, int32_t n, const int32_t* 
   if (layer < 0 || layer >= c->view.layers) return set_error(TG_ERR_INVALID_ARG, "layer outside [0, layers)");
   if (nodes < 1 || nodes > TG_MAX_TREE_NODES) return set_error(TG_ERR_UNSUPPORTED, "nodes outside [1, TG_MAX_TREE_NODES]");
   if (q_heads <= 0 || q_heads % c->view.kv_heads) return set_error(TG_ERR_INVALID_ARG, "q_heads must be a multiple of kv_heads");
-  if (!(scale == scale) || std::isinf(scale)) return set_error(TG_ERR_INVALID_ARG, "scale must be finite");
+  if (q_heads / c->view.kv_heads > 4096) return set_error(TG_ERR_UNSUPPORTED, "more than 4096 query heads per key head");
+  if (!std::isfinite(scale)) return set_error(TG_ERR_INVALID_ARG, "scale must be finite");
   if (n == 0) return TG_OK;
   if (!seqs || !q || !k || !v || !out) return set_error(TG_ERR_INVALID_ARG, "seqs, q, k, v and out are required");
+  if (reinterpret_cast<uintptr_t>(out) & 15) return set_error(TG_ERR_INVALID_ARG, "out must be 16-byte aligned");
   tg::CurrentDevice g(c->device);
+  tg::TreeArgs a{};
+  a.layer = layer;
+  a.n = n;
+  a.nodes = nodes;
+  a.q_heads = q_heads;
+  a.group = q_heads / c->view.kv_heads;
+  const bool wide = nodes * a.group > tg::kTile;  // more rows than one block of the tensor cores takes
+  const int rows = wide ? 2 * tg::kTile : tg::kTile;
+  a.blocks = (nodes * a.group + rows - 1) / rows;
+  a.min_tiles = 2;
+  a.vec = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+            static_cast<uintptr_t>((q_row | q_node | q_head | k_row | k_node | k_head | v_row | v_node | v_head) * 2)) & 15) == 0;
+  a.seqs = seqs;
+  a.n_nodes = n_nodes;
+  a.masks = masks;
+  a.q = {static_cast<const uint16_t*>(q), q_row, q_node, q_head};
+  a.k = {static_cast<const uint16_t*>(k), k_row, k_node, k_head};
+  a.v = {static_cast<const uint16_t*>(v), v_row, v_node, v_head};
+  a.scale = scale;
+  a.out = static_cast<uint16_t*>(out);
+  a.out_lse = out_lse;
+  a.starts = static_cast<int64_t*>(c->partial);
+  a.partial = reinterpret_cast<float*>(static_cast<char*>(c->partial) + tg::kStartBytes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const tg::TreeArgs a{layer, n, nodes, q_heads, seqs, n_nodes, masks, {q, q_row, q_node, q_head}, {k, k_row, k_node, k_head},
-                       {v, v_row, v_node, v_head}, scale, out, out_lse};
-  const int32_t rc = tg_cache_append(c, layer, n, seqs, n_nodes, nodes, k, k_row, k_node, k_head, v, v_row, v_node, v_head, stream);
-  if (rc != TG_OK) return rc;
-  const dim3 grid(q_heads, nodes, n);
-  TG_TRY(tg::launch_after(c->dtype == TG_DTYPE_BF16 ? tg::tree_kernel<__nv_bfloat16> : tg::tree_kernel<__half>, grid, tg::kThreads, 0, st, 1, c->view, a));
+  TG_TRY(c->view.head_dim <= 64 ? tg::launch_dim<64>(c, a, wide, st) : tg::launch_dim<128>(c, a, wide, st));
   return TG_OK;
 }
 
