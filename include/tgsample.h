@@ -488,8 +488,8 @@ int32_t tg_cache_append(tg_cache* c, int32_t layer, int32_t n, const int32_t* se
  *             cache's dtype; strides in elements (row, node, head)
  *   out       [n, nodes, q_heads, head_dim] contiguous, of the cache's dtype
  *   out_lse   [n, nodes, q_heads] float: log of the sum of exp(score) (NULL: none)
- * q_heads is a multiple of kv_heads; query head h reads key head h / (q_heads /
- * kv_heads).  score = scale * q.k; softmax and sums in 32 bits, the weights rounded
+ * q_heads is a multiple of kv_heads, at most 256 times; query head h reads key head h /
+ * (q_heads / kv_heads).  score = scale * q.k; softmax and sums in 32 bits, the weights rounded
  * to the cache's dtype for the product with the values.  A node that sees
  * nothing has output 0 and out_lse -inf.  A node's key or value influences only the
  * nodes that see it, infinities and NaN included. */

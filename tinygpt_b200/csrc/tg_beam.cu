@@ -94,7 +94,7 @@ template <>
 struct Elem<TG_DTYPE_F32> {
   static constexpr int kPer = 4;
   using T = float;
-  static __device__ __forceinline__ float get(const float* p) { return __ldg(p); }
+  static __device__ __forceinline__ float get(const float* p) { return *p; }
   static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
     x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
   }
@@ -104,7 +104,7 @@ template <>
 struct Elem<TG_DTYPE_BF16> {
   static constexpr int kPer = 8;
   using T = uint16_t;
-  static __device__ __forceinline__ float get(const uint16_t* p) { return __uint_as_float(static_cast<uint32_t>(__ldg(p)) << 16); }
+  static __device__ __forceinline__ float get(const uint16_t* p) { return __uint_as_float(static_cast<uint32_t>(*p) << 16); }
   static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -125,8 +125,8 @@ __device__ __forceinline__ uint4 load_stream(const uint4* p) {
 // The bits of `kPer` tokens from token v on (v + kPer <= vocab).
 template <int kPer>
 __device__ __forceinline__ uint32_t mask_bits(const uint32_t* mask, int v) {
-  const uint32_t lo = __ldg(mask + (v >> 5));
-  const uint32_t hi = (v & 31) + kPer > 32 ? __ldg(mask + (v >> 5) + 1) : 0;
+  const uint32_t lo = mask[v >> 5];
+  const uint32_t hi = (v & 31) + kPer > 32 ? mask[(v >> 5) + 1] : 0;
   return __funnelshift_r(lo, hi, v & 31);
 }
 

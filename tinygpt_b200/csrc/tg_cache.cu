@@ -352,14 +352,14 @@ __global__ void __launch_bounds__(kCopyThreads) append_kernel(CacheView c, int l
     const char* b = v.p + i * v.row + t * v.token + head * v.head + col * 16;
     int4 x, y;
     if (kAligned) {
-      x = __ldg(reinterpret_cast<const int4*>(a));
-      y = __ldg(reinterpret_cast<const int4*>(b));
+      x = *reinterpret_cast<const int4*>(a);
+      y = *reinterpret_cast<const int4*>(b);
     } else {
       uint16_t e[8], f[8];
 #pragma unroll
       for (int m = 0; m < 8; m++) {
-        e[m] = __ldg(reinterpret_cast<const uint16_t*>(a) + m);
-        f[m] = __ldg(reinterpret_cast<const uint16_t*>(b) + m);
+        e[m] = reinterpret_cast<const uint16_t*>(a)[m];
+        f[m] = reinterpret_cast<const uint16_t*>(b)[m];
       }
       memcpy(&x, e, 16);
       memcpy(&y, f, 16);

@@ -34,16 +34,22 @@
 #include <cuda_fp16.h>
 
 #include <cmath>
+#include <type_traits>
 
 namespace tg {
 namespace {
 
-constexpr int kThreads = 320;    // 8 softmax warps, a loading warp, an issuing warp
+constexpr int kThreads = 384;    // 8 softmax warps, a loading warp, an issuing warp, 2 without work
 constexpr int kTile = 128;       // cached tokens of a tile, rows of a row block
 constexpr int kTreeTile = TG_MAX_TREE_NODES;
-constexpr int kWaitLimit = 1 << 21;  // polls of at most about a microsecond
+constexpr int kWaitLimit = 1 << 24;
+constexpr long long kWaitCycles = 1ll << 31;
 constexpr float kSlack = 8.0f;   // log2 of how far P may exceed 1
 constexpr float kLog2e = 1.44269504f;
+
+// x / group by ceil(2^32 / group) (0: group 1): exact while x group^2 < 2^32, as rows below
+// 64 x group and groups up to 256 are.
+__device__ __forceinline__ int divide(int x, uint32_t inverse) { return inverse ? static_cast<int>(__umulhi(x, inverse)) : x; }
 
 struct Rows {  // [n, nodes, heads, head_dim]: strides in elements
   const uint16_t* p;
@@ -52,6 +58,9 @@ struct Rows {  // [n, nodes, heads, head_dim]: strides in elements
 
 struct TreeArgs {
   int32_t layer, n, nodes, q_heads, group, blocks, min_tiles, vec;  // vec: all rows are 16-byte aligned
+  uint32_t group_inverse;  // ceil(2^32 / group)
+  int32_t q_rows, tree_rows, slots;  // shared memory: rows of a row block, of the nodes' tile, ring slots
+  int32_t by_item;         // join_kernel: a block column per item, not per cut
   const int32_t* seqs;
   const int32_t* n_nodes;
   const uint64_t* masks;
@@ -60,7 +69,7 @@ struct TreeArgs {
   uint16_t* out;
   float* out_lse;
   int64_t* starts;  // [n + 2] first tile of each sequence, all tiles, tiles of a run
-  float* partial;   // [blocks of the grid, 2, rows, padded dim + 2]
+  float* partial;   // [blocks of the grid, 2] parts of items (see Part)
 };
 
 // ---- PTX -----------------------------------------------------------------------------
@@ -79,10 +88,16 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
 }
 __device__ __forceinline__ bool bar_poll(uint32_t bar, uint32_t parity) {
   uint32_t ok;
+  asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+// The same from lane 0 alone, by predicate: the warp stays together.
+__device__ __forceinline__ bool bar_poll_lane0(uint32_t bar, uint32_t parity, uint32_t lane) {
+  uint32_t ok;
   asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity), "r"(1000u)
+      "{\n .reg .pred p, q;\n setp.eq.u32 q, %3, 0;\n mov.u32 %0, 0;\n @q mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @q selp.u32 %0, 1, 0, p;\n}"
+      : "=&r"(ok)
+      : "r"(bar), "r"(parity), "r"(lane)
       : "memory");
   return ok != 0;
 }
@@ -172,13 +187,13 @@ struct Seq {
 template <int kRows>
 __device__ __forceinline__ Seq sequence(const CacheView& c, const TreeArgs& a, int b) {
   Seq q;
-  q.slot = __ldg(a.seqs + b);
-  q.nodes = a.n_nodes ? __ldg(a.n_nodes + b) : a.nodes;
+  q.slot = a.seqs[b];
+  q.nodes = a.n_nodes ? a.n_nodes[b] : a.nodes;
   q.bad = 0;
   if (q.nodes < 0 || q.nodes > a.nodes) q.bad |= kBadTree;
   if (q.slot < 0 || q.slot >= c.max_seqs) q.bad |= kBadSlot;
   if (q.bad) q.nodes = 0;
-  q.len = q.bad ? 0 : __ldg(c.lens + q.slot);
+  q.len = q.bad ? 0 : c.lens[q.slot];
   q.ctx = (q.len + kTile - 1) / kTile;
   q.active = (q.nodes * a.group + kRows - 1) / kRows;
   q.per_head = q.active * (q.ctx + 1) + (a.blocks - q.active);
@@ -236,19 +251,25 @@ struct Walk {
 
 // ---- shared memory ----------------------------------------------------------------------
 
+// In front the control block, then Q (each row block [64-column blocks][q_rows][128 bytes]),
+// the nodes' keys and values ([64-column blocks][tree_rows][128 bytes] each) and the ring
+// ([64-column blocks][128][128 bytes] per slot).  Q takes only the rows that the call
+// has: the products read 128 rows from its start, and what the rows past the last hold
+// reaches only results that nothing reads.  The space saved is ring: bytes in flight.
 template <int kDim, bool kWide>
 struct Layout {
-  static constexpr int kBlocks = kDim / 64;                 // 64-column blocks of a row
-  static constexpr int kSlot = kTile * kDim * 2;            // 128 keys or values
-  static constexpr int kQ = (kWide ? 2 : 1) * kTile * kDim * 2;
-  static constexpr int kTree = kTreeTile * kDim * 2;        // the nodes' keys, and as much for their values
-  static constexpr int kSlots = kDim == 128 ? (kWide ? 4 : 5) : 10;
-  static constexpr int kRing = 0, kQAt = kSlots * kSlot, kTreeK = kQAt + kQ, kTreeV = kTreeK + kTree, kBytes = kTreeV + kTree;
+  static constexpr int kBlocks = kDim / 64;       // 64-column blocks of a row
+  static constexpr int kSlot = kTile * kDim * 2;  // 128 keys or values
   static constexpr int kRows = kWide ? 2 * kTile : kTile;
 };
+constexpr int kMaxSlots = 12;
+
+// A part of an item in the workspace: float4 o[kDim / 4][kRows], float2 (t, sum)[kRows].
+template <int kDim, int kRows>
+__device__ __forceinline__ constexpr int part_floats() { return kRows * (kDim + 2); }
 
 struct Control {
-  uint64_t full[10], empty[10], q_full, s_full[2], p_full[2], done, meet, drain;
+  uint64_t full[kMaxSlots], empty[kMaxSlots], q_full, s_full[2], p_full[2], done, meet, drain;
   uint64_t odd[3];  // nodes with a value that is not finite, by segment modulo 3
   float sums[2][2][kTile];  // join of the two groups: t and sum of each row
   int64_t scan[kThreads / 32 + 1];
@@ -259,16 +280,53 @@ struct Control {
 constexpr int kControl = 3072;  // its share of shared memory, in front of the 1024-byte-aligned tiles
 static_assert(sizeof(Control) <= kControl, "the control block outgrew its space");
 
-// Waits for a phase; all 32 lanes get the same answer.  False: the block gives up (this
-// wait or another took too long).
+// A wait gives up after kWaitLimit polls or kWaitCycles cycles (about a second),
+// whichever is first.
+struct Patience {
+  int polls = 0;
+  long long since = 0;
+  __device__ __forceinline__ bool over() {
+    if (++polls == 16) since = clock64();
+    return polls > kWaitLimit || (polls > 16 && (polls & 63) == 0 && clock64() - since > kWaitCycles);
+  }
+};
+
+// Waits for a phase, by a whole warp that stays together (its tcgen05 instructions need
+// that).  False: the block gives up (this wait or another took too long).
 __device__ __forceinline__ bool wait(Control* ctl, uint64_t* bar, uint32_t parity) {
-  const uint32_t at = smem_addr(bar);
-  for (int i = 0; i < kWaitLimit; i++) {
-    if (__all_sync(~0u, bar_poll(at, parity))) return true;
-    if (__any_sync(~0u, *reinterpret_cast<volatile int32_t*>(&ctl->give_up))) return false;
+  const uint32_t at = smem_addr(bar), lane = threadIdx.x & 31;
+  for (Patience p;;) {
+    if (__any_sync(~0u, bar_poll_lane0(at, parity, lane))) {
+      __syncwarp();
+      return true;
+    }
+    if (__any_sync(~0u, *reinterpret_cast<volatile int32_t*>(&ctl->give_up) || p.over())) break;
   }
   *reinterpret_cast<volatile int32_t*>(&ctl->give_up) = 1;
   return false;
+}
+// The same by one lane.
+__device__ __forceinline__ bool wait_alone(Control* ctl, uint64_t* bar, uint32_t parity) {
+  const uint32_t at = smem_addr(bar);
+  for (Patience p;;) {
+    if (bar_poll(at, parity)) return true;
+    if (*reinterpret_cast<volatile int32_t*>(&ctl->give_up) || p.over()) break;
+  }
+  *reinterpret_cast<volatile int32_t*>(&ctl->give_up) = 1;
+  return false;
+}
+// For what is under way when a block gives up.
+__device__ __forceinline__ void wait_out(uint64_t* bar, uint32_t parity) {
+  const uint32_t at = smem_addr(bar);
+  for (Patience p; !bar_poll(at, parity) && !p.over();) {
+  }
+}
+
+// One lane of the warp, the same in every call.
+__device__ __forceinline__ bool elect() {
+  uint32_t yes;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(yes));
+  return yes != 0;
 }
 
 __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
@@ -281,11 +339,11 @@ __device__ __forceinline__ uint4 load8(const uint16_t* row, int col, int dim, bo
   uint4 x = make_uint4(0, 0, 0, 0);
   if (col < dim) {
     if (vec) {
-      x = __ldg(reinterpret_cast<const uint4*>(row + col));
+      x = *reinterpret_cast<const uint4*>(row + col);
     } else {
       uint32_t w[4];
 #pragma unroll
-      for (int i = 0; i < 4; i++) w[i] = __ldg(row + col + 2 * i) | static_cast<uint32_t>(__ldg(row + col + 2 * i + 1)) << 16;
+      for (int i = 0; i < 4; i++) w[i] = row[col + 2 * i] | static_cast<uint32_t>(row[col + 2 * i + 1]) << 16;
       x = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
@@ -296,14 +354,20 @@ __device__ __forceinline__ uint4 load8(const uint16_t* row, int col, int dim, bo
 // nothing; NaN where all that it saw were NaN.
 __device__ __forceinline__ float weight(float t, float sum, float t_all) { return t == -INFINITY ? sum : exp2_fast(t - t_all); }
 
+// ln 2^t sum, with ln 2 in two parts.
+__device__ __forceinline__ float log_sum(float t, float sum) {
+  return sum == 0.0f ? -INFINITY : __fmaf_rn(t, 0.693147182f, __fmaf_rn(t, -1.90465421e-9f, logf(sum)));
+}
+
 template <int kDim, bool kWide, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   using L = Layout<kDim, kWide>;
   constexpr int kRows = L::kRows, kChunks = kDim / 8;
   extern __shared__ __align__(1024) uint8_t raw[];
   Control& ctl = *reinterpret_cast<Control*>(raw);
-  uint8_t* smem = raw + kControl;
-  const uint32_t base = smem_addr(smem);
+  const uint32_t q_block = a.q_rows * 128, q_tile = L::kBlocks * q_block, tree_block = a.tree_rows * 128;  // bytes
+  const uint32_t q_at = kControl, tk_at = q_at + (kWide ? 2 : 1) * q_tile, tv_at = tk_at + L::kBlocks * tree_block, ring_at = tv_at + L::kBlocks * tree_block;
+  const uint32_t base = smem_addr(raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (base & 1023) {  // the swizzle needs it; shared memory starts on such a boundary
     if (tid == 0) atomicOr(c.status, kGaveUp);
@@ -311,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
   }
 
   if (tid == 0) {
-    for (int i = 0; i < L::kSlots; i++) {
+    for (int i = 0; i < kMaxSlots; i++) {
       bar_init(smem_addr(&ctl.full[i]), 1);
       bar_init(smem_addr(&ctl.empty[i]), 1);
     }
@@ -328,7 +392,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
     ctl.run_b = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 9) {  // all 512 columns: shared memory allows one block per SM
+  __syncwarp();
+  if (warp == 1) {  // all 512 columns: shared memory allows one block per SM
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&ctl.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -386,30 +451,33 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
     }
     __syncthreads();
   }
-  const uint32_t tmem = ctl.tmem;
-  const bool work = ctl.run_b >= 0;
+  constexpr uint32_t tmem = 0;  // where 512 columns start
+  const bool work = ctl.run_b >= 0 && ctl.tmem == tmem;
+  if (ctl.tmem != tmem && tid == 0) ctl.give_up = 1;
 
-  if (work && warp == 8) {
+  // registers: 384 x 168 at launch = 256 x 208 (softmax) + 128 x 88 (the rest)
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (work && warp == 8) {
     // ---- loading warp: a lane per page of a tile
     Walk<kRows> w;
     w.start(c, a, ctl.run_b, ctl.run_off, ctl.run_at);
     const int box = min(c.page_size, kTile);  // tokens of a page in a tile
-    uint32_t loaded = 0;
+    uint32_t slot = 0, turn = 0;
     bool ok = true;
     do {
       for (int t = max(w.t0, 1); ok && t < w.t1; t++) {
         const int token = (t - 1) * kTile, here = min(kTile, w.q.len - token), n = (here + box - 1) / box;
         int page = 0;
-        if (lane < n) page = __ldg(c.tables + static_cast<size_t>(w.q.slot) * c.width + ((token + lane * box) >> c.page_log2));
+        if (lane < n) page = c.tables[static_cast<size_t>(w.q.slot) * c.width + ((token + lane * box) >> c.page_log2)];
         const int z = a.layer * c.num_pages + page, y = (token + lane * box) & (c.page_size - 1);
 #pragma unroll
         for (int kv = 0; kv < 2; kv++) {
-          const uint32_t slot = loaded % L::kSlots, turn = loaded / L::kSlots;
           if (turn > 0 && !wait(&ctl, &ctl.empty[slot], (turn - 1) & 1)) {
             ok = false;
             break;
           }
-          const uint32_t bar = smem_addr(&ctl.full[slot]), to = base + L::kRing + slot * L::kSlot;
+          const uint32_t bar = smem_addr(&ctl.full[slot]), to = base + ring_at + slot * L::kSlot;
           if (lane == 0) bar_expect(bar, n * box * L::kBlocks * 128);
           __syncwarp();
           if (lane < n) {
@@ -417,92 +485,105 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
             for (int x = 0; x < L::kBlocks; x++)
               tma_load(to + x * (kTile * 128) + lane * box * 128, kv ? &v_map : &k_map, bar, x * 64, y, w.head, z);
           }
-          loaded++;
+          __syncwarp();
+          if (++slot == static_cast<uint32_t>(a.slots)) slot = 0, turn++;
         }
       }
     } while (ok && w.next(c, a));
     // on giving up, no copy may still be under way when the block ends
-    if (*reinterpret_cast<volatile int32_t*>(&ctl.give_up)) {
-      const uint32_t from = loaded > L::kSlots ? loaded - L::kSlots : 0;
-      for (uint32_t i = from; i < loaded; i++) {
-        const uint32_t at = smem_addr(&ctl.full[i % L::kSlots]);
-        for (int poll = 0; poll < kWaitLimit && !__all_sync(~0u, bar_poll(at, (i / L::kSlots) & 1)); poll++) {
-        }
+    if (lane == 0 && *reinterpret_cast<volatile int32_t*>(&ctl.give_up)) {
+      for (uint32_t i = 0; i < static_cast<uint32_t>(a.slots); i++) {
+        const uint32_t loads = turn + (i < slot ? 1 : 0);  // copies that this slot was given
+        if (loads > 0) wait_out(&ctl.full[i], (loads - 1) & 1);
       }
     }
-  } else if (work && warp == 9) {
-    // ---- issuing warp: S = Q K^T two steps ahead of O += P V
-    Walk<kRows> w;
-    w.start(c, a, ctl.run_b, ctl.run_off, ctl.run_at);
-    constexpr uint32_t s_wide = instruction(kBf16, kTile, 0), s_tree = instruction(kBf16, kTreeTile, 0), o_inst = instruction(kBf16, kDim, 1);
-    uint32_t loaded = 0;              // ring entries before this segment
-    uint32_t segment = 0, p_turn[2] = {0, 0};
-    bool ok = true;
-    do {
-      const int n = (w.t1 - w.t0) * (kWide ? 2 : 1), ctx0 = max(w.t0, 1);
-      ok = wait(&ctl, &ctl.q_full, segment & 1);
-      const auto tile_of = [&](int j) { return w.t0 + (kWide ? j >> 1 : j); };
-      const auto scores = [&](int j) {
-        const int t = tile_of(j), s = j & 1;
-        const uint32_t d = tmem + s * kTile, q = base + L::kQAt + (kWide ? s * (kTile * kDim * 2) : 0);
-        uint32_t k = base + L::kTreeK, rows = kTreeTile, inst = s_tree;
-        if (t > 0) {
-          const uint32_t e = loaded + 2 * (t - ctx0), slot = e % L::kSlots;
-          if (!wait(&ctl, &ctl.full[slot], (e / L::kSlots) & 1)) return false;
-          k = base + L::kRing + slot * L::kSlot, rows = kTile, inst = s_wide;
-          tmem_after();
-        }
-        if (lane == 0) {
+    } else if (work && warp == 9) {
+    // ---- issuing lane: S = Q K^T two steps ahead of O += P V
+    if (elect()) {
+      Walk<kRows> w;
+      w.start(c, a, ctl.run_b, ctl.run_off, ctl.run_at);
+      constexpr uint32_t s_inst = instruction(kBf16, kTile, 0), o_inst = instruction(kBf16, kDim, 1);
+      const uint32_t tree_inst = s_inst - (static_cast<uint32_t>((kTile - a.tree_rows) >> 3) << 17);
+      const uint64_t q_desc = operand(base + q_at, 16, 1024), k_desc = operand(base + ring_at, 16, 1024), v_desc = operand(base + ring_at, kTile * 128, 1024),
+                     tk_desc = operand(base + tk_at, 16, 1024), tv_desc = operand(base + tv_at, tree_block, 1024);
+      const uint32_t slots = a.slots, q_step = q_block / 16, tree_step = tree_block / 16;
+      uint32_t k_slot = 0, k_turn = 0, v_slot = 1 % slots, v_turn = 0;  // the next keys and values in the ring
+      uint32_t segment = 0, p_turn[2] = {0, 0};
+      bool ok = true;
+      do {
+        const int n = (w.t1 - w.t0) * (kWide ? 2 : 1);
+        const auto scores = [&](int j, auto group) {
+          constexpr int s = decltype(group)::value;
+          const int t = w.t0 + (kWide ? j >> 1 : j);
+          const uint64_t qd = q_desc + (kWide ? s * (q_tile / 16) : 0);
+          constexpr uint32_t d = s * kTile;
+          if (t > 0) {
+            if (!wait_alone(&ctl, &ctl.full[k_slot], k_turn & 1)) return false;
+            tmem_after();
+            const uint64_t kd = k_desc + k_slot * (L::kSlot / 16);
 #pragma unroll
-          for (int i = 0; i < kDim / 16; i++) {
-            const uint32_t qa = q + (i >> 2) * (kTile * 128) + (i & 3) * 32, ka = k + (i >> 2) * (rows * 128) + (i & 3) * 32;
-            mma_ss(d, operand(qa, 16, 1024), operand(ka, 16, 1024), inst, i > 0);
+            for (int i = 0; i < kDim / 16; i++) mma_ss(d, qd + (i >> 2) * q_step + (i & 3) * 2, kd + (i >> 2) * (kTile * 128 / 16) + (i & 3) * 2, s_inst, i > 0);
+            tmem_commit(smem_addr(&ctl.s_full[s]));
+            if (!kWide || s == 1) {
+              tmem_commit(smem_addr(&ctl.empty[k_slot]));
+              k_slot += 2;
+              if (k_slot >= slots) k_slot -= slots, k_turn++;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < kDim / 16; i++) mma_ss(d, qd + (i >> 2) * q_step + (i & 3) * 2, tk_desc + (i >> 2) * tree_step + (i & 3) * 2, tree_inst, i > 0);
+            tmem_commit(smem_addr(&ctl.s_full[s]));
           }
-          tmem_commit(smem_addr(&ctl.s_full[s]));
-          if (t > 0 && (!kWide || s == 1)) tmem_commit(smem_addr(&ctl.empty[(loaded + 2 * (t - ctx0)) % L::kSlots]));
-        }
-        __syncwarp();
-        return true;
-      };
-      tmem_after();
-      for (int j = 0; ok && j < min(n, 2); j++) ok = scores(j);
-      for (int j = 0; ok && j < n; j++) {
-        const int t = tile_of(j), s = j & 1;
-        uint32_t v = base + L::kTreeV, rows = kTreeTile, slot = 0;
-        int keys = w.q.nodes;
-        if (t > 0) {
-          const uint32_t e = loaded + 2 * (t - ctx0) + 1;
-          slot = e % L::kSlots;
-          ok = wait(&ctl, &ctl.full[slot], (e / L::kSlots) & 1);
-          v = base + L::kRing + slot * L::kSlot, rows = kTile;
-          keys = min(kTile, w.q.len - (t - 1) * kTile);
-        }
-        ok = ok && wait(&ctl, &ctl.p_full[s], p_turn[s] & 1);
-        if (!ok) break;
-        p_turn[s]++;
-        tmem_after();
-        if (lane == 0) {
-          const uint32_t d = tmem + 2 * kTile + s * kDim, p = tmem + s * kTile;
-          const int steps = max(1, (keys + 15) / 16);
-          for (int i = 0; i < steps; i++)
-            mma_ts(d, p + i * 8, operand(v + i * 2048, rows * 128, 1024), o_inst, j >= 2 || i > 0);
-          if (t > 0 && (!kWide || s == 1)) tmem_commit(smem_addr(&ctl.empty[slot]));
+          return true;
+        };
+        const auto outputs = [&](int j, auto group) {
+          constexpr int s = decltype(group)::value;
+          const int t = w.t0 + (kWide ? j >> 1 : j);
+          uint64_t vd = tv_desc;
+          int steps = max(1, (w.q.nodes + 15) / 16);
+          if (t > 0) {
+            if (!wait_alone(&ctl, &ctl.full[v_slot], v_turn & 1)) return false;
+            vd = v_desc + v_slot * (L::kSlot / 16);
+            steps = (min(kTile, w.q.len - (t - 1) * kTile) + 15) / 16;
+          }
+          if (!wait_alone(&ctl, &ctl.p_full[s], p_turn[s] & 1)) return false;
+          p_turn[s]++;
+          tmem_after();
+          constexpr uint32_t d = 2 * kTile + s * kDim, p = s * kTile;
+#pragma unroll
+          for (int i = 0; i < kTile / 16; i++)
+            if (i < steps) mma_ts(d, p + i * 8, vd + i * (2048 / 16), o_inst, j >= 2 || i > 0);
+          if (t > 0 && (!kWide || s == 1)) {
+            tmem_commit(smem_addr(&ctl.empty[v_slot]));
+            v_slot += 2;
+            if (v_slot >= slots) v_slot -= slots, v_turn++;
+          }
           if (j == n - 1) tmem_commit(smem_addr(&ctl.done));
+          return true;
+        };
+        const std::integral_constant<int, 0> even;
+        const std::integral_constant<int, 1> odd;
+        ok = wait_alone(&ctl, &ctl.q_full, segment & 1);
+        tmem_after();
+        ok = ok && scores(0, even);
+        if (n > 1) ok = ok && scores(1, odd);
+        for (int j = 0; ok && j < n; j += 2) {
+          ok = outputs(j, even);
+          if (j + 2 < n) ok = ok && scores(j + 2, even);
+          if (j + 1 < n) ok = ok && outputs(j + 1, odd);
+          if (j + 3 < n) ok = ok && scores(j + 3, odd);
         }
-        __syncwarp();
-        if (j + 2 < n) ok = scores(j + 2);
-      }
-      loaded += 2 * w.context_tiles();
-      segment++;
-    } while (ok && w.next(c, a));
-    if (!ok) {  // what was issued ends before the block does
-      if (lane == 0) tmem_commit(smem_addr(&ctl.drain));
-      __syncwarp();
-      const uint32_t at = smem_addr(&ctl.drain);
-      for (int poll = 0; poll < kWaitLimit && !__all_sync(~0u, bar_poll(at, 0)); poll++) {
+        segment++;
+      } while (ok && w.next(c, a));
+      if (!ok) {  // what was issued ends before the block does
+        tmem_commit(smem_addr(&ctl.drain));
+        wait_out(&ctl.drain, 0);
       }
     }
-  } else if (work) {
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    if (work) {
     // ---- softmax warps: a thread per row
     Walk<kRows> w;
     w.start(c, a, ctl.run_b, ctl.run_off, ctl.run_at);
@@ -511,66 +592,91 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
     const uint32_t s_at = tmem + lanes + g * kTile, o_at = tmem + lanes + 2 * kTile + g * kDim;
     const float cs = fmaxf(fabsf(a.scale) * kLog2e, 1.17549435e-38f);  // not 0: a masked -inf stays -inf
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0;  // scale's sign goes into Q
-    uint32_t loaded = 0, segment = 0, s_turn = 0, meets = 0;
+    uint32_t loaded = 0, segment = 0, s_turn = 0;
     bool ok = true;
     do {
       const int rows0 = w.block * kRows, rows = min(kRows, w.q.nodes * a.group - rows0);  // rows that are there
-      // Q, and with tile 0 the nodes' keys and values, which also go to the cache
-      if (rows > 0) {
-        for (int i = tid; i < rows * kChunks; i += 256) {
-          const int r = i / kChunks, ch = i % kChunks, node = (rows0 + r) / a.group, h = w.head * a.group + (rows0 + r) % a.group;
-          uint4 x = load8(a.q.p + w.b * a.q.row + node * a.q.node + h * a.q.head, ch * 8, c.head_dim, a.vec);
-          x.x ^= flip, x.y ^= flip, x.z ^= flip, x.w ^= flip;
-          const int rr = r & (kTile - 1);
-          *reinterpret_cast<uint4*>(smem + L::kQAt + (r / kTile) * (kTile * kDim * 2) + (ch >> 3) * (kTile * 128) + rr * 128 + ((ch ^ rr) & 7) * 16) = x;
+      // Q, and with tile 0 the nodes' keys and values: 8 loads of Q and all of the nodes are
+      // on their way before the first is used
+      constexpr int kTreeLoads = kTreeTile * kChunks / 256, kRowStep = 256 / kChunks;
+      const int ch = tid % kChunks, first_row = tid / kChunks;  // a thread keeps its column of chunks
+      const bool tree = w.t0 == 0;
+      uint4 xk[kTreeLoads], xv[kTreeLoads];
+#pragma unroll
+      for (int u = 0; u < kTreeLoads; u++) {
+        const int j = first_row + u * kRowStep;
+        xk[u] = xv[u] = make_uint4(0, 0, 0, 0);
+        if (tree && j < w.q.nodes) {
+          xk[u] = load8(a.k.p + w.b * a.k.row + j * a.k.node + w.head * a.k.head, ch * 8, c.head_dim, a.vec);
+          xv[u] = load8(a.v.p + w.b * a.v.row + j * a.v.node + w.head * a.v.head, ch * 8, c.head_dim, a.vec);
+        }
+      }
+      for (int r0 = first_row; r0 < rows; r0 += 8 * kRowStep) {
+        uint4 x[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+          const int r = r0 + u * kRowStep;
+          if (r < rows) {
+            const int node = divide(rows0 + r, a.group_inverse), h = w.head * a.group + rows0 + r - node * a.group;
+            x[u] = load8(a.q.p + w.b * a.q.row + node * a.q.node + h * a.q.head, ch * 8, c.head_dim, a.vec);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+          const int r = r0 + u * kRowStep, rr = r & (kTile - 1);
+          if (r < rows) {
+            x[u].x ^= flip, x[u].y ^= flip, x[u].z ^= flip, x[u].w ^= flip;
+            *reinterpret_cast<uint4*>(raw + q_at + (r / kTile) * q_tile + (ch >> 3) * q_block + rr * 128 + ((ch ^ rr) & 7) * 16) = x[u];
+          }
         }
       }
       if (tid == 0) ctl.odd[(segment + 1) % 3] = 0;
-      if (w.t0 == 0) {
-        const int room = w.q.nodes > 0 ? (__ldg(c.counts + w.q.slot) << c.page_log2) - w.q.len : 0;
-        const int keep = w.block == 0 ? min(w.q.nodes, room) : 0;
-        if (tid == 0 && w.block == 0 && w.head == 0 && w.q.nodes > room) atomicOr(c.status, kNotReserved);
-        for (int i = tid; i < kTreeTile * kChunks; i += 256) {
-          const int j = i / kChunks, ch = i % kChunks;
-          uint4 x = make_uint4(0, 0, 0, 0), y = x;
-          if (j < w.q.nodes) {
-            x = load8(a.k.p + w.b * a.k.row + j * a.k.node + w.head * a.k.head, ch * 8, c.head_dim, a.vec);
-            y = load8(a.v.p + w.b * a.v.row + j * a.v.node + w.head * a.v.head, ch * 8, c.head_dim, a.vec);
-            if (j < keep && ch * 8 < c.head_dim) {
-              const int pos = w.q.len + j;
-              const int64_t page = c.tables[static_cast<size_t>(w.q.slot) * c.width + (pos >> c.page_log2)] + static_cast<int64_t>(a.layer) * c.num_pages;
-              const int64_t at = (((page * c.kv_heads + w.head) << c.page_log2) + (pos & (c.page_size - 1))) * c.head_dim * 2 + ch * 16;
-              *reinterpret_cast<uint4*>(c.k + at) = x;
-              *reinterpret_cast<uint4*>(c.v + at) = y;
-            }
-            // a value that is not finite would reach every row as 0 * inf: it is taken
-            // out here and added to the rows that see it at the end
-            uint32_t ws[4] = {y.x, y.y, y.z, y.w};
-            bool odd = false;
+      if (tree) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-              if (not_finite<kBf16>(ws[e] & 0xffff)) ws[e] &= 0xffff0000u, odd = true;
-              if (not_finite<kBf16>(ws[e] >> 16)) ws[e] &= 0xffffu, odd = true;
-            }
-            if (odd) {
-              atomicOr(reinterpret_cast<unsigned long long*>(&ctl.odd[segment % 3]), 1ull << j);
-              y = make_uint4(ws[0], ws[1], ws[2], ws[3]);
-            }
+        for (int u = 0; u < kTreeLoads; u++) {
+          const int j = first_row + u * kRowStep;
+          if (j >= a.tree_rows) continue;
+          // a value that is not finite would reach every row as 0 * inf: it is taken out
+          // here and added to the rows that see it at the end
+          uint32_t ws[4] = {xv[u].x, xv[u].y, xv[u].z, xv[u].w};
+          bool odd = false;
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            if (not_finite<kBf16>(ws[e] & 0xffff)) ws[e] &= 0xffff0000u, odd = true;
+            if (not_finite<kBf16>(ws[e] >> 16)) ws[e] &= 0xffffu, odd = true;
           }
-          const int at = (ch >> 3) * (kTreeTile * 128) + j * 128 + ((ch ^ j) & 7) * 16;
-          *reinterpret_cast<uint4*>(smem + L::kTreeK + at) = x;
-          *reinterpret_cast<uint4*>(smem + L::kTreeV + at) = y;
+          if (odd) atomicOr(reinterpret_cast<unsigned long long*>(&ctl.odd[segment % 3]), 1ull << j);
+          const int at = (ch >> 3) * tree_block + j * 128 + ((ch ^ j) & 7) * 16;
+          *reinterpret_cast<uint4*>(raw + tk_at + at) = xk[u];
+          *reinterpret_cast<uint4*>(raw + tv_at + at) = make_uint4(ws[0], ws[1], ws[2], ws[3]);
         }
       }
       fence_async();
       warp_arrive(&ctl.q_full);
+      if (tree && w.block == 0 && w.q.nodes > 0) {  // the nodes' keys and values go to the cache
+        const int room = (c.counts[w.q.slot] << c.page_log2) - w.q.len, keep = min(w.q.nodes, room);
+        if (tid == 0 && w.head == 0 && w.q.nodes > room) atomicOr(c.status, kNotReserved);
+        if (ch * 8 < c.head_dim) {
+#pragma unroll
+          for (int u = 0; u < kTreeLoads; u++) {
+            const int j = first_row + u * kRowStep, pos = w.q.len + j;
+            if (j < keep) {
+              const int64_t page = c.tables[static_cast<size_t>(w.q.slot) * c.width + (pos >> c.page_log2)] + static_cast<int64_t>(a.layer) * c.num_pages;
+              const int64_t at = (((page * c.kv_heads + w.head) << c.page_log2) + (pos & (c.page_size - 1))) * c.head_dim * 2 + ch * 16;
+              *reinterpret_cast<uint4*>(c.k + at) = xk[u];
+              *reinterpret_cast<uint4*>(c.v + at) = xv[u];
+            }
+          }
+        }
+      }
+      __syncwarp();
 
       const int r = row + (kWide ? g * kTile : 0);
       const bool mine = r < rows, any = (r & ~31) < rows;  // this row, this warp's rows are there
-      const int node = mine ? (rows0 + r) / a.group : 0, h = w.head * a.group + (mine ? (rows0 + r) % a.group : 0);
+      const int node = mine ? divide(rows0 + r, a.group_inverse) : 0, h = w.head * a.group + (mine ? rows0 + r - node * a.group : 0);
       uint64_t sees = 0;
       if (mine && w.t0 == 0) {
-        sees = a.masks ? __ldg(reinterpret_cast<const unsigned long long*>(a.masks) + static_cast<int64_t>(w.b) * a.nodes + node) : ~0ull >> (63 - node);
+        sees = a.masks ? a.masks[static_cast<int64_t>(w.b) * a.nodes + node] : ~0ull >> (63 - node);
         if (w.q.nodes < 64) sees &= (1ull << w.q.nodes) - 1;
       }
       float t_ref = -INFINITY, sum = 0.0f;
@@ -647,13 +753,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
         if (t > 0 && keys < kTile) {
           // the rows of V past the sequence's end that the last 16-key step reads are
           // not its tokens: zeros in their place
-          const uint32_t e = loaded + 2 * (t - max(w.t0, 1)) + 1, slot = e % L::kSlots;
-          ok = wait(&ctl, &ctl.full[slot], (e / L::kSlots) & 1);
+          const uint32_t e = loaded + 2 * (t - max(w.t0, 1)) + 1, slot = e % a.slots;
+          ok = wait(&ctl, &ctl.full[slot], (e / a.slots) & 1);
           if (!ok) break;
           const int end = (keys + 15) & ~15;
           for (int i = row; i < (end - keys) * kChunks; i += kTile) {
             const int j = keys + i / kChunks, ch = i % kChunks;
-            *reinterpret_cast<uint4*>(smem + L::kRing + slot * L::kSlot + (ch >> 3) * (kTile * 128) + j * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(raw + ring_at + slot * L::kSlot + (ch >> 3) * (kTile * 128) + j * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_async();
         }
@@ -669,64 +775,43 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
       constexpr int kMine = kWide ? kDim : kDim / 2;  // columns that this thread writes
       const int col0 = kWide ? 0 : g * kMine;
       const bool whole = w.t0 == 0 && w.t1 == w.tiles;
-      const bool two = !kWide && w.t1 - w.t0 > 1;     // both groups had tiles
-      float f_mine = 1.0f, f_other = 0.0f;
-      const float* other = nullptr;
+      float f0 = 1.0f, f1 = 0.0f;  // factors of the first and the second group's O
       if (!kWide) {
-        // each group hands the other its half of the columns, [column][row]; the space of
-        // Q and the tree is free until the next segment
-        float* give = reinterpret_cast<float*>(smem + L::kQAt) + (g ^ 1) * (kMine * kTile);
-        other = reinterpret_cast<const float*>(smem + L::kQAt) + g * (kMine * kTile);
+        // both groups' threads of a row can read both O: each writes half the columns
         ctl.sums[g][0][row] = t_ref;
         ctl.sums[g][1][row] = sum;
-        if (any && (two || g == 0)) {
-#pragma unroll 1
-          for (int i = 0; i < kMine; i += 32) {
-            uint32_t o[32];
-            __syncwarp();
-            tmem_load32(o_at + (g ^ 1) * kMine + i, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; e++) give[(i + e) * kTile + row] = __uint_as_float(o[e]);
-          }
-        }
         warp_arrive(&ctl.meet);
-        ok = wait(&ctl, &ctl.meet, meets++ & 1);
+        ok = wait(&ctl, &ctl.meet, segment & 1);
         if (!ok) break;
-        const float t2 = ctl.sums[g ^ 1][0][row], sum2 = ctl.sums[g ^ 1][1][row];
-        const float t_all = fmaxf(t_ref, t2);
-        f_mine = weight(t_ref, sum, t_all);
-        f_other = weight(t2, sum2, t_all);
-        // in group order in both groups, so that both write the same sum
-        sum = g == 0 ? sum * f_mine + sum2 * f_other : sum2 * f_other + sum * f_mine;
-        t_ref = t_all;
+        const float ta = ctl.sums[0][0][row], tb = ctl.sums[1][0][row], sa = ctl.sums[0][1][row], sb = ctl.sums[1][1][row];
+        t_ref = fmaxf(ta, tb);
+        f0 = weight(ta, sa, t_ref);
+        f1 = weight(tb, sb, t_ref);
+        sum = sa * f0 + sb * f1;
       }
       if (any) {
         const int64_t at = (static_cast<int64_t>(w.b) * a.nodes + node) * a.q_heads + h;
         const uint64_t odd = w.t0 == 0 ? ctl.odd[segment % 3] & sees : 0;
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        float* part = a.partial + ((static_cast<int64_t>(blockIdx.x) * 2 + (w.first ? 0 : 1)) * kRows + r) * (kDim + 2);
+        float* part = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (w.first ? 0 : 1)) * part_floats<kDim, kRows>();
+        const bool one = kWide || w.t1 - w.t0 == 1;  // only one group had tiles
 #pragma unroll 1
         for (int i = 0; i < kMine; i += 32) {
-          uint32_t o[32];
           const int col = col0 + i;
-          __syncwarp();
-          if (kWide || two || g == 0) {
-            tmem_load32(o_at + col, o);
-            tmem_wait_ld();
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; e++) o[e] = 0;
-          }
           float x[32];
+          {
+            uint32_t o[32];
+            __syncwarp();
+            tmem_load32(kWide ? o_at + col : tmem + lanes + 2 * kTile + col, o);
+            tmem_wait_ld();
+            // a factor of 0 must not meet what an unused accumulator holds
 #pragma unroll
-          for (int e = 0; e < 32; e++) x[e] = __uint_as_float(o[e]);
-          if (!kWide) {
+            for (int e = 0; e < 32; e++) x[e] = kWide ? __uint_as_float(o[e]) : f0 == 0.0f ? 0.0f : __uint_as_float(o[e]) * f0;
+            if (!one) {
+              tmem_load32(tmem + lanes + 2 * kTile + kDim + col, o);
+              tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; e++) {
-              const float y = (two || g == 1) ? other[(i + e) * kTile + row] : 0.0f;
-              // a factor of 0 must not meet what an unused accumulator holds
-              x[e] = (f_mine == 0.0f ? 0.0f : x[e] * f_mine) + (f_other == 0.0f ? 0.0f : y * f_other);
+              for (int e = 0; e < 32; e++) x[e] += f1 == 0.0f ? 0.0f : __uint_as_float(o[e]) * f1;
             }
           }
           if (odd) {  // rare: the values that were taken out
@@ -747,15 +832,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
                   out[e / 8] = make_uint4(pack<kBf16>(x[e] * inv, x[e + 1] * inv), pack<kBf16>(x[e + 2] * inv, x[e + 3] * inv), pack<kBf16>(x[e + 4] * inv, x[e + 5] * inv),
                                           pack<kBf16>(x[e + 6] * inv, x[e + 7] * inv));
             } else {
-              float2* to = reinterpret_cast<float2*>(part + col);
+              float4* to = reinterpret_cast<float4*>(part) + (col / 4) * kRows + r;
 #pragma unroll
-              for (int e = 0; e < 32; e += 2) to[e / 2] = make_float2(x[e], x[e + 1]);
+              for (int e = 0; e < 32; e += 4) to[e / 4 * kRows] = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
             }
           }
         }
         if (mine && (kWide || g == 0)) {
-          if (!whole) *reinterpret_cast<float2*>(part + kDim) = make_float2(t_ref, sum);
-          else if (a.out_lse) a.out_lse[at] = sum == 0.0f ? -INFINITY : static_cast<float>(static_cast<double>(t_ref) * 0.6931471805599453 + log(static_cast<double>(sum)));
+          if (!whole) reinterpret_cast<float2*>(part + kDim * kRows)[r] = make_float2(t_ref, sum);
+          else if (a.out_lse) a.out_lse[at] = log_sum(t_ref, sum);
         }
       }
       if (w.t0 == 0) {  // rows of nodes that are not there: zeros
@@ -768,87 +853,106 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
         }
       }
       tmem_before();  // O has been read before the next segment's first product writes it
-      if (!kWide) {   // and the space of Q before the next segment's Q
-        warp_arrive(&ctl.meet);
-        ok = wait(&ctl, &ctl.meet, meets++ & 1);
-      }
+      __syncwarp();
       segment++;
     } while (ok && w.next(c, a));
+    }
   }
   __syncwarp();
   tmem_before();
   __syncthreads();
   if (tid == 0 && ctl.give_up) atomicOr(c.status, kGaveUp);
-  if (warp == 9) {
+  __syncwarp();
+  if (warp == 1) {
     tmem_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(ctl.tmem));
   }
 }
 
-// Joins the rows of items that runs cut.  Block x is the cut between runs x and x + 1;
-// the first cut inside an item does the item, a warp per row.
+// Joins the rows of items that runs cut: a thread per row and 4 columns, a warp per 32
+// rows, so that parts are read in whole lines.  Block x is an item when there are few
+// (by_item), else the cut between runs x and x + 1, and the first cut inside an item
+// does the item.  y: 32 rows, z: 32 columns.
 template <int kDim, bool kWide, bool kBf16>
 __global__ void __launch_bounds__(256) join_kernel(CacheView c, TreeArgs a) {
-  constexpr int kRows = Layout<kDim, kWide>::kRows, kPer = kDim / 32;
+  constexpr int kRows = Layout<kDim, kWide>::kRows;
   after_previous_work();
-  const int64_t total = a.starts[a.n], run = a.starts[a.n + 1], cut = run * (blockIdx.x + 1);
-  if (cut >= total) return;
-  int lo = 0, hi = a.n - 1;  // the sequence that holds the cut
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.starts[mid] <= cut) lo = mid; else hi = mid - 1;
-  }
+  const int64_t total = a.starts[a.n], run = a.starts[a.n + 1];
   Walk<kRows> w;
-  w.start(c, a, lo, cut - a.starts[lo], 1);
-  const int64_t begin = cut - w.t0, end = begin + w.tiles;  // the item's tiles
-  if (w.t0 == 0 || cut - run > begin) return;               // not inside an item, or not the first cut in it
-  const int64_t first = begin / run, last = (end - 1) / run;
-  const int rows0 = w.block * kRows, rows = min(kRows, w.q.nodes * a.group - rows0);
-  const int lane = threadIdx.x & 31;
-  for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 8) {
-    // the item is the second segment of its first run unless the run starts with it
-    const auto part = [&](int64_t x) { return a.partial + ((x * 2 + (x == first && begin % run != 0 ? 1 : 0)) * kRows + r) * (kDim + 2); };
-    float t = -INFINITY;
-    for (int64_t x = first + lane; x <= last; x += 32) t = fmaxf(t, __ldcg(part(x) + kDim));
-    for (int d = 16; d; d >>= 1) t = fmaxf(t, __shfl_xor_sync(~0u, t, d));
-    float sum = 0.0f, o[kPer] = {};
-    for (int64_t x = first; x <= last; x++) {
-      const float* p = part(x);
-      const float2 ts = __ldcg(reinterpret_cast<const float2*>(p + kDim));
-      const float f = weight(ts.x, ts.y, t);
-      sum += f == 0.0f ? 0.0f : f * ts.y;
-#pragma unroll
-      for (int e = 0; e < kPer; e += 2) {
-        const float2 y = __ldcg(reinterpret_cast<const float2*>(p + lane * 2 + e * 32));
-        o[e] += f == 0.0f ? 0.0f : f * y.x;
-        o[e + 1] += f == 0.0f ? 0.0f : f * y.y;
-      }
+  int64_t begin;
+  if (a.by_item) {
+    const int per = c.kv_heads * a.blocks, b = blockIdx.x / per, i = blockIdx.x % per;
+    w.q = sequence<kRows>(c, a, b);
+    w.b = b;
+    w.head = i / a.blocks;
+    w.block = i % a.blocks;
+    w.tiles = w.block < w.q.active ? w.q.ctx + 1 : 1;
+    begin = a.starts[b] + static_cast<int64_t>(w.head) * w.q.per_head + min(w.block, w.q.active) * static_cast<int64_t>(w.q.ctx + 1) + max(0, w.block - w.q.active);
+  } else {
+    const int64_t cut = run * (blockIdx.x + 1);
+    if (cut >= total) return;
+    int lo = 0, hi = a.n - 1;  // the sequence that holds the cut
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (a.starts[mid] <= cut) lo = mid; else hi = mid - 1;
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int q = rows0 + r;
-    const int64_t at = (static_cast<int64_t>(w.b) * a.nodes + q / a.group) * a.q_heads + w.head * a.group + q % a.group;
-#pragma unroll
-    for (int e = 0; e < kPer; e += 2) {
-      const int col = lane * 2 + e * 32;
-      if (col < c.head_dim) *reinterpret_cast<uint32_t*>(a.out + at * c.head_dim + col) = pack<kBf16>(o[e] * inv, o[e + 1] * inv);
-    }
-    if (lane == 0 && a.out_lse) a.out_lse[at] = sum == 0.0f ? -INFINITY : static_cast<float>(static_cast<double>(t) * 0.6931471805599453 + log(static_cast<double>(sum)));
+    w.start(c, a, lo, cut - a.starts[lo], 1);
+    begin = cut - w.t0;
+    if (w.t0 == 0 || cut - run > begin) return;  // not inside an item, or not the first cut in it
   }
+  const int64_t first = begin / run, last = (begin + w.tiles - 1) / run;
+  if (first == last) return;  // whole
+  const int rows0 = w.block * kRows, rows = min(kRows, w.q.nodes * a.group - rows0);
+  const int r = blockIdx.y * 32 + (threadIdx.x & 31), col4 = blockIdx.z * 8 + (threadIdx.x >> 5);
+  if (r >= rows || col4 * 4 >= c.head_dim) return;
+  // the item is the second segment of its first run unless the run starts with it
+  const auto part = [&](int64_t x) { return a.partial + (x * 2 + (x == first && begin % run != 0 ? 1 : 0)) * part_floats<kDim, kRows>(); };
+  const auto stats = [&](int64_t x) { return __ldcg(reinterpret_cast<const float2*>(part(x) + kDim * kRows) + r); };
+  float t = -INFINITY;
+#pragma unroll 4
+  for (int64_t x = first; x <= last; x++) t = fmaxf(t, stats(x).x);
+  float sum = 0.0f;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+  for (int64_t x = first; x <= last; x++) {
+    const float2 ts = stats(x);
+    const float4 y = __ldcg(reinterpret_cast<const float4*>(part(x)) + col4 * kRows + r);
+    const float f = weight(ts.x, ts.y, t);
+    if (f != 0.0f) {
+      sum += f * ts.y;
+      o.x += f * y.x, o.y += f * y.y, o.z += f * y.z, o.w += f * y.w;
+    }
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const int q = rows0 + r, node = divide(q, a.group_inverse);
+  const int64_t at = (static_cast<int64_t>(w.b) * a.nodes + node) * a.q_heads + w.head * a.group + q - node * a.group;
+  *reinterpret_cast<uint2*>(a.out + at * c.head_dim + col4 * 4) = make_uint2(pack<kBf16>(o.x * inv, o.y * inv), pack<kBf16>(o.z * inv, o.w * inv));
+  if (col4 == 0 && a.out_lse) a.out_lse[at] = log_sum(t, sum);
 }
 
-template <int kDim, bool kWide>
-constexpr size_t block_smem() { return kControl + Layout<kDim, kWide>::kBytes; }
+constexpr int kMaxSmem = 227 * 1024;
 
 template <int kDim, bool kWide, bool kBf16>
 cudaError_t allow_smem() {
-  return cudaFuncSetAttribute(tree_kernel<kDim, kWide, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(block_smem<kDim, kWide>()));
+  return cudaFuncSetAttribute(tree_kernel<kDim, kWide, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
 }
 
 template <int kDim, bool kWide, bool kBf16>
-cudaError_t launch(tg_cache* c, const TreeArgs& a, cudaStream_t st) {
-  cudaError_t e = launch_after(tree_kernel<kDim, kWide, kBf16>, dim3(c->sms), kThreads, block_smem<kDim, kWide>(), st, 1, c->view, a, c->k_map, c->v_map);
-  const int rows = a.nodes * a.group < Layout<kDim, kWide>::kRows ? a.nodes * a.group : Layout<kDim, kWide>::kRows;
-  if (e == cudaSuccess) e = launch_after(join_kernel<kDim, kWide, kBf16>, dim3(c->sms - 1, (rows + 15) / 16), 256, 0, st, 1, c->view, a);
+cudaError_t launch(tg_cache* c, TreeArgs a, cudaStream_t st) {
+  using L = Layout<kDim, kWide>;
+  const int rows = a.nodes * a.group < L::kRows ? a.nodes * a.group : L::kRows;
+  a.q_rows = kWide ? kTile : (rows + 7) & ~7;
+  a.tree_rows = (a.nodes + 15) & ~15;
+  const int fixed = kControl + (kWide ? 2 : 1) * a.q_rows * kDim * 2 + 2 * a.tree_rows * kDim * 2;
+  a.slots = (kMaxSmem - fixed) / L::kSlot;
+  if (a.slots > kMaxSlots) a.slots = kMaxSlots;
+  // the last row block's 128 rows, read from its start, end inside the block's memory:
+  // at least 4 slots of 128 rows follow it
+  cudaError_t e = launch_after(tree_kernel<kDim, kWide, kBf16>, dim3(c->sms), kThreads, fixed + a.slots * L::kSlot, st, 1, c->view, a, c->k_map, c->v_map);
+  const int64_t items = static_cast<int64_t>(a.n) * c->view.kv_heads * a.blocks;
+  a.by_item = items < c->sms;
+  const dim3 grid(static_cast<unsigned>(a.by_item ? items : c->sms - 1), (rows + 31) / 32, kDim / 32);
+  if (e == cudaSuccess) e = launch_after(join_kernel<kDim, kWide, kBf16>, grid, 256, 0, st, 1, c->view, a);
   return e;
 }
 
@@ -860,7 +964,7 @@ cudaError_t launch_dim(tg_cache* c, const TreeArgs& a, bool wide, cudaStream_t s
 }
 
 // Starts of the sequences, then the partial rows of every block's two cut items.
-constexpr size_t kStartBytes = (65535 + 2 + 64) * sizeof(int64_t);
+constexpr size_t kStartBytes = (65536 + 64) * sizeof(int64_t);
 constexpr size_t partial_bytes(int sms) { return static_cast<size_t>(sms) * 2 * 2 * kTile * (128 + 2) * sizeof(float); }
 
 }  // namespace
@@ -910,7 +1014,7 @@ int32_t tg_tree_attention(tg_cache* c, int32_t layer, int32_t n, const int32_t* 
   if (layer < 0 || layer >= c->view.layers) return set_error(TG_ERR_INVALID_ARG, "layer outside [0, layers)");
   if (nodes < 1 || nodes > TG_MAX_TREE_NODES) return set_error(TG_ERR_UNSUPPORTED, "nodes outside [1, TG_MAX_TREE_NODES]");
   if (q_heads <= 0 || q_heads % c->view.kv_heads) return set_error(TG_ERR_INVALID_ARG, "q_heads must be a multiple of kv_heads");
-  if (q_heads / c->view.kv_heads > 4096) return set_error(TG_ERR_UNSUPPORTED, "more than 4096 query heads per key head");
+  if (q_heads / c->view.kv_heads > 256) return set_error(TG_ERR_UNSUPPORTED, "more than 256 query heads per key head");
   if (!std::isfinite(scale)) return set_error(TG_ERR_INVALID_ARG, "scale must be finite");
   if (n == 0) return TG_OK;
   if (!seqs || !q || !k || !v || !out) return set_error(TG_ERR_INVALID_ARG, "seqs, q, k, v and out are required");
@@ -922,6 +1026,7 @@ int32_t tg_tree_attention(tg_cache* c, int32_t layer, int32_t n, const int32_t* 
   a.nodes = nodes;
   a.q_heads = q_heads;
   a.group = q_heads / c->view.kv_heads;
+  a.group_inverse = a.group == 1 ? 0 : static_cast<uint32_t>(((1ull << 32) + a.group - 1) / a.group);
   const bool wide = nodes * a.group > tg::kTile;  // more rows than one block of the tensor cores takes
   const int rows = wide ? 2 * tg::kTile : tg::kTile;
   a.blocks = (nodes * a.group + rows - 1) / rows;
