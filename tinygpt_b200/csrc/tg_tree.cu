@@ -39,7 +39,7 @@
 namespace tg {
 namespace {
 
-constexpr int kThreads = 384;    // 8 softmax warps, a loading warp, an issuing warp, 2 without work
+constexpr int kThreads = 384;    // 8 softmax warps, a loading, an issuing and a walking warp, one without work
 constexpr int kTile = 128;       // cached tokens of a tile, rows of a row block
 constexpr int kTreeTile = TG_MAX_TREE_NODES;
 constexpr int kWaitLimit = 1 << 24;
@@ -132,6 +132,11 @@ __device__ __forceinline__ void tmem_commit(uint32_t bar) {
 // 32 columns of this warp's 32 lanes, a lane per thread.
 __device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t* v) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 " TG_REGS32 ", [%32];" : TG_R32(v, 0) : "r"(at));
+}
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(at)
+               : "memory");
 }
 __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t* v) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], " TG_REGS32 ";" ::TG_I32(v, 0), "r"(at) : "memory");
@@ -246,7 +251,6 @@ struct Walk {
     place();
     return true;
   }
-  __device__ int context_tiles() const { return t1 - max(t0, 1); }
 };
 
 // ---- shared memory ----------------------------------------------------------------------
@@ -268,12 +272,23 @@ constexpr int kMaxSlots = 12;
 template <int kDim, int kRows>
 __device__ __forceinline__ constexpr int part_floats() { return kRows * (kDim + 2); }
 
+// A run of tiles of one item, as the walking warp hands it to the others.
+struct Segment {
+  int32_t b, head, block;         // the item
+  int32_t t0, t1, tiles;          // [t0, t1) of the item's tiles
+  int32_t slot, len, nodes;       // the sequence
+  int32_t first, last;            // the run's first, last segment
+};
+constexpr int kSegments = 3;      // handed over ahead
+
 struct Control {
   uint64_t full[kMaxSlots], empty[kMaxSlots], q_full, s_full[2], p_full[2], done, meet, drain;
+  uint64_t seg_full[kSegments], seg_empty[kSegments];
   uint64_t odd[3];  // nodes with a value that is not finite, by segment modulo 3
   float sums[2][2][kTile];  // join of the two groups: t and sum of each row
   int64_t scan[kThreads / 32 + 1];
   int64_t run_at, run_off;
+  Segment seg[kSegments];
   int32_t run_b, give_up;
   uint32_t tmem;
 };
@@ -350,6 +365,27 @@ __device__ __forceinline__ uint4 load8(const uint16_t* row, int col, int dim, bo
   return x;
 }
 
+// Scores of keys that a row does not see (their bit is clear): -inf.
+__device__ __forceinline__ void unseen(uint32_t* v, uint32_t seen) {
+  if (__all_sync(~0u, seen == ~0u)) return;
+#pragma unroll
+  for (int e = 0; e < 32; e++) v[e] = seen >> e & 1 ? v[e] : 0xff800000u;
+}
+
+template <int kDim>
+__device__ __forceinline__ void prefetch_row(const uint16_t* row) {
+#pragma unroll
+  for (int x = 0; x < kDim; x += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + x));
+}
+
+// A place in the queue of segments, and the parity of its phase.
+struct Turn {
+  uint32_t at = 0, phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++at == kSegments) at = 0, phase ^= 1;
+  }
+};
+
 // The factor of a part (t, sum) of a row in the whole: nothing where the part saw
 // nothing; NaN where all that it saw were NaN.
 __device__ __forceinline__ float weight(float t, float sum, float t_all) { return t == -INFINITY ? sum : exp2_fast(t - t_all); }
@@ -387,6 +423,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
     bar_init(smem_addr(&ctl.done), 1);
     bar_init(smem_addr(&ctl.meet), 8);
     bar_init(smem_addr(&ctl.drain), 1);
+    for (int i = 0; i < kSegments; i++) {
+      bar_init(smem_addr(&ctl.seg_full[i]), 1);
+      bar_init(smem_addr(&ctl.seg_empty[i]), 10);  // 8 softmax warps, the loading and the issuing warp
+    }
     ctl.odd[0] = ctl.odd[1] = ctl.odd[2] = 0;
     ctl.give_up = 0;
     ctl.run_b = -1;
@@ -455,41 +495,43 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
   const bool work = ctl.run_b >= 0 && ctl.tmem == tmem;
   if (ctl.tmem != tmem && tid == 0) ctl.give_up = 1;
 
-  // registers: 384 x 168 at launch = 256 x 208 (softmax) + 128 x 88 (the rest)
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (work && warp == 8) {
+  if (work && warp == 8) {
     // ---- loading warp: a lane per page of a tile
-    Walk<kRows> w;
-    w.start(c, a, ctl.run_b, ctl.run_off, ctl.run_at);
     const int box = min(c.page_size, kTile);  // tokens of a page in a tile
     uint32_t slot = 0, turn = 0;
-    bool ok = true;
-    do {
-      for (int t = max(w.t0, 1); ok && t < w.t1; t++) {
-        const int token = (t - 1) * kTile, here = min(kTile, w.q.len - token), n = (here + box - 1) / box;
+    int tiles = 0;
+    bool ok = true, last = false;
+    for (Turn k; ok && !last; k.next()) {
+      ok = wait(&ctl, &ctl.seg_full[k.at], k.phase);
+      if (!ok) break;
+      const Segment g = ctl.seg[k.at];
+      last = g.last;
+      for (int t = max(g.t0, 1); ok && t < g.t1; t++) {
+        const int token = (t - 1) * kTile, here = min(kTile, g.len - token), n = (here + box - 1) / box;
         int page = 0;
-        if (lane < n) page = c.tables[static_cast<size_t>(w.q.slot) * c.width + ((token + lane * box) >> c.page_log2)];
+        if (lane < n) page = c.tables[static_cast<size_t>(g.slot) * c.width + ((token + lane * box) >> c.page_log2)];
         const int z = a.layer * c.num_pages + page, y = (token + lane * box) & (c.page_size - 1);
-#pragma unroll
-        for (int kv = 0; kv < 2; kv++) {
-          if (turn > 0 && !wait(&ctl, &ctl.empty[slot], (turn - 1) & 1)) {
-            ok = false;
-            break;
-          }
+        // past the first tile the run's first Q goes before: behind a full ring of
+        // copies its loads would wait for all of them
+        if (g.first && ++tiles == 2) ok = wait(&ctl, &ctl.q_full, 0);
+#pragma unroll 1
+        for (int kv = 0; ok && kv < 2; kv++) {
+          if (turn > 0) ok = wait(&ctl, &ctl.empty[slot], (turn - 1) & 1);
+          if (!ok) break;
           const uint32_t bar = smem_addr(&ctl.full[slot]), to = base + ring_at + slot * L::kSlot;
           if (lane == 0) bar_expect(bar, n * box * L::kBlocks * 128);
           __syncwarp();
           if (lane < n) {
 #pragma unroll
             for (int x = 0; x < L::kBlocks; x++)
-              tma_load(to + x * (kTile * 128) + lane * box * 128, kv ? &v_map : &k_map, bar, x * 64, y, w.head, z);
+              tma_load(to + x * (kTile * 128) + lane * box * 128, kv ? &v_map : &k_map, bar, x * 64, y, g.head, z);
           }
           __syncwarp();
           if (++slot == static_cast<uint32_t>(a.slots)) slot = 0, turn++;
         }
       }
-    } while (ok && w.next(c, a));
+      warp_arrive(&ctl.seg_empty[k.at]);
+    }
     // on giving up, no copy may still be under way when the block ends
     if (lane == 0 && *reinterpret_cast<volatile int32_t*>(&ctl.give_up)) {
       for (uint32_t i = 0; i < static_cast<uint32_t>(a.slots); i++) {
@@ -497,28 +539,32 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
         if (loads > 0) wait_out(&ctl.full[i], (loads - 1) & 1);
       }
     }
-    } else if (work && warp == 9) {
+  } else if (work && warp == 9) {
     // ---- issuing lane: S = Q K^T two steps ahead of O += P V
     if (elect()) {
-      Walk<kRows> w;
-      w.start(c, a, ctl.run_b, ctl.run_off, ctl.run_at);
       constexpr uint32_t s_inst = instruction(kBf16, kTile, 0), o_inst = instruction(kBf16, kDim, 1);
       const uint32_t tree_inst = s_inst - (static_cast<uint32_t>((kTile - a.tree_rows) >> 3) << 17);
       const uint64_t q_desc = operand(base + q_at, 16, 1024), k_desc = operand(base + ring_at, 16, 1024), v_desc = operand(base + ring_at, kTile * 128, 1024),
                      tk_desc = operand(base + tk_at, 16, 1024), tv_desc = operand(base + tv_at, tree_block, 1024);
       const uint32_t slots = a.slots, q_step = q_block / 16, tree_step = tree_block / 16;
-      uint32_t k_slot = 0, k_turn = 0, v_slot = 1 % slots, v_turn = 0;  // the next keys and values in the ring
+      uint32_t k_slot = 0, k_turn = 0, v_slot = 1, v_turn = 0;  // the next keys and values in the ring
       uint32_t segment = 0, p_turn[2] = {0, 0};
-      bool ok = true;
-      do {
-        const int n = (w.t1 - w.t0) * (kWide ? 2 : 1);
+      bool ok = true, last = false;
+      for (Turn k; ok && !last; k.next()) {
+        ok = wait_alone(&ctl, &ctl.seg_full[k.at], k.phase);
+        if (!ok) break;
+        const int t0 = ctl.seg[k.at].t0, t1 = ctl.seg[k.at].t1, len = ctl.seg[k.at].len, nodes = ctl.seg[k.at].nodes;
+        last = ctl.seg[k.at].last;
+        const int n = (t1 - t0) * (kWide ? 2 : 1);
+        bool k_ready = false;  // the next keys were seen in the ring
         const auto scores = [&](int j, auto group) {
           constexpr int s = decltype(group)::value;
-          const int t = w.t0 + (kWide ? j >> 1 : j);
+          const int t = t0 + (kWide ? j >> 1 : j);
           const uint64_t qd = q_desc + (kWide ? s * (q_tile / 16) : 0);
           constexpr uint32_t d = s * kTile;
           if (t > 0) {
-            if (!wait_alone(&ctl, &ctl.full[k_slot], k_turn & 1)) return false;
+            if (!k_ready && !wait_alone(&ctl, &ctl.full[k_slot], k_turn & 1)) return false;
+            k_ready = kWide && s == 0;
             tmem_after();
             const uint64_t kd = k_desc + k_slot * (L::kSlot / 16);
 #pragma unroll
@@ -538,14 +584,16 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
         };
         const auto outputs = [&](int j, auto group) {
           constexpr int s = decltype(group)::value;
-          const int t = w.t0 + (kWide ? j >> 1 : j);
+          const int t = t0 + (kWide ? j >> 1 : j);
           uint64_t vd = tv_desc;
-          int steps = max(1, (w.q.nodes + 15) / 16);
+          int steps = max(1, (nodes + 15) / 16);
           if (t > 0) {
-            if (!wait_alone(&ctl, &ctl.full[v_slot], v_turn & 1)) return false;
+            if ((!kWide || s == 0) && !wait_alone(&ctl, &ctl.full[v_slot], v_turn & 1)) return false;
             vd = v_desc + v_slot * (L::kSlot / 16);
-            steps = (min(kTile, w.q.len - (t - 1) * kTile) + 15) / 16;
+            steps = (min(kTile, len - (t - 1) * kTile) + 15) / 16;
           }
+          // look for the next keys before P is there, not between its product and theirs
+          if (j + 2 < n && (!kWide || s == 0)) k_ready = bar_poll(smem_addr(&ctl.full[k_slot]), k_turn & 1);
           if (!wait_alone(&ctl, &ctl.p_full[s], p_turn[s] & 1)) return false;
           p_turn[s]++;
           tmem_after();
@@ -567,6 +615,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
         tmem_after();
         ok = ok && scores(0, even);
         if (n > 1) ok = ok && scores(1, odd);
+        k_ready = false;
         for (int j = 0; ok && j < n; j += 2) {
           ok = outputs(j, even);
           if (j + 2 < n) ok = ok && scores(j + 2, even);
@@ -574,28 +623,56 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
           if (j + 3 < n) ok = ok && scores(j + 3, odd);
         }
         segment++;
-      } while (ok && w.next(c, a));
+        if (ok) bar_arrive(smem_addr(&ctl.seg_empty[k.at]));
+      }
       if (!ok) {  // what was issued ends before the block does
         tmem_commit(smem_addr(&ctl.drain));
         wait_out(&ctl.drain, 0);
       }
     }
-    }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    if (work) {
-    // ---- softmax warps: a thread per row
+  } else if (work && warp == 10) {
+    // ---- walking warp: the run's segments, ahead of the others, and the first lines of
+    // what the softmax warps will load for them into L2
     Walk<kRows> w;
     w.start(c, a, ctl.run_b, ctl.run_off, ctl.run_at);
+    bool ok = true, more = true;
+    uint32_t used = 0;
+    for (Turn k; ok && more; k.next(), used++) {
+      if (used >= kSegments) ok = wait(&ctl, &ctl.seg_empty[k.at], k.phase ^ 1);
+      if (!ok) break;
+      if (lane == 0) {
+        ctl.seg[k.at] = Segment{w.b, w.head, w.block, w.t0, w.t1, w.tiles, w.q.slot, w.q.len, w.q.nodes, w.first, w.last};
+        bar_arrive(smem_addr(&ctl.seg_full[k.at]));
+      }
+      __syncwarp();
+      if (!w.first) {
+        const int rows0 = w.block * kRows, rows = min(kRows, w.q.nodes * a.group - rows0);
+        for (int r = lane; r < rows; r += 32) {
+          const int node = divide(rows0 + r, a.group_inverse), h = w.head * a.group + rows0 + r - node * a.group;
+          prefetch_row<kDim>(a.q.p + w.b * a.q.row + node * a.q.node + h * a.q.head);
+        }
+        if (w.t0 == 0)
+          for (int j = lane; j < w.q.nodes; j += 32) {
+            prefetch_row<kDim>(a.k.p + w.b * a.k.row + j * a.k.node + w.head * a.k.head);
+            prefetch_row<kDim>(a.v.p + w.b * a.v.row + j * a.v.node + w.head * a.v.head);
+          }
+      }
+      more = w.next(c, a);
+    }
+  } else if (work && warp < 8) {
+    // ---- softmax warps: a thread per row
     const int g = warp >> 2, row = tid & (kTile - 1);       // group, row of its row block
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
     const uint32_t s_at = tmem + lanes + g * kTile, o_at = tmem + lanes + 2 * kTile + g * kDim;
     const float cs = fmaxf(fabsf(a.scale) * kLog2e, 1.17549435e-38f);  // not 0: a masked -inf stays -inf
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0;  // scale's sign goes into Q
     uint32_t loaded = 0, segment = 0, s_turn = 0;
-    bool ok = true;
-    do {
-      const int rows0 = w.block * kRows, rows = min(kRows, w.q.nodes * a.group - rows0);  // rows that are there
+    bool ok = true, last = false;
+    for (Turn k; ok && !last; k.next()) {
+      ok = wait(&ctl, &ctl.seg_full[k.at], k.phase);
+      if (!ok) break;
+      const Segment& w = ctl.seg[k.at];  // read where it is needed: registers are for the scores
+      const int rows0 = w.block * kRows, rows = min(kRows, w.nodes * a.group - rows0);  // rows that are there
       // Q, and with tile 0 the nodes' keys and values: 8 loads of Q and all of the nodes are
       // on their way before the first is used
       constexpr int kTreeLoads = kTreeTile * kChunks / 256, kRowStep = 256 / kChunks;
@@ -606,7 +683,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
       for (int u = 0; u < kTreeLoads; u++) {
         const int j = first_row + u * kRowStep;
         xk[u] = xv[u] = make_uint4(0, 0, 0, 0);
-        if (tree && j < w.q.nodes) {
+        if (tree && j < w.nodes) {
           xk[u] = load8(a.k.p + w.b * a.k.row + j * a.k.node + w.head * a.k.head, ch * 8, c.head_dim, a.vec);
           xv[u] = load8(a.v.p + w.b * a.v.row + j * a.v.node + w.head * a.v.head, ch * 8, c.head_dim, a.vec);
         }
@@ -653,15 +730,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
       }
       fence_async();
       warp_arrive(&ctl.q_full);
-      if (tree && w.block == 0 && w.q.nodes > 0) {  // the nodes' keys and values go to the cache
-        const int room = (c.counts[w.q.slot] << c.page_log2) - w.q.len, keep = min(w.q.nodes, room);
-        if (tid == 0 && w.head == 0 && w.q.nodes > room) atomicOr(c.status, kNotReserved);
+      if (tree && w.block == 0 && w.nodes > 0) {  // the nodes' keys and values go to the cache
+        const int room = (c.counts[w.slot] << c.page_log2) - w.len, keep = min(w.nodes, room);
+        if (tid == 0 && w.head == 0 && w.nodes > room) atomicOr(c.status, kNotReserved);
         if (ch * 8 < c.head_dim) {
 #pragma unroll
           for (int u = 0; u < kTreeLoads; u++) {
-            const int j = first_row + u * kRowStep, pos = w.q.len + j;
+            const int j = first_row + u * kRowStep, pos = w.len + j;
             if (j < keep) {
-              const int64_t page = c.tables[static_cast<size_t>(w.q.slot) * c.width + (pos >> c.page_log2)] + static_cast<int64_t>(a.layer) * c.num_pages;
+              const int64_t page = c.tables[static_cast<size_t>(w.slot) * c.width + (pos >> c.page_log2)] + static_cast<int64_t>(a.layer) * c.num_pages;
               const int64_t at = (((page * c.kv_heads + w.head) << c.page_log2) + (pos & (c.page_size - 1))) * c.head_dim * 2 + ch * 16;
               *reinterpret_cast<uint4*>(c.k + at) = xk[u];
               *reinterpret_cast<uint4*>(c.v + at) = xv[u];
@@ -677,7 +754,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
       uint64_t sees = 0;
       if (mine && w.t0 == 0) {
         sees = a.masks ? a.masks[static_cast<int64_t>(w.b) * a.nodes + node] : ~0ull >> (63 - node);
-        if (w.q.nodes < 64) sees &= (1ull << w.q.nodes) - 1;
+        if (w.nodes < 64) sees &= (1ull << w.nodes) - 1;
       }
       float t_ref = -INFINITY, sum = 0.0f;
       const int step = kWide ? 1 : 2;
@@ -686,32 +763,26 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
         if (!ok) break;
         s_turn++;
         tmem_after();
-        const int keys = t > 0 ? min(kTile, w.q.len - (t - 1) * kTile) : kTreeTile;
+        const int keys = t > 0 ? min(kTile, w.len - (t - 1) * kTile) : kTreeTile;
         if (any) {
-          float top = -INFINITY;
-          uint32_t v[kTile];
+          // the scores are read from TMEM twice, 32 at a time: for their maximum and for
+          // their exponentials.  128 at once would not fit beside the rest in registers,
+          // and what spills is evicted from the little L1 that the ring leaves.
+          float m0 = -INFINITY, m1 = -INFINITY;
+          const int columns = t > 0 ? kTile : kTreeTile;
+#pragma unroll 1
+          for (int i = 0; i < columns; i += 32) {
+            uint32_t v[32];
+            tmem_load32(s_at + i, v);
+            tmem_wait_ld();
+            unseen(v, t == 0 ? static_cast<uint32_t>(sees >> i) : i + 32 <= keys ? ~0u : i < keys ? (1u << (keys - i)) - 1 : 0u);
 #pragma unroll
-          for (int i = 0; i < kTile; i += 32)
-            if (i < 64 || t > 0) tmem_load32(s_at + i, v + i);
-          tmem_wait_ld();
-          if (t == 0) {
-#pragma unroll
-            for (int i = 0; i < 64; i++) v[i] = sees >> i & 1 ? v[i] : 0xff800000u;
-#pragma unroll
-            for (int i = 64; i < kTile; i++) v[i] = 0xff800000u;
-          } else if (keys < kTile) {
-#pragma unroll
-            for (int i = 0; i < kTile; i++) v[i] = i < keys ? v[i] : 0xff800000u;
+            for (int e = 0; e < 32; e += 2) {
+              m0 = fmaxf(m0, __uint_as_float(v[e]));
+              m1 = fmaxf(m1, __uint_as_float(v[e + 1]));
+            }
           }
-          float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < kTile; i += 4) {
-            m0 = fmaxf(m0, __uint_as_float(v[i]));
-            m1 = fmaxf(m1, __uint_as_float(v[i + 1]));
-            m2 = fmaxf(m2, __uint_as_float(v[i + 2]));
-            m3 = fmaxf(m3, __uint_as_float(v[i + 3]));
-          }
-          top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * cs;
+          const float top = fmaxf(m0, m1) * cs;
           const bool begun = t >= w.t0 + step;  // O holds something
           const bool move = top > t_ref + kSlack;
           if (__any_sync(~0u, move)) {
@@ -731,23 +802,24 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
             }
           }
           const float t_use = t_ref == -INFINITY ? 0.0f : t_ref;
-          float a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
+          float a0 = 0.0f, a1 = 0.0f;
+#pragma unroll 1
+          for (int i = 0; i < columns; i += 32) {
+            uint32_t v[32];
+            tmem_load32(s_at + i, v);
+            tmem_wait_ld();
+            unseen(v, t == 0 ? static_cast<uint32_t>(sees >> i) : i + 32 <= keys ? ~0u : i < keys ? (1u << (keys - i)) - 1 : 0u);
+            uint32_t p[16];
 #pragma unroll
-          for (int i = 0; i < kTile; i += 64) {
-            uint32_t p[32];
-#pragma unroll
-            for (int e = 0; e < 64; e += 4) {
-              const float p0 = exp2_fast(__fmaf_rn(__uint_as_float(v[i + e]), cs, -t_use));
-              const float p1 = exp2_fast(__fmaf_rn(__uint_as_float(v[i + e + 1]), cs, -t_use));
-              const float p2 = exp2_fast(__fmaf_rn(__uint_as_float(v[i + e + 2]), cs, -t_use));
-              const float p3 = exp2_fast(__fmaf_rn(__uint_as_float(v[i + e + 3]), cs, -t_use));
-              a0 += p0, a1 += p1, a2 += p2, a3 += p3;
+            for (int e = 0; e < 32; e += 2) {
+              const float p0 = exp2_fast(__fmaf_rn(__uint_as_float(v[e]), cs, -t_use));
+              const float p1 = exp2_fast(__fmaf_rn(__uint_as_float(v[e + 1]), cs, -t_use));
+              a0 += p0, a1 += p1;
               p[e / 2] = pack<kBf16>(p0, p1);
-              p[e / 2 + 1] = pack<kBf16>(p2, p3);
             }
-            if (i == 0 || t > 0) tmem_store32(s_at + i / 2, p);
+            tmem_store16(s_at + i / 2, p);  // over scores already read
           }
-          sum += (a0 + a1) + (a2 + a3);
+          sum += a0 + a1;
           tmem_wait_st();
         }
         if (t > 0 && keys < kTile) {
@@ -769,7 +841,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
       ok = ok && wait(&ctl, &ctl.done, segment & 1);
       if (!ok) break;
       tmem_after();
-      loaded += 2 * w.context_tiles();
+      loaded += 2 * (w.t1 - max(w.t0, 1));
 
       // ---- the segment's end: join the groups, write the rows or leave them to be joined
       constexpr int kMine = kWide ? kDim : kDim / 2;  // columns that this thread writes
@@ -816,11 +888,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
           }
           if (odd) {  // rare: the values that were taken out
             for (uint64_t m = odd; m; m &= m - 1) {
-              const int j = __ffsll(m) - 1;
-              const uint16_t* vr = a.v.p + w.b * a.v.row + j * a.v.node + w.head * a.v.head;
+              const uint16_t* vr = a.v.p + w.b * a.v.row + (__ffsll(m) - 1) * a.v.node + w.head * a.v.head;
 #pragma unroll
-              for (int e = 0; e < 32; e++)
-                if (col + e < c.head_dim && not_finite<kBf16>(vr[col + e])) x[e] += widen<kBf16>(vr[col + e]);
+              for (int e = 0; e < 32; e++) {
+                const uint16_t y = col + e < c.head_dim ? vr[col + e] : 0;
+                if (not_finite<kBf16>(y)) x[e] += widen<kBf16>(y);
+              }
             }
           }
           if (mine) {
@@ -855,7 +928,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
       tmem_before();  // O has been read before the next segment's first product writes it
       __syncwarp();
       segment++;
-    } while (ok && w.next(c, a));
+      last = w.last;
+      warp_arrive(&ctl.seg_empty[k.at]);
     }
   }
   __syncwarp();
