@@ -39,7 +39,7 @@
 namespace tg {
 namespace {
 
-constexpr int kThreads = 384;    // 8 softmax warps, a loading, an issuing and a walking warp, one without work
+constexpr int kThreads = 512;    // 8 softmax warps, a TMA, an issuing and two loading warps, 4 that write results
 constexpr int kTile = 128;       // cached tokens of a tile, rows of a row block
 constexpr int kTreeTile = TG_MAX_TREE_NODES;
 constexpr int kWaitLimit = 1 << 24;
@@ -61,6 +61,7 @@ struct TreeArgs {
   uint32_t group_inverse;  // ceil(2^32 / group)
   int32_t q_rows, tree_rows, slots;  // shared memory: rows of a row block, of the nodes' tile, ring slots
   int32_t by_item;         // join_kernel: a block column per item, not per cut
+  int32_t run_blocks;      // blocks of tree_kernel's grid
   const int32_t* seqs;
   const int32_t* n_nodes;
   const uint64_t* masks;
@@ -68,8 +69,9 @@ struct TreeArgs {
   float scale;
   uint16_t* out;
   float* out_lse;
-  int64_t* starts;  // [n + 2] first tile of each sequence, all tiles, tiles of a run
-  float* partial;   // [blocks of the grid, 2] parts of items (see Part)
+  int64_t* total;          // all items' measure; for join_kernel, as starts
+  int64_t* starts;         // [n] where each sequence begins in it
+  float* partial;          // [runs, 2] parts of items (see part_floats)
 };
 
 // ---- PTX -----------------------------------------------------------------------------
@@ -133,11 +135,6 @@ __device__ __forceinline__ void tmem_commit(uint32_t bar) {
 __device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t* v) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 " TG_REGS32 ", [%32];" : TG_R32(v, 0) : "r"(at));
 }
-__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
-               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(at)
-               : "memory");
-}
 __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t* v) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], " TG_REGS32 ";" ::TG_I32(v, 0), "r"(at) : "memory");
 }
@@ -180,12 +177,21 @@ __device__ __forceinline__ float widen(uint16_t x) {
 
 // ---- the division of the work ---------------------------------------------------------
 
-// A sequence's part of the work.
+// Quotient of numbers that are nearly always below 2^32 (the 64-bit division is long).
+__device__ __noinline__ int64_t long_quotient(int64_t x, int64_t d) { return x / d; }
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t d) {
+  return ((x | d) >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(x) / static_cast<uint32_t>(d)) : long_quotient(x, d);
+}
+
+// A sequence's part of the work.  An item counts as its tiles and kOverhead more, for
+// what a block does once per item: runs are cut in this measure, so that a run of many
+// short items has as much to do as one of a few long ones.
+constexpr int kOverhead = 3;
 struct Seq {
   int slot, len, nodes;  // nodes 0 where the row cannot be served
   int ctx;               // tiles of cached tokens
   int active;            // row blocks with rows
-  int per_head;          // tiles of a key head
+  int per_head;          // measure of a key head's items
   uint32_t bad;
 };
 
@@ -201,63 +207,65 @@ __device__ __forceinline__ Seq sequence(const CacheView& c, const TreeArgs& a, i
   q.len = q.bad ? 0 : c.lens[q.slot];
   q.ctx = (q.len + kTile - 1) / kTile;
   q.active = (q.nodes * a.group + kRows - 1) / kRows;
-  q.per_head = q.active * (q.ctx + 1) + (a.blocks - q.active);
+  q.per_head = q.active * (q.ctx + 1 + kOverhead) + (a.blocks - q.active) * (1 + kOverhead);
   return q;
 }
 
-// A run of tiles of one item.
+// Walks over the segments of a run: over [t0, t1) of an item's tiles, item after item.
+// A segment may be empty, where a run's end falls into an item's overhead.
 template <int kRows>
 struct Walk {
-  int64_t left;  // tiles of the block's run from this segment on
-  int64_t off;   // this segment's first tile in the sequence's tiles
-  int b, head, block;
-  int t0, t1, tiles;  // [t0, t1) of the item's tiles
-  bool first, last;   // the run's first, last segment
+  int64_t left;  // what is left of the run from this item on
+  int64_t at;    // where the run enters the item, in the sequence's measure
+  int into;      // where in the item's measure that is
+  int b, head, block, tiles;
+  bool fresh;    // a sequence not looked at yet
   Seq q;
 
-  __device__ void start(const CacheView& c, const TreeArgs& a, int b0, int64_t off0, int64_t count) {
-    b = b0, off = off0, left = count, first = true;
-    q = sequence<kRows>(c, a, b);
-    place();
-  }
-  __device__ void place() {
-    head = static_cast<int>(off / q.per_head);
-    int r = static_cast<int>(off % q.per_head);
-    const int full = q.active * (q.ctx + 1);
+  __device__ __forceinline__ void start(int b0, int64_t at0, int64_t count) { b = b0, at = at0, left = count, fresh = true; }
+  // Fills in the item.
+  __device__ __forceinline__ void enter(const CacheView& c, const TreeArgs& a) {
+    if (fresh) q = sequence<kRows>(c, a, b);
+    fresh = false;
+    head = static_cast<int>(quotient(at, q.per_head));
+    int r = static_cast<int>(at - static_cast<int64_t>(head) * q.per_head);
+    const int full = q.active * (q.ctx + 1 + kOverhead);
     if (r < full) {
       tiles = q.ctx + 1;
-      block = r / tiles;
-      t0 = r % tiles;
+      block = static_cast<uint32_t>(r) / static_cast<uint32_t>(tiles + kOverhead);
+      into = r - block * (tiles + kOverhead);
     } else {
+      r -= full;
       tiles = 1;
-      block = q.active + r - full;
-      t0 = 0;
+      block = q.active + r / (1 + kOverhead);
+      into = r % (1 + kOverhead);
     }
-    const int64_t rest = tiles - t0;
-    t1 = t0 + static_cast<int>(rest < left ? rest : left);
-    last = left <= rest;
   }
-  __device__ bool next(const CacheView& c, const TreeArgs& a) {
-    const int n = t1 - t0;
-    if (last) return false;
-    left -= n;
-    off += n;
-    first = false;
-    if (off == static_cast<int64_t>(q.per_head) * c.kv_heads) {
-      off = 0;
-      b++;
-      q = sequence<kRows>(c, a, b);
-    }
-    place();
+  __device__ int t0() const { return max(0, into - kOverhead); }
+  __device__ int t1() const { return static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(tiles), into + left - kOverhead))); }
+  // To the next item of the run; false: there is none.
+  __device__ __forceinline__ bool advance(const CacheView& c) {
+    const int rest = tiles + kOverhead - into;
+    if (left <= rest) return false;
+    left -= rest;
+    at += rest;
+    if (at == static_cast<int64_t>(q.per_head) * c.kv_heads) b++, at = 0, fresh = true;
     return true;
   }
 };
 
+// The measure of a run.
+__device__ __forceinline__ int64_t run_length(int64_t total, int blocks, int min_tiles) {
+  const int64_t run = quotient(total + blocks - 1, blocks);
+  return run < min_tiles ? min_tiles : run;
+}
+
 // ---- shared memory ----------------------------------------------------------------------
 
-// In front the control block, then Q (each row block [64-column blocks][q_rows][128 bytes]),
-// the nodes' keys and values ([64-column blocks][tree_rows][128 bytes] each) and the ring
-// ([64-column blocks][128][128 bytes] per slot).  Q takes only the rows that the call
+// In front the control block, then Q (each row block [64-column blocks][q_rows][128 bytes])
+// and the nodes' keys and values ([64-column blocks][tree_rows][128 bytes] each), twice
+// where there is room (the next segment's are loaded while this one runs), and the
+// ring ([64-column blocks][128][128 bytes] per slot).  Q takes only the rows that the call
 // has: the products read 128 rows from its start, and what the rows past the last hold
 // reaches only results that nothing reads.  The space saved is ring: bytes in flight.
 template <int kDim, bool kWide>
@@ -265,8 +273,9 @@ struct Layout {
   static constexpr int kBlocks = kDim / 64;       // 64-column blocks of a row
   static constexpr int kSlot = kTile * kDim * 2;  // 128 keys or values
   static constexpr int kRows = kWide ? 2 * kTile : kTile;
+  static constexpr int kBuffers = kWide ? 1 : 2;  // of Q and the nodes
 };
-constexpr int kMaxSlots = 12;
+constexpr int kMaxSlots = 9;
 
 // A part of an item in the workspace: float4 o[kDim / 4][kRows], float2 (t, sum)[kRows].
 template <int kDim, int kRows>
@@ -274,26 +283,38 @@ __device__ __forceinline__ constexpr int part_floats() { return kRows * (kDim + 
 
 // A run of tiles of one item, as the walking warp hands it to the others.
 struct Segment {
-  int32_t b, head, block;         // the item
-  int32_t t0, t1, tiles;          // [t0, t1) of the item's tiles
+  int32_t b, head, block;         // the item; b < 0: there are no more
+  int32_t t0, t1;                 // [t0, t1) of the item's tiles
   int32_t slot, len, nodes;       // the sequence
-  int32_t first, last;            // the run's first, last segment
+  int32_t part;                   // the part that its rows make; -1: they are whole
 };
 constexpr int kSegments = 3;      // handed over ahead
 
 struct Control {
-  uint64_t full[kMaxSlots], empty[kMaxSlots], q_full, s_full[2], p_full[2], done, meet, drain;
+  uint64_t full[kMaxSlots], empty[kMaxSlots], q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], stats, done, read, drain;
   uint64_t seg_full[kSegments], seg_empty[kSegments];
-  uint64_t odd[3];  // nodes with a value that is not finite, by segment modulo 3
-  float sums[2][2][kTile];  // join of the two groups: t and sum of each row
-  int64_t scan[kThreads / 32 + 1];
-  int64_t run_at, run_off;
+  uint64_t odd[4][2];  // nodes with a value that is not finite, by segment modulo 4 and loading warp
+  int64_t total, run_off;
   Segment seg[kSegments];
   int32_t run_b, give_up;
   uint32_t tmem;
 };
-constexpr int kControl = 3072;  // its share of shared memory, in front of the 1024-byte-aligned tiles
-static_assert(sizeof(Control) <= kControl, "the control block outgrew its space");
+// After it, by Q buffer: the nodes' sets, and t and sum of each row in each group.  All in
+// front of the 1024-byte-aligned tiles, within 3 KB for a wide block, which leaves it 4
+// ring slots with 64 nodes.
+struct Sets {
+  uint64_t of[TG_MAX_TREE_NODES];
+};
+struct Sums {
+  float t[2][kTile], sum[2][kTile];
+};
+constexpr int kSetsAt = 512;
+static_assert(sizeof(Control) <= kSetsAt, "the control block outgrew its space");
+template <int kBuffers>
+__host__ __device__ constexpr int control_bytes() {
+  return (kSetsAt + kBuffers * static_cast<int>(sizeof(Sets) + sizeof(Sums)) + 1023) / 1024 * 1024;
+}
+static_assert(control_bytes<1>() == 3072, "a wide block's share");
 
 // A wait gives up after kWaitLimit polls or kWaitCycles cycles (about a second),
 // whichever is first.
@@ -306,23 +327,18 @@ struct Patience {
   }
 };
 
-// Waits for a phase, by a whole warp that stays together (its tcgen05 instructions need
-// that).  False: the block gives up (this wait or another took too long).
-__device__ __forceinline__ bool wait(Control* ctl, uint64_t* bar, uint32_t parity) {
-  const uint32_t at = smem_addr(bar), lane = threadIdx.x & 31;
+// The long way of the waits below.  Not inlined, like other rare paths here: the code of
+// all roles has to fit the instruction caches (at 140 KB everything ran half as fast).
+__device__ __noinline__ bool wait_on(Control* ctl, uint32_t at, uint32_t parity) {
+  const uint32_t lane = threadIdx.x & 31;
   for (Patience p;;) {
-    if (__any_sync(~0u, bar_poll_lane0(at, parity, lane))) {
-      __syncwarp();
-      return true;
-    }
+    if (__any_sync(~0u, bar_poll_lane0(at, parity, lane))) return true;
     if (__any_sync(~0u, *reinterpret_cast<volatile int32_t*>(&ctl->give_up) || p.over())) break;
   }
   *reinterpret_cast<volatile int32_t*>(&ctl->give_up) = 1;
   return false;
 }
-// The same by one lane.
-__device__ __forceinline__ bool wait_alone(Control* ctl, uint64_t* bar, uint32_t parity) {
-  const uint32_t at = smem_addr(bar);
+__device__ __noinline__ bool wait_on_alone(Control* ctl, uint32_t at, uint32_t parity) {
   for (Patience p;;) {
     if (bar_poll(at, parity)) return true;
     if (*reinterpret_cast<volatile int32_t*>(&ctl->give_up) || p.over()) break;
@@ -330,8 +346,21 @@ __device__ __forceinline__ bool wait_alone(Control* ctl, uint64_t* bar, uint32_t
   *reinterpret_cast<volatile int32_t*>(&ctl->give_up) = 1;
   return false;
 }
+
+// Waits for a phase, by a whole warp that stays together (its tcgen05 instructions need
+// that).  False: the block gives up (this wait or another took too long).
+__device__ __forceinline__ bool wait(Control* ctl, uint64_t* bar, uint32_t parity) {
+  const bool ok = wait_on(ctl, smem_addr(bar), parity);
+  __syncwarp();
+  return ok;
+}
+// The same by one lane.
+__device__ __forceinline__ bool wait_alone(Control* ctl, uint64_t* bar, uint32_t parity) {
+  const uint32_t at = smem_addr(bar);
+  return bar_poll(at, parity) || wait_on_alone(ctl, at, parity);
+}
 // For what is under way when a block gives up.
-__device__ __forceinline__ void wait_out(uint64_t* bar, uint32_t parity) {
+__device__ __noinline__ void wait_out(uint64_t* bar, uint32_t parity) {
   const uint32_t at = smem_addr(bar);
   for (Patience p; !bar_poll(at, parity) && !p.over();) {
   }
@@ -349,33 +378,27 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   if ((threadIdx.x & 31) == 0) bar_arrive(smem_addr(bar));
 }
 
+// 16 bytes to shared memory, asynchronously; zeros where `there` is false.
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+
 // 8 elements of a row from column `col` on, zeros past the head's dimension.
-__device__ __forceinline__ uint4 load8(const uint16_t* row, int col, int dim, bool vec) {
-  uint4 x = make_uint4(0, 0, 0, 0);
-  if (col < dim) {
-    if (vec) {
-      x = *reinterpret_cast<const uint4*>(row + col);
-    } else {
-      uint32_t w[4];
+__device__ __noinline__ uint4 load8_by_element(const uint16_t* row, int col) {
+  uint32_t w[4];
 #pragma unroll
-      for (int i = 0; i < 4; i++) w[i] = row[col + 2 * i] | static_cast<uint32_t>(row[col + 2 * i + 1]) << 16;
-      x = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  }
-  return x;
+  for (int i = 0; i < 4; i++) w[i] = row[col + 2 * i] | static_cast<uint32_t>(row[col + 2 * i + 1]) << 16;
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 load8(const uint16_t* row, int col, int dim, bool vec) {
+  if (col >= dim) return make_uint4(0, 0, 0, 0);
+  return vec ? *reinterpret_cast<const uint4*>(row + col) : load8_by_element(row, col);
 }
 
 // Scores of keys that a row does not see (their bit is clear): -inf.
 __device__ __forceinline__ void unseen(uint32_t* v, uint32_t seen) {
-  if (__all_sync(~0u, seen == ~0u)) return;
 #pragma unroll
   for (int e = 0; e < 32; e++) v[e] = seen >> e & 1 ? v[e] : 0xff800000u;
-}
-
-template <int kDim>
-__device__ __forceinline__ void prefetch_row(const uint16_t* row) {
-#pragma unroll
-  for (int x = 0; x < kDim; x += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + x));
 }
 
 // A place in the queue of segments, and the parity of its phase.
@@ -385,6 +408,21 @@ struct Turn {
     if (++at == kSegments) at = 0, phase ^= 1;
   }
 };
+
+// Adds the values that are not finite of the nodes in `seen` to a row that was written:
+// to its result, or (out null) to its part, 4 columns at each `stride`.
+template <bool kBf16>
+__device__ __noinline__ void add_odd(const uint16_t* v, int64_t v_node, uint64_t seen, int dim, uint16_t* out, float* part, int stride) {
+  for (; seen; seen &= seen - 1) {
+    const uint16_t* row = v + (__ffsll(seen) - 1) * v_node;
+    for (int d = 0; d < dim; d++)
+      if (not_finite<kBf16>(row[d])) {
+        const float y = widen<kBf16>(row[d]);
+        if (out) out[d] = static_cast<uint16_t>(pack<kBf16>(widen<kBf16>(out[d]) + y, 0.0f));
+        else part[(d >> 2) * stride + (d & 3)] += y;
+      }
+  }
+}
 
 // The factor of a part (t, sum) of a row in the whole: nothing where the part saw
 // nothing; NaN where all that it saw were NaN.
@@ -401,8 +439,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
   constexpr int kRows = L::kRows, kChunks = kDim / 8;
   extern __shared__ __align__(1024) uint8_t raw[];
   Control& ctl = *reinterpret_cast<Control*>(raw);
+  Sets* sets = reinterpret_cast<Sets*>(raw + kSetsAt);
+  Sums* sums = reinterpret_cast<Sums*>(raw + kSetsAt + L::kBuffers * sizeof(Sets));
+  int64_t* scan = reinterpret_cast<int64_t*>(sums);  // before the roles begin
+  constexpr int kBuffers = L::kBuffers;
   const uint32_t q_block = a.q_rows * 128, q_tile = L::kBlocks * q_block, tree_block = a.tree_rows * 128;  // bytes
-  const uint32_t q_at = kControl, tk_at = q_at + (kWide ? 2 : 1) * q_tile, tv_at = tk_at + L::kBlocks * tree_block, ring_at = tv_at + L::kBlocks * tree_block;
+  const uint32_t q_at = control_bytes<L::kBuffers>(), tk_at = q_at + (kWide ? 2 : 1) * q_tile, tv_at = tk_at + L::kBlocks * tree_block;
+  const uint32_t q_size = tv_at + L::kBlocks * tree_block - q_at, ring_at = q_at + kBuffers * q_size;  // of a buffer: Q and the nodes
   const uint32_t base = smem_addr(raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (base & 1023) {  // the swizzle needs it; shared memory starts on such a boundary
@@ -415,19 +458,21 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
       bar_init(smem_addr(&ctl.full[i]), 1);
       bar_init(smem_addr(&ctl.empty[i]), 1);
     }
-    bar_init(smem_addr(&ctl.q_full), 8);
     for (int i = 0; i < 2; i++) {
+      bar_init(smem_addr(&ctl.q_full[i]), 2);
+      bar_init(smem_addr(&ctl.q_empty[i]), 1);
       bar_init(smem_addr(&ctl.s_full[i]), 1);
+      bar_init(smem_addr(&ctl.p_half[i]), 4);
       bar_init(smem_addr(&ctl.p_full[i]), 4);
     }
     bar_init(smem_addr(&ctl.done), 1);
-    bar_init(smem_addr(&ctl.meet), 8);
+    bar_init(smem_addr(&ctl.stats), 8);
+    bar_init(smem_addr(&ctl.read), 4);
     bar_init(smem_addr(&ctl.drain), 1);
     for (int i = 0; i < kSegments; i++) {
       bar_init(smem_addr(&ctl.seg_full[i]), 1);
-      bar_init(smem_addr(&ctl.seg_empty[i]), 10);  // 8 softmax warps, the loading and the issuing warp
+      bar_init(smem_addr(&ctl.seg_empty[i]), 16);  // every warp
     }
-    ctl.odd[0] = ctl.odd[1] = ctl.odd[2] = 0;
     ctl.give_up = 0;
     ctl.run_b = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -443,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
   }
   after_previous_work();
 
-  // this block's run: each thread adds up some sequences' tiles, the one whose sum
+  // this block's first run: each thread adds up some sequences' tiles, the one whose sum
   // reaches the run's first tile finds its place
   {
     const int per = (a.n + kThreads - 1) / kThreads, b0 = min(tid * per, a.n), b1 = min(b0 + per, a.n);
@@ -459,32 +504,29 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
       const int64_t y = __shfl_up_sync(~0u, inc, d);
       if (lane >= d) inc += y;
     }
-    if (lane == 31) ctl.scan[warp] = inc;
+    if (lane == 31) scan[warp] = inc;
     tmem_before();
     __syncthreads();
     tmem_after();
     int64_t before = 0, total = 0;
     for (int w = 0; w < kThreads / 32; w++) {
-      if (w < warp) before += ctl.scan[w];
-      total += ctl.scan[w];
+      if (w < warp) before += scan[w];
+      total += scan[w];
     }
     int64_t at = before + inc - mine;
-    int64_t run = (total + gridDim.x - 1) / gridDim.x;
-    if (run < a.min_tiles) run = a.min_tiles;
-    const int64_t first = run * blockIdx.x;
+    const int64_t run = run_length(total, gridDim.x, a.min_tiles), first = run * blockIdx.x;
+    if (tid == 0) ctl.total = total;
     if (blockIdx.x == 0) {
       if (bad) atomicOr(c.status, bad);
-      if (tid == 0) a.starts[a.n] = total, a.starts[a.n + 1] = run;
+      if (tid == 0) *a.total = total;
     }
-    if (first < total && first >= at && first < at + mine || blockIdx.x == 0) {
+    if ((first < total && first >= at && first < at + mine) || blockIdx.x == 0) {
       for (int b = b0; b < b1; b++) {
-        const Seq q = sequence<kRows>(c, a, b);
-        const int64_t n = static_cast<int64_t>(q.per_head) * c.kv_heads;
+        const int64_t n = static_cast<int64_t>(sequence<kRows>(c, a, b).per_head) * c.kv_heads;
         if (blockIdx.x == 0) a.starts[b] = at;
         if (first >= at && first < at + n) {
           ctl.run_b = b;
           ctl.run_off = first - at;
-          ctl.run_at = run < total - first ? run : total - first;
         }
         at += n;
       }
@@ -495,17 +537,102 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
   const bool work = ctl.run_b >= 0 && ctl.tmem == tmem;
   if (ctl.tmem != tmem && tid == 0) ctl.give_up = 1;
 
+  // Q of a segment and, with tile 0, the nodes' keys and values into a buffer, the nodes'
+  // also into the cache: by the two warps 10 and 11.
+  const auto load_rows = [&](const Segment& w, uint32_t segment) {
+    const uint32_t buffer = segment % kBuffers;
+    if (segment >= kBuffers && !wait(&ctl, &ctl.q_empty[buffer], (segment / kBuffers - 1) & 1)) return false;
+    const uint32_t to = buffer * q_size;
+    const int rows0 = w.block * kRows, rows = min(kRows, w.nodes * a.group - rows0);  // rows that are there
+    const bool tree = w.t0 == 0;
+    const int me = tid - 320, ch = me % kChunks, first_row = me / kChunks;  // a thread keeps its column of chunks
+    constexpr int kRowStep = 64 / kChunks, kAhead = 4;                      // nodes' rows of a thread on their way at a time
+    if (a.vec) {
+      for (int r = first_row; r < rows; r += kRowStep) {
+        const int node = divide(rows0 + r, a.group_inverse), h = w.head * a.group + rows0 + r - node * a.group, rr = r & (kTile - 1);
+        copy16(base + q_at + to + (r / kTile) * q_tile + (ch >> 3) * q_block + rr * 128 + ((ch ^ rr) & 7) * 16,
+               a.q.p + w.b * a.q.row + node * a.q.node + h * a.q.head + (ch * 8 < c.head_dim ? ch * 8 : 0), ch * 8 < c.head_dim);
+      }
+    } else {
+      for (int r = first_row; r < rows; r += kRowStep) {
+        const int node = divide(rows0 + r, a.group_inverse), h = w.head * a.group + rows0 + r - node * a.group, rr = r & (kTile - 1);
+        *reinterpret_cast<uint4*>(raw + q_at + to + (r / kTile) * q_tile + (ch >> 3) * q_block + rr * 128 + ((ch ^ rr) & 7) * 16) =
+            load8(a.q.p + w.b * a.q.row + node * a.q.node + h * a.q.head, ch * 8, c.head_dim, false);
+      }
+    }
+    uint32_t odd_lo = 0, odd_hi = 0;
+    if (tree) {
+      if (me < w.nodes) {
+        const uint64_t all = w.nodes < 64 ? (1ull << w.nodes) - 1 : ~0ull;
+        sets[buffer].of[me] = (a.masks ? a.masks[static_cast<int64_t>(w.b) * a.nodes + me] : ~0ull >> (63 - me)) & all;
+      }
+      const int room = w.nodes > 0 ? (c.counts[w.slot] << c.page_log2) - w.len : 0, keep = w.block == 0 ? min(w.nodes, room) : 0;
+      if (me == 0 && w.block == 0 && w.head == 0 && w.nodes > room) atomicOr(c.status, kNotReserved);
+#pragma unroll 1
+      for (int j0 = first_row; j0 < a.tree_rows; j0 += kAhead * kRowStep) {
+        uint4 x[kAhead], y[kAhead];
+        int page[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+          const int j = j0 + u * kRowStep;
+          x[u] = y[u] = make_uint4(0, 0, 0, 0);
+          if (j < w.nodes) {
+            x[u] = load8(a.k.p + w.b * a.k.row + j * a.k.node + w.head * a.k.head, ch * 8, c.head_dim, a.vec);
+            y[u] = load8(a.v.p + w.b * a.v.row + j * a.v.node + w.head * a.v.head, ch * 8, c.head_dim, a.vec);
+          }
+          page[u] = j < keep ? c.tables[static_cast<size_t>(w.slot) * c.width + ((w.len + j) >> c.page_log2)] : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+          const int j = j0 + u * kRowStep, at = to + (ch >> 3) * tree_block + j * 128 + ((ch ^ j) & 7) * 16;
+          if (j >= a.tree_rows) continue;
+          if (page[u] >= 0 && ch * 8 < c.head_dim) {
+            const int64_t in_pool = (((static_cast<int64_t>(a.layer) * c.num_pages + page[u]) * c.kv_heads + w.head) << c.page_log2) + ((w.len + j) & (c.page_size - 1));
+            *reinterpret_cast<uint4*>(c.k + in_pool * c.head_dim * 2 + ch * 16) = x[u];
+            *reinterpret_cast<uint4*>(c.v + in_pool * c.head_dim * 2 + ch * 16) = y[u];
+          }
+          // a value that is not finite would reach every row as 0 * inf: it is taken out
+          // here and added to the rows that see it at the end
+          uint32_t ws[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
+          bool odd = false;
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            if (not_finite<kBf16>(ws[e] & 0xffff)) ws[e] &= 0xffff0000u, odd = true;
+            if (not_finite<kBf16>(ws[e] >> 16)) ws[e] &= 0xffffu, odd = true;
+          }
+          if (odd) (j < 32 ? odd_lo : odd_hi) |= 1u << (j & 31);
+          *reinterpret_cast<uint4*>(raw + tk_at + at) = x[u];
+          *reinterpret_cast<uint4*>(raw + tv_at + at) = make_uint4(ws[0], ws[1], ws[2], ws[3]);
+        }
+      }
+    }
+    odd_lo = __reduce_or_sync(~0u, odd_lo);
+    odd_hi = __reduce_or_sync(~0u, odd_hi);
+    if (lane == 0) ctl.odd[segment % 4][warp & 1] = static_cast<uint64_t>(odd_hi) << 32 | odd_lo;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (a.scale < 0.0f) {  // scale's sign goes into Q
+      for (int r = first_row; r < rows; r += kRowStep) {
+        const int rr = r & (kTile - 1);
+        uint4* q = reinterpret_cast<uint4*>(raw + q_at + to + (r / kTile) * q_tile + (ch >> 3) * q_block + rr * 128 + ((ch ^ rr) & 7) * 16);
+        *q = make_uint4(q->x ^ 0x80008000u, q->y ^ 0x80008000u, q->z ^ 0x80008000u, q->w ^ 0x80008000u);
+      }
+    }
+    fence_async();
+    warp_arrive(&ctl.q_full[buffer]);
+    return true;
+  };
+
   if (work && warp == 8) {
     // ---- loading warp: a lane per page of a tile
     const int box = min(c.page_size, kTile);  // tokens of a page in a tile
     uint32_t slot = 0, turn = 0;
-    int tiles = 0;
-    bool ok = true, last = false;
-    for (Turn k; ok && !last; k.next()) {
+    int tiles = 0;  // of the first segment
+    bool ok = true;
+    for (Turn k; ok; k.next()) {
       ok = wait(&ctl, &ctl.seg_full[k.at], k.phase);
       if (!ok) break;
       const Segment g = ctl.seg[k.at];
-      last = g.last;
+      if (g.b < 0) break;
       for (int t = max(g.t0, 1); ok && t < g.t1; t++) {
         const int token = (t - 1) * kTile, here = min(kTile, g.len - token), n = (here + box - 1) / box;
         int page = 0;
@@ -513,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
         const int z = a.layer * c.num_pages + page, y = (token + lane * box) & (c.page_size - 1);
         // past the first tile the run's first Q goes before: behind a full ring of
         // copies its loads would wait for all of them
-        if (g.first && ++tiles == 2) ok = wait(&ctl, &ctl.q_full, 0);
+        if (tiles >= 0 && ++tiles == 2) ok = wait(&ctl, &ctl.q_full[0], 0);
 #pragma unroll 1
         for (int kv = 0; ok && kv < 2; kv++) {
           if (turn > 0) ok = wait(&ctl, &ctl.empty[slot], (turn - 1) & 1);
@@ -530,6 +657,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
           if (++slot == static_cast<uint32_t>(a.slots)) slot = 0, turn++;
         }
       }
+      tiles = -1;
       warp_arrive(&ctl.seg_empty[k.at]);
     }
     // on giving up, no copy may still be under way when the block ends
@@ -544,85 +672,88 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
     if (elect()) {
       constexpr uint32_t s_inst = instruction(kBf16, kTile, 0), o_inst = instruction(kBf16, kDim, 1);
       const uint32_t tree_inst = s_inst - (static_cast<uint32_t>((kTile - a.tree_rows) >> 3) << 17);
-      const uint64_t q_desc = operand(base + q_at, 16, 1024), k_desc = operand(base + ring_at, 16, 1024), v_desc = operand(base + ring_at, kTile * 128, 1024),
-                     tk_desc = operand(base + tk_at, 16, 1024), tv_desc = operand(base + tv_at, tree_block, 1024);
+      const uint64_t k_desc = operand(base + ring_at, 16, 1024), v_desc = operand(base + ring_at, kTile * 128, 1024);
+      uint64_t q_desc = operand(base + q_at, 16, 1024), tk_desc = operand(base + tk_at, 16, 1024), tv_desc = operand(base + tv_at, tree_block, 1024);
       const uint32_t slots = a.slots, q_step = q_block / 16, tree_step = tree_block / 16;
       uint32_t k_slot = 0, k_turn = 0, v_slot = 1, v_turn = 0;  // the next keys and values in the ring
-      uint32_t segment = 0, p_turn[2] = {0, 0};
-      bool ok = true, last = false;
-      for (Turn k; ok && !last; k.next()) {
+      uint32_t segment = 0, p_turn = 0;  // p_turn: bit s is group s's parity
+      bool ok = true;
+      for (Turn k; ok; k.next()) {
         ok = wait_alone(&ctl, &ctl.seg_full[k.at], k.phase);
-        if (!ok) break;
+        if (!ok || ctl.seg[k.at].b < 0) break;
         const int t0 = ctl.seg[k.at].t0, t1 = ctl.seg[k.at].t1, len = ctl.seg[k.at].len, nodes = ctl.seg[k.at].nodes;
-        last = ctl.seg[k.at].last;
         const int n = (t1 - t0) * (kWide ? 2 : 1);
+        ok = wait_alone(&ctl, &ctl.q_full[segment % kBuffers], segment / kBuffers & 1);
+        tmem_after();
         bool k_ready = false;  // the next keys were seen in the ring
-        const auto scores = [&](int j, auto group) {
-          constexpr int s = decltype(group)::value;
-          const int t = t0 + (kWide ? j >> 1 : j);
-          const uint64_t qd = q_desc + (kWide ? s * (q_tile / 16) : 0);
-          constexpr uint32_t d = s * kTile;
-          if (t > 0) {
-            if (!k_ready && !wait_alone(&ctl, &ctl.full[k_slot], k_turn & 1)) return false;
-            k_ready = kWide && s == 0;
+        // step j makes the scores of step j + 2, after the output of its own; group s
+        for (int j = -2; ok && j < n; j++) {
+          const int s = j & 1;
+          if (j >= 0) {
+            const int t = t0 + (kWide ? j >> 1 : j);
+            uint64_t vd = tv_desc;
+            int steps = max(1, (nodes + 15) / 16);
+            if (t > 0) {
+              ok = (kWide && s == 1) || wait_alone(&ctl, &ctl.full[v_slot], v_turn & 1);
+              if (!ok) break;
+              vd = v_desc + v_slot * (L::kSlot / 16);
+              steps = (min(kTile, len - (t - 1) * kTile) + 15) / 16;
+            }
+            // look for the next keys before P is there, not between its product and theirs
+            if (j + 2 < n && (!kWide || s == 0)) k_ready = bar_poll(smem_addr(&ctl.full[k_slot]), k_turn & 1);
+            // the products with the first 64 keys run while the other weights are made
+            const uint32_t d = 2 * kTile + s * kDim, p = s * kTile, turn = p_turn >> s & 1;
+            ok = wait_alone(&ctl, &ctl.p_half[s], turn);
+            if (!ok) break;
             tmem_after();
-            const uint64_t kd = k_desc + k_slot * (L::kSlot / 16);
 #pragma unroll
-            for (int i = 0; i < kDim / 16; i++) mma_ss(d, qd + (i >> 2) * q_step + (i & 3) * 2, kd + (i >> 2) * (kTile * 128 / 16) + (i & 3) * 2, s_inst, i > 0);
+            for (int i = 0; i < kTile / 32; i++)
+              if (i < steps) mma_ts(d, p + i * 8, vd + i * (2048 / 16), o_inst, j >= 2 || i > 0);
+            ok = wait_alone(&ctl, &ctl.p_full[s], turn);
+            if (!ok) break;
+            p_turn ^= 1u << s;
+            tmem_after();
+#pragma unroll
+            for (int i = kTile / 32; i < kTile / 16; i++)
+              if (i < steps) mma_ts(d, p + i * 8, vd + i * (2048 / 16), o_inst, 1);
+            if (t > 0 && (!kWide || s == 1)) {
+              tmem_commit(smem_addr(&ctl.empty[v_slot]));
+              v_slot += 2;
+              if (v_slot >= slots) v_slot -= slots, v_turn++;
+            }
+            if (j == n - 1) {
+              tmem_commit(smem_addr(&ctl.done));
+              tmem_commit(smem_addr(&ctl.q_empty[segment % kBuffers]));
+            }
+          }
+          if (j + 2 < n) {
+            const int t = t0 + (kWide ? (j + 2) >> 1 : j + 2);
+            const uint64_t qd = q_desc + (kWide ? s * (q_tile / 16) : 0);
+            const uint32_t d = s * kTile;
+            uint64_t kd = tk_desc;
+            uint32_t step = tree_step, inst = tree_inst;
+            if (t > 0) {
+              ok = k_ready || wait_alone(&ctl, &ctl.full[k_slot], k_turn & 1);
+              if (!ok) break;
+              k_ready = kWide && s == 0;
+              tmem_after();
+              kd = k_desc + k_slot * (L::kSlot / 16), step = kTile * 128 / 16, inst = s_inst;
+            }
+#pragma unroll
+            for (int i = 0; i < kDim / 16; i++) mma_ss(d, qd + (i >> 2) * q_step + (i & 3) * 2, kd + (i >> 2) * step + (i & 3) * 2, inst, i > 0);
             tmem_commit(smem_addr(&ctl.s_full[s]));
-            if (!kWide || s == 1) {
+            if (t > 0 && (!kWide || s == 1)) {
               tmem_commit(smem_addr(&ctl.empty[k_slot]));
               k_slot += 2;
               if (k_slot >= slots) k_slot -= slots, k_turn++;
             }
-          } else {
-#pragma unroll
-            for (int i = 0; i < kDim / 16; i++) mma_ss(d, qd + (i >> 2) * q_step + (i & 3) * 2, tk_desc + (i >> 2) * tree_step + (i & 3) * 2, tree_inst, i > 0);
-            tmem_commit(smem_addr(&ctl.s_full[s]));
           }
-          return true;
-        };
-        const auto outputs = [&](int j, auto group) {
-          constexpr int s = decltype(group)::value;
-          const int t = t0 + (kWide ? j >> 1 : j);
-          uint64_t vd = tv_desc;
-          int steps = max(1, (nodes + 15) / 16);
-          if (t > 0) {
-            if ((!kWide || s == 0) && !wait_alone(&ctl, &ctl.full[v_slot], v_turn & 1)) return false;
-            vd = v_desc + v_slot * (L::kSlot / 16);
-            steps = (min(kTile, len - (t - 1) * kTile) + 15) / 16;
-          }
-          // look for the next keys before P is there, not between its product and theirs
-          if (j + 2 < n && (!kWide || s == 0)) k_ready = bar_poll(smem_addr(&ctl.full[k_slot]), k_turn & 1);
-          if (!wait_alone(&ctl, &ctl.p_full[s], p_turn[s] & 1)) return false;
-          p_turn[s]++;
-          tmem_after();
-          constexpr uint32_t d = 2 * kTile + s * kDim, p = s * kTile;
-#pragma unroll
-          for (int i = 0; i < kTile / 16; i++)
-            if (i < steps) mma_ts(d, p + i * 8, vd + i * (2048 / 16), o_inst, j >= 2 || i > 0);
-          if (t > 0 && (!kWide || s == 1)) {
-            tmem_commit(smem_addr(&ctl.empty[v_slot]));
-            v_slot += 2;
-            if (v_slot >= slots) v_slot -= slots, v_turn++;
-          }
-          if (j == n - 1) tmem_commit(smem_addr(&ctl.done));
-          return true;
-        };
-        const std::integral_constant<int, 0> even;
-        const std::integral_constant<int, 1> odd;
-        ok = wait_alone(&ctl, &ctl.q_full, segment & 1);
-        tmem_after();
-        ok = ok && scores(0, even);
-        if (n > 1) ok = ok && scores(1, odd);
-        k_ready = false;
-        for (int j = 0; ok && j < n; j += 2) {
-          ok = outputs(j, even);
-          if (j + 2 < n) ok = ok && scores(j + 2, even);
-          if (j + 1 < n) ok = ok && outputs(j + 1, odd);
-          if (j + 3 < n) ok = ok && scores(j + 3, odd);
         }
         segment++;
+        if (kBuffers == 2) {
+          const uint64_t to = segment & 1 ? q_size / 16 : -static_cast<uint64_t>(q_size / 16);  // the other buffer
+          q_desc += to, tk_desc += to, tv_desc += to;
+        }
         if (ok) bar_arrive(smem_addr(&ctl.seg_empty[k.at]));
       }
       if (!ok) {  // what was issued ends before the block does
@@ -630,34 +761,40 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
         wait_out(&ctl.drain, 0);
       }
     }
-  } else if (work && warp == 10) {
-    // ---- walking warp: the run's segments, ahead of the others, and the first lines of
-    // what the softmax warps will load for them into L2
+  } else if (work && warp < 12 && warp >= 10) {
+    // ---- the warps that load Q and the nodes; the first of them walks: it hands the block's
+    // segments over, ahead of the others
     Walk<kRows> w;
-    w.start(c, a, ctl.run_b, ctl.run_off, ctl.run_at);
-    bool ok = true, more = true;
-    uint32_t used = 0;
-    for (Turn k; ok && more; k.next(), used++) {
-      if (used >= kSegments) ok = wait(&ctl, &ctl.seg_empty[k.at], k.phase ^ 1);
-      if (!ok) break;
-      if (lane == 0) {
-        ctl.seg[k.at] = Segment{w.b, w.head, w.block, w.t0, w.t1, w.tiles, w.q.slot, w.q.len, w.q.nodes, w.first, w.last};
-        bar_arrive(smem_addr(&ctl.seg_full[k.at]));
-      }
-      __syncwarp();
-      if (!w.first) {
-        const int rows0 = w.block * kRows, rows = min(kRows, w.q.nodes * a.group - rows0);
-        for (int r = lane; r < rows; r += 32) {
-          const int node = divide(rows0 + r, a.group_inverse), h = w.head * a.group + rows0 + r - node * a.group;
-          prefetch_row<kDim>(a.q.p + w.b * a.q.row + node * a.q.node + h * a.q.head);
+    const int64_t run = run_length(ctl.total, gridDim.x, a.min_tiles), first = run * blockIdx.x;
+    w.start(ctl.run_b, ctl.run_off, min(run, ctl.total - first));
+    uint32_t segment = 0;
+    bool ok = true, more = true, opening = true;
+    for (Turn k; ok; k.next(), segment++) {
+      if (warp == 10) {
+        Segment g;
+        g.b = -1;
+        while (more && g.b < 0) {
+          w.enter(c, a);
+          const int t0 = w.t0(), t1 = w.t1();
+          if (t0 < t1)
+            g = Segment{w.b, w.head, w.block, t0, t1, w.q.slot, w.q.len, w.q.nodes, t0 == 0 && t1 == w.tiles ? -1 : static_cast<int32_t>(blockIdx.x) * 2 + (opening ? 0 : 1)};
+          more = w.advance(c);
+          opening = false;
         }
-        if (w.t0 == 0)
-          for (int j = lane; j < w.q.nodes; j += 32) {
-            prefetch_row<kDim>(a.k.p + w.b * a.k.row + j * a.k.node + w.head * a.k.head);
-            prefetch_row<kDim>(a.v.p + w.b * a.v.row + j * a.v.node + w.head * a.v.head);
-          }
+        if (segment >= kSegments) ok = wait(&ctl, &ctl.seg_empty[k.at], k.phase ^ 1);
+        if (!ok) break;
+        if (lane == 0) {
+          ctl.seg[k.at] = g;
+          bar_arrive(smem_addr(&ctl.seg_full[k.at]));
+        }
+        __syncwarp();
       }
-      more = w.next(c, a);
+      ok = wait(&ctl, &ctl.seg_full[k.at], k.phase);
+      if (!ok) break;
+      const Segment g = ctl.seg[k.at];
+      if (g.b < 0) break;
+      ok = load_rows(g, segment);
+      warp_arrive(&ctl.seg_empty[k.at]);
     }
   } else if (work && warp < 8) {
     // ---- softmax warps: a thread per row
@@ -665,119 +802,70 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
     const uint32_t s_at = tmem + lanes + g * kTile, o_at = tmem + lanes + 2 * kTile + g * kDim;
     const float cs = fmaxf(fabsf(a.scale) * kLog2e, 1.17549435e-38f);  // not 0: a masked -inf stays -inf
-    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0;  // scale's sign goes into Q
     uint32_t loaded = 0, segment = 0, s_turn = 0;
-    bool ok = true, last = false;
-    for (Turn k; ok && !last; k.next()) {
+    bool ok = true;
+    for (Turn k; ok; k.next()) {
       ok = wait(&ctl, &ctl.seg_full[k.at], k.phase);
       if (!ok) break;
       const Segment& w = ctl.seg[k.at];  // read where it is needed: registers are for the scores
-      const int rows0 = w.block * kRows, rows = min(kRows, w.nodes * a.group - rows0);  // rows that are there
-      // Q, and with tile 0 the nodes' keys and values: 8 loads of Q and all of the nodes are
-      // on their way before the first is used
-      constexpr int kTreeLoads = kTreeTile * kChunks / 256, kRowStep = 256 / kChunks;
-      const int ch = tid % kChunks, first_row = tid / kChunks;  // a thread keeps its column of chunks
-      const bool tree = w.t0 == 0;
-      uint4 xk[kTreeLoads], xv[kTreeLoads];
-#pragma unroll
-      for (int u = 0; u < kTreeLoads; u++) {
-        const int j = first_row + u * kRowStep;
-        xk[u] = xv[u] = make_uint4(0, 0, 0, 0);
-        if (tree && j < w.nodes) {
-          xk[u] = load8(a.k.p + w.b * a.k.row + j * a.k.node + w.head * a.k.head, ch * 8, c.head_dim, a.vec);
-          xv[u] = load8(a.v.p + w.b * a.v.row + j * a.v.node + w.head * a.v.head, ch * 8, c.head_dim, a.vec);
-        }
-      }
-      for (int r0 = first_row; r0 < rows; r0 += 8 * kRowStep) {
-        uint4 x[8];
-#pragma unroll
-        for (int u = 0; u < 8; u++) {
-          const int r = r0 + u * kRowStep;
-          if (r < rows) {
-            const int node = divide(rows0 + r, a.group_inverse), h = w.head * a.group + rows0 + r - node * a.group;
-            x[u] = load8(a.q.p + w.b * a.q.row + node * a.q.node + h * a.q.head, ch * 8, c.head_dim, a.vec);
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < 8; u++) {
-          const int r = r0 + u * kRowStep, rr = r & (kTile - 1);
-          if (r < rows) {
-            x[u].x ^= flip, x[u].y ^= flip, x[u].z ^= flip, x[u].w ^= flip;
-            *reinterpret_cast<uint4*>(raw + q_at + (r / kTile) * q_tile + (ch >> 3) * q_block + rr * 128 + ((ch ^ rr) & 7) * 16) = x[u];
-          }
-        }
-      }
-      if (tid == 0) ctl.odd[(segment + 1) % 3] = 0;
-      if (tree) {
-#pragma unroll
-        for (int u = 0; u < kTreeLoads; u++) {
-          const int j = first_row + u * kRowStep;
-          if (j >= a.tree_rows) continue;
-          // a value that is not finite would reach every row as 0 * inf: it is taken out
-          // here and added to the rows that see it at the end
-          uint32_t ws[4] = {xv[u].x, xv[u].y, xv[u].z, xv[u].w};
-          bool odd = false;
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            if (not_finite<kBf16>(ws[e] & 0xffff)) ws[e] &= 0xffff0000u, odd = true;
-            if (not_finite<kBf16>(ws[e] >> 16)) ws[e] &= 0xffffu, odd = true;
-          }
-          if (odd) atomicOr(reinterpret_cast<unsigned long long*>(&ctl.odd[segment % 3]), 1ull << j);
-          const int at = (ch >> 3) * tree_block + j * 128 + ((ch ^ j) & 7) * 16;
-          *reinterpret_cast<uint4*>(raw + tk_at + at) = xk[u];
-          *reinterpret_cast<uint4*>(raw + tv_at + at) = make_uint4(ws[0], ws[1], ws[2], ws[3]);
-        }
-      }
-      fence_async();
-      warp_arrive(&ctl.q_full);
-      if (tree && w.block == 0 && w.nodes > 0) {  // the nodes' keys and values go to the cache
-        const int room = (c.counts[w.slot] << c.page_log2) - w.len, keep = min(w.nodes, room);
-        if (tid == 0 && w.head == 0 && w.nodes > room) atomicOr(c.status, kNotReserved);
-        if (ch * 8 < c.head_dim) {
-#pragma unroll
-          for (int u = 0; u < kTreeLoads; u++) {
-            const int j = first_row + u * kRowStep, pos = w.len + j;
-            if (j < keep) {
-              const int64_t page = c.tables[static_cast<size_t>(w.slot) * c.width + (pos >> c.page_log2)] + static_cast<int64_t>(a.layer) * c.num_pages;
-              const int64_t at = (((page * c.kv_heads + w.head) << c.page_log2) + (pos & (c.page_size - 1))) * c.head_dim * 2 + ch * 16;
-              *reinterpret_cast<uint4*>(c.k + at) = xk[u];
-              *reinterpret_cast<uint4*>(c.v + at) = xv[u];
-            }
-          }
-        }
-      }
-      __syncwarp();
-
+      if (w.b < 0) break;
+      const int rows0 = w.block * kRows, rows = min(kRows, w.nodes * a.group - rows0);
       const int r = row + (kWide ? g * kTile : 0);
       const bool mine = r < rows, any = (r & ~31) < rows;  // this row, this warp's rows are there
       const int node = mine ? divide(rows0 + r, a.group_inverse) : 0, h = w.head * a.group + (mine ? rows0 + r - node * a.group : 0);
       uint64_t sees = 0;
-      if (mine && w.t0 == 0) {
-        sees = a.masks ? a.masks[static_cast<int64_t>(w.b) * a.nodes + node] : ~0ull >> (63 - node);
-        if (w.nodes < 64) sees &= (1ull << w.nodes) - 1;
-      }
       float t_ref = -INFINITY, sum = 0.0f;
+      bool clear = segment == 0;
       const int step = kWide ? 1 : 2;
       for (int t = w.t0 + (kWide ? 0 : g); ok && t < w.t1; t += step) {
         ok = wait(&ctl, &ctl.s_full[g], s_turn & 1);
         if (!ok) break;
         s_turn++;
+        // the last segment's O has been read before a product writes it again
+        if (!clear) {
+          ok = wait(&ctl, &ctl.read, (segment - 1) & 1);
+          if (!ok) break;
+          clear = true;
+        }
+        if (t == 0 && mine) sees = sets[segment % kBuffers].of[node];
         tmem_after();
         const int keys = t > 0 ? min(kTile, w.len - (t - 1) * kTile) : kTreeTile;
+        if (t > 0 && keys < kTile) {
+          // the rows of V past the sequence's end that the last 16-key step reads are
+          // not its tokens: zeros in their place
+          const uint32_t e = loaded + 2 * (t - max(w.t0, 1)) + 1, slot = e % a.slots;
+          ok = wait(&ctl, &ctl.full[slot], (e / a.slots) & 1);
+          if (!ok) break;
+          const int end = (keys + 15) & ~15;
+          for (int i = row; i < (end - keys) * kChunks; i += kTile) {
+            const int j = keys + i / kChunks, ch = i % kChunks;
+            *reinterpret_cast<uint4*>(raw + ring_at + slot * L::kSlot + (ch >> 3) * (kTile * 128) + j * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_async();
+        }
         if (any) {
-          // the scores are read from TMEM twice, 32 at a time: for their maximum and for
-          // their exponentials.  128 at once would not fit beside the rest in registers,
-          // and what spills is evicted from the little L1 that the ring leaves.
+          // The scores are read from TMEM twice, 64 at a time, in loops: for their maximum
+          // and for their exponentials.  All 128 at once, unrolled, make a step shorter but
+          // the whole a quarter slower: the code no longer fits the instruction caches
+          // beside the rest.
           float m0 = -INFINITY, m1 = -INFINITY;
           const int columns = t > 0 ? kTile : kTreeTile;
-#pragma unroll 1
-          for (int i = 0; i < columns; i += 32) {
-            uint32_t v[32];
+          const auto scores = [&](int i, uint32_t* v) {
             tmem_load32(s_at + i, v);
+            tmem_load32(s_at + i + 32, v + 32);
             tmem_wait_ld();
-            unseen(v, t == 0 ? static_cast<uint32_t>(sees >> i) : i + 32 <= keys ? ~0u : i < keys ? (1u << (keys - i)) - 1 : 0u);
+            const uint64_t seen = t == 0 ? sees : i + 64 <= keys ? ~0ull : i < keys ? (1ull << (keys - i)) - 1 : 0ull;
+            if (!__all_sync(~0u, seen == ~0ull)) {
+              unseen(v, static_cast<uint32_t>(seen));
+              unseen(v + 32, static_cast<uint32_t>(seen >> 32));
+            }
+          };
+#pragma unroll 1
+          for (int i = 0; i < columns; i += 64) {
+            uint32_t v[64];
+            scores(i, v);
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
+            for (int e = 0; e < 64; e += 2) {
               m0 = fmaxf(m0, __uint_as_float(v[e]));
               m1 = fmaxf(m1, __uint_as_float(v[e + 1]));
             }
@@ -804,96 +892,96 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
           const float t_use = t_ref == -INFINITY ? 0.0f : t_ref;
           float a0 = 0.0f, a1 = 0.0f;
 #pragma unroll 1
-          for (int i = 0; i < columns; i += 32) {
-            uint32_t v[32];
-            tmem_load32(s_at + i, v);
-            tmem_wait_ld();
-            unseen(v, t == 0 ? static_cast<uint32_t>(sees >> i) : i + 32 <= keys ? ~0u : i < keys ? (1u << (keys - i)) - 1 : 0u);
-            uint32_t p[16];
+          for (int i = 0; i < columns; i += 64) {
+            uint32_t v[64];
+            scores(i, v);
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
+            for (int e = 0; e < 64; e += 2) {
               const float p0 = exp2_fast(__fmaf_rn(__uint_as_float(v[e]), cs, -t_use));
               const float p1 = exp2_fast(__fmaf_rn(__uint_as_float(v[e + 1]), cs, -t_use));
               a0 += p0, a1 += p1;
-              p[e / 2] = pack<kBf16>(p0, p1);
+              v[e / 2] = pack<kBf16>(p0, p1);
             }
-            tmem_store16(s_at + i / 2, p);  // over scores already read
+            tmem_store32(s_at + i / 2, v);  // over scores already read
+            if (i == 0) {
+              tmem_wait_st();
+              tmem_before();
+              warp_arrive(&ctl.p_half[g]);
+            }
           }
           sum += a0 + a1;
           tmem_wait_st();
-        }
-        if (t > 0 && keys < kTile) {
-          // the rows of V past the sequence's end that the last 16-key step reads are
-          // not its tokens: zeros in their place
-          const uint32_t e = loaded + 2 * (t - max(w.t0, 1)) + 1, slot = e % a.slots;
-          ok = wait(&ctl, &ctl.full[slot], (e / a.slots) & 1);
-          if (!ok) break;
-          const int end = (keys + 15) & ~15;
-          for (int i = row; i < (end - keys) * kChunks; i += kTile) {
-            const int j = keys + i / kChunks, ch = i % kChunks;
-            *reinterpret_cast<uint4*>(raw + ring_at + slot * L::kSlot + (ch >> 3) * (kTile * 128) + j * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fence_async();
+        } else {
+          warp_arrive(&ctl.p_half[g]);
         }
         tmem_before();
         warp_arrive(&ctl.p_full[g]);
       }
-      ok = ok && wait(&ctl, &ctl.done, segment & 1);
+      if (ok && !clear) ok = wait(&ctl, &ctl.read, (segment - 1) & 1);
+      if (!ok) break;
+      loaded += 2 * (w.t1 - max(w.t0, 1));
+      sums[segment % kBuffers].t[g][row] = t_ref;
+      sums[segment % kBuffers].sum[g][row] = sum;
+      warp_arrive(&ctl.stats);
+      segment++;
+      warp_arrive(&ctl.seg_empty[k.at]);
+    }
+  } else if (work && warp >= 12) {
+    // ---- writing warps: a segment's rows are joined over the two groups and written, or
+    // left to be joined over blocks, while the others begin the next segment
+    const int row = tid & (kTile - 1);
+    const uint32_t o_at = tmem + (static_cast<uint32_t>(warp & 3) << 21) + 2 * kTile;
+    uint32_t segment = 0;
+    bool ok = true;
+    for (Turn k; ok; k.next()) {
+      ok = wait(&ctl, &ctl.seg_full[k.at], k.phase);
+      if (!ok) break;
+      const Segment& w = ctl.seg[k.at];
+      if (w.b < 0) break;
+      ok = wait(&ctl, &ctl.stats, segment & 1) && wait(&ctl, &ctl.done, segment & 1);
       if (!ok) break;
       tmem_after();
-      loaded += 2 * (w.t1 - max(w.t0, 1));
-
-      // ---- the segment's end: join the groups, write the rows or leave them to be joined
-      constexpr int kMine = kWide ? kDim : kDim / 2;  // columns that this thread writes
-      const int col0 = kWide ? 0 : g * kMine;
-      const bool whole = w.t0 == 0 && w.t1 == w.tiles;
-      float f0 = 1.0f, f1 = 0.0f;  // factors of the first and the second group's O
-      if (!kWide) {
-        // both groups' threads of a row can read both O: each writes half the columns
-        ctl.sums[g][0][row] = t_ref;
-        ctl.sums[g][1][row] = sum;
-        warp_arrive(&ctl.meet);
-        ok = wait(&ctl, &ctl.meet, segment & 1);
-        if (!ok) break;
-        const float ta = ctl.sums[0][0][row], tb = ctl.sums[1][0][row], sa = ctl.sums[0][1][row], sb = ctl.sums[1][1][row];
-        t_ref = fmaxf(ta, tb);
-        f0 = weight(ta, sa, t_ref);
-        f1 = weight(tb, sb, t_ref);
-        sum = sa * f0 + sb * f1;
-      }
-      if (any) {
-        const int64_t at = (static_cast<int64_t>(w.b) * a.nodes + node) * a.q_heads + h;
-        const uint64_t odd = w.t0 == 0 ? ctl.odd[segment % 3] & sees : 0;
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        float* part = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (w.first ? 0 : 1)) * part_floats<kDim, kRows>();
-        const bool one = kWide || w.t1 - w.t0 == 1;  // only one group had tiles
+      const int rows0 = w.block * kRows, rows = min(kRows, w.nodes * a.group - rows0);
+      const bool whole = w.part < 0;
+      const bool one = kWide || w.t1 - w.t0 == 1;  // a row's O is in one group only
+      const uint64_t odd = w.t0 == 0 ? ctl.odd[segment % 4][0] | ctl.odd[segment % 4][1] : 0;
+      const Sums& of = sums[segment % kBuffers];
+      float* part = a.partial + static_cast<int64_t>(w.part) * part_floats<kDim, kRows>();
 #pragma unroll 1
-        for (int i = 0; i < kMine; i += 32) {
-          const int col = col0 + i;
+      for (int g = 0; g < (kWide ? 2 : 1); g++) {
+        const int r = row + g * kTile;
+        const bool mine = r < rows, any = (r & ~31) < rows;  // this row, this warp's rows are there
+        if (!any) break;
+        const float ta = of.t[g][row], sa = of.sum[g][row];
+        float t_ref = ta, sum = sa, f0 = 1.0f, f1 = 0.0f;  // factors of the two groups' O
+        if (!kWide) {
+          const float tb = of.t[1][row], sb = of.sum[1][row];
+          t_ref = fmaxf(ta, tb);
+          f0 = weight(ta, sa, t_ref);
+          f1 = weight(tb, sb, t_ref);
+          sum = sa * f0 + sb * f1;
+        }
+        const int node = mine ? divide(rows0 + r, a.group_inverse) : 0, h = w.head * a.group + (mine ? rows0 + r - node * a.group : 0);
+        const int64_t at = (static_cast<int64_t>(w.b) * a.nodes + node) * a.q_heads + h;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        uint64_t seen = 0;
+        if (odd && mine) seen = odd & (a.masks ? a.masks[static_cast<int64_t>(w.b) * a.nodes + node] : ~0ull >> (63 - node));
+#pragma unroll 1
+        for (int col = 0; col < kDim; col += 32) {
           float x[32];
           {
             uint32_t o[32];
             __syncwarp();
-            tmem_load32(kWide ? o_at + col : tmem + lanes + 2 * kTile + col, o);
+            tmem_load32(o_at + (kWide ? g * kDim : 0) + col, o);
             tmem_wait_ld();
             // a factor of 0 must not meet what an unused accumulator holds
 #pragma unroll
             for (int e = 0; e < 32; e++) x[e] = kWide ? __uint_as_float(o[e]) : f0 == 0.0f ? 0.0f : __uint_as_float(o[e]) * f0;
             if (!one) {
-              tmem_load32(tmem + lanes + 2 * kTile + kDim + col, o);
+              tmem_load32(o_at + kDim + col, o);
               tmem_wait_ld();
 #pragma unroll
               for (int e = 0; e < 32; e++) x[e] += f1 == 0.0f ? 0.0f : __uint_as_float(o[e]) * f1;
-            }
-          }
-          if (odd) {  // rare: the values that were taken out
-            for (uint64_t m = odd; m; m &= m - 1) {
-              const uint16_t* vr = a.v.p + w.b * a.v.row + (__ffsll(m) - 1) * a.v.node + w.head * a.v.head;
-#pragma unroll
-              for (int e = 0; e < 32; e++) {
-                const uint16_t y = col + e < c.head_dim ? vr[col + e] : 0;
-                if (not_finite<kBf16>(y)) x[e] += widen<kBf16>(y);
-              }
             }
           }
           if (mine) {
@@ -911,24 +999,26 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
             }
           }
         }
-        if (mine && (kWide || g == 0)) {
+        if (mine) {
           if (!whole) reinterpret_cast<float2*>(part + kDim * kRows)[r] = make_float2(t_ref, sum);
           else if (a.out_lse) a.out_lse[at] = log_sum(t_ref, sum);
+          if (seen)  // rare: the values that were taken out
+            add_odd<kBf16>(a.v.p + w.b * a.v.row + w.head * a.v.head, a.v.node, seen, c.head_dim, whole ? a.out + at * c.head_dim : nullptr, part + 4 * r, 4 * kRows);
         }
       }
+      tmem_before();
+      warp_arrive(&ctl.read);
       if (w.t0 == 0) {  // rows of nodes that are not there: zeros
-        const int have = max(rows, 0), want = min(kRows, a.nodes * a.group - rows0);
-        for (int i = tid; i < (want - have) * (c.head_dim / 8); i += 256) {
-          const int q = rows0 + have + i / (c.head_dim / 8);
-          const int64_t at = (static_cast<int64_t>(w.b) * a.nodes + q / a.group) * a.q_heads + w.head * a.group + q % a.group;
-          reinterpret_cast<uint4*>(a.out + at * c.head_dim)[i % (c.head_dim / 8)] = make_uint4(0, 0, 0, 0);
-          if (i % (c.head_dim / 8) == 0 && a.out_lse) a.out_lse[at] = -INFINITY;
+        const int have = max(rows, 0), want = min(kRows, a.nodes * a.group - rows0), chunks = c.head_dim >> 3;
+        for (int i = row; i < (want - have) * chunks; i += kTile) {
+          const int q = rows0 + have + i / chunks, node = divide(q, a.group_inverse);
+          const int64_t at = (static_cast<int64_t>(w.b) * a.nodes + node) * a.q_heads + w.head * a.group + q - node * a.group;
+          reinterpret_cast<uint4*>(a.out + at * c.head_dim)[i % chunks] = make_uint4(0, 0, 0, 0);
+          if (i % chunks == 0 && a.out_lse) a.out_lse[at] = -INFINITY;
         }
       }
-      tmem_before();  // O has been read before the next segment's first product writes it
       __syncwarp();
       segment++;
-      last = w.last;
       warp_arrive(&ctl.seg_empty[k.at]);
     }
   }
@@ -951,9 +1041,9 @@ template <int kDim, bool kWide, bool kBf16>
 __global__ void __launch_bounds__(256) join_kernel(CacheView c, TreeArgs a) {
   constexpr int kRows = Layout<kDim, kWide>::kRows;
   after_previous_work();
-  const int64_t total = a.starts[a.n], run = a.starts[a.n + 1];
+  const int64_t total = *a.total, run = run_length(total, a.run_blocks, a.min_tiles);
   Walk<kRows> w;
-  int64_t begin;
+  int64_t begin;  // the item's in the measure
   if (a.by_item) {
     const int per = c.kv_heads * a.blocks, b = blockIdx.x / per, i = blockIdx.x % per;
     w.q = sequence<kRows>(c, a, b);
@@ -961,7 +1051,8 @@ __global__ void __launch_bounds__(256) join_kernel(CacheView c, TreeArgs a) {
     w.head = i / a.blocks;
     w.block = i % a.blocks;
     w.tiles = w.block < w.q.active ? w.q.ctx + 1 : 1;
-    begin = a.starts[b] + static_cast<int64_t>(w.head) * w.q.per_head + min(w.block, w.q.active) * static_cast<int64_t>(w.q.ctx + 1) + max(0, w.block - w.q.active);
+    begin = a.starts[b] + static_cast<int64_t>(w.head) * w.q.per_head + static_cast<int64_t>(min(w.block, w.q.active)) * (w.q.ctx + 1 + kOverhead) +
+            max(0, w.block - w.q.active) * (1 + kOverhead);
   } else {
     const int64_t cut = run * (blockIdx.x + 1);
     if (cut >= total) return;
@@ -970,17 +1061,20 @@ __global__ void __launch_bounds__(256) join_kernel(CacheView c, TreeArgs a) {
       const int mid = (lo + hi + 1) >> 1;
       if (a.starts[mid] <= cut) lo = mid; else hi = mid - 1;
     }
-    w.start(c, a, lo, cut - a.starts[lo], 1);
-    begin = cut - w.t0;
-    if (w.t0 == 0 || cut - run > begin) return;  // not inside an item, or not the first cut in it
+    w.start(lo, cut - a.starts[lo], 1);
+    w.enter(c, a);
+    begin = cut - w.into;
+    if (cut <= begin + kOverhead || cut - run > begin + kOverhead) return;  // not the first cut between the item's tiles
   }
-  const int64_t first = begin / run, last = (begin + w.tiles - 1) / run;
+  // the runs that have tiles of it
+  const int64_t first = quotient(begin + kOverhead, run), last = quotient(begin + kOverhead + w.tiles - 1, run);
   if (first == last) return;  // whole
   const int rows0 = w.block * kRows, rows = min(kRows, w.q.nodes * a.group - rows0);
   const int r = blockIdx.y * 32 + (threadIdx.x & 31), col4 = blockIdx.z * 8 + (threadIdx.x >> 5);
   if (r >= rows || col4 * 4 >= c.head_dim) return;
-  // the item is the second segment of its first run unless the run starts with it
-  const auto part = [&](int64_t x) { return a.partial + (x * 2 + (x == first && begin % run != 0 ? 1 : 0)) * part_floats<kDim, kRows>(); };
+  // in its first run the item is not the first of the run's unless the run starts in it
+  const int later = begin > run * first ? 1 : 0;
+  const auto part = [&](int64_t x) { return a.partial + (x * 2 + (x == first ? later : 0)) * part_floats<kDim, kRows>(); };
   const auto stats = [&](int64_t x) { return __ldcg(reinterpret_cast<const float2*>(part(x) + kDim * kRows) + r); };
   float t = -INFINITY;
 #pragma unroll 4
@@ -1017,7 +1111,8 @@ cudaError_t launch(tg_cache* c, TreeArgs a, cudaStream_t st) {
   const int rows = a.nodes * a.group < L::kRows ? a.nodes * a.group : L::kRows;
   a.q_rows = kWide ? kTile : (rows + 7) & ~7;
   a.tree_rows = (a.nodes + 15) & ~15;
-  const int fixed = kControl + (kWide ? 2 : 1) * a.q_rows * kDim * 2 + 2 * a.tree_rows * kDim * 2;
+  a.run_blocks = c->sms;
+  const int fixed = control_bytes<L::kBuffers>() + L::kBuffers * ((kWide ? 2 : 1) * a.q_rows + 2 * a.tree_rows) * kDim * 2;
   a.slots = (kMaxSmem - fixed) / L::kSlot;
   if (a.slots > kMaxSlots) a.slots = kMaxSlots;
   // the last row block's 128 rows, read from its start, end inside the block's memory:
@@ -1037,9 +1132,9 @@ cudaError_t launch_dim(tg_cache* c, const TreeArgs& a, bool wide, cudaStream_t s
   return bf16 ? launch<kDim, false, true>(c, a, st) : launch<kDim, false, false>(c, a, st);
 }
 
-// Starts of the sequences, then the partial rows of every block's two cut items.
+// The workspace: total and starts, then the parts of cut items, two per run.
 constexpr size_t kStartBytes = (65536 + 64) * sizeof(int64_t);
-constexpr size_t partial_bytes(int sms) { return static_cast<size_t>(sms) * 2 * 2 * kTile * (128 + 2) * sizeof(float); }
+constexpr size_t part_bytes(int sms) { return static_cast<size_t>(sms) * 2 * 2 * kTile * (128 + 2) * sizeof(float); }
 
 }  // namespace
 
@@ -1069,7 +1164,7 @@ int32_t tree_setup(tg_cache* c) noexcept {
   TG_TRY((allow_smem<128, false, true>()));
   TG_TRY((allow_smem<128, true, false>()));
   TG_TRY((allow_smem<128, true, true>()));
-  TG_TRY(cudaMalloc(&c->partial, kStartBytes + partial_bytes(c->sms)));
+  TG_TRY(cudaMalloc(&c->partial, kStartBytes + part_bytes(c->sms)));
   return TG_OK;
 }
 
@@ -1104,7 +1199,7 @@ int32_t tg_tree_attention(tg_cache* c, int32_t layer, int32_t n, const int32_t* 
   const bool wide = nodes * a.group > tg::kTile;  // more rows than one block of the tensor cores takes
   const int rows = wide ? 2 * tg::kTile : tg::kTile;
   a.blocks = (nodes * a.group + rows - 1) / rows;
-  a.min_tiles = 2;
+  a.min_tiles = 2 + tg::kOverhead;
   a.vec = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
             static_cast<uintptr_t>((q_row | q_node | q_head | k_row | k_node | k_head | v_row | v_node | v_head) * 2)) & 15) == 0;
   a.seqs = seqs;
@@ -1116,8 +1211,10 @@ int32_t tg_tree_attention(tg_cache* c, int32_t layer, int32_t n, const int32_t* 
   a.scale = scale;
   a.out = static_cast<uint16_t*>(out);
   a.out_lse = out_lse;
-  a.starts = static_cast<int64_t*>(c->partial);
-  a.partial = reinterpret_cast<float*>(static_cast<char*>(c->partial) + tg::kStartBytes);
+  char* space = static_cast<char*>(c->partial);
+  a.total = reinterpret_cast<int64_t*>(space);
+  a.starts = reinterpret_cast<int64_t*>(space + 128);
+  a.partial = reinterpret_cast<float*>(space + tg::kStartBytes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   TG_TRY(c->view.head_dim <= 64 ? tg::launch_dim<64>(c, a, wide, st) : tg::launch_dim<128>(c, a, wide, st));
   return TG_OK;
