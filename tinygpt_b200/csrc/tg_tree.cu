@@ -123,11 +123,6 @@ __device__ __forceinline__ void tmem_commit(uint32_t bar) {
       "=r"(v[o + 10]), "=r"(v[o + 11]), "=r"(v[o + 12]), "=r"(v[o + 13]), "=r"(v[o + 14]), "=r"(v[o + 15]), "=r"(v[o + 16]), "=r"(v[o + 17]), "=r"(v[o + 18]), \
       "=r"(v[o + 19]), "=r"(v[o + 20]), "=r"(v[o + 21]), "=r"(v[o + 22]), "=r"(v[o + 23]), "=r"(v[o + 24]), "=r"(v[o + 25]), "=r"(v[o + 26]), "=r"(v[o + 27]), \
       "=r"(v[o + 28]), "=r"(v[o + 29]), "=r"(v[o + 30]), "=r"(v[o + 31])
-#define TG_I32(v, o) \
-  "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7]), "r"(v[o + 8]), "r"(v[o + 9]), \
-      "r"(v[o + 10]), "r"(v[o + 11]), "r"(v[o + 12]), "r"(v[o + 13]), "r"(v[o + 14]), "r"(v[o + 15]), "r"(v[o + 16]), "r"(v[o + 17]), "r"(v[o + 18]), \
-      "r"(v[o + 19]), "r"(v[o + 20]), "r"(v[o + 21]), "r"(v[o + 22]), "r"(v[o + 23]), "r"(v[o + 24]), "r"(v[o + 25]), "r"(v[o + 26]), "r"(v[o + 27]), \
-      "r"(v[o + 28]), "r"(v[o + 29]), "r"(v[o + 30]), "r"(v[o + 31])
 #define TG_REGS32 \
   "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}"
 
@@ -135,8 +130,16 @@ __device__ __forceinline__ void tmem_commit(uint32_t bar) {
 __device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t* v) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 " TG_REGS32 ", [%32];" : TG_R32(v, 0) : "r"(at));
 }
-__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t* v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], " TG_REGS32 ";" ::TG_I32(v, 0), "r"(at) : "memory");
+__device__ __forceinline__ void tmem_load16(uint32_t at, uint32_t* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
+                 "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+               : "r"(at));
+}
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(at)
+               : "memory");
 }
 
 // Shared-memory matrix descriptor, 128-byte swizzle: start, leading and stride byte
@@ -291,7 +294,7 @@ struct Segment {
 constexpr int kSegments = 3;      // handed over ahead
 
 struct Control {
-  uint64_t full[kMaxSlots], empty[kMaxSlots], q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], stats, done, read, drain;
+  uint64_t full[kMaxSlots], empty[kMaxSlots], q_full[2], q_empty[2], s_full[2], p_full[2], stats, done, read, drain;
   uint64_t seg_full[kSegments], seg_empty[kSegments];
   uint64_t odd[4][2];  // nodes with a value that is not finite, by segment modulo 4 and loading warp
   int64_t total, run_off;
@@ -395,6 +398,32 @@ __device__ __forceinline__ uint4 load8(const uint16_t* row, int col, int dim, bo
   return vec ? *reinterpret_cast<const uint4*>(row + col) : load8_by_element(row, col);
 }
 
+// A row's fp32 columns in TMEM by f; its 16-bit weights by f.  By whole warps.
+__device__ __forceinline__ void scale_columns(uint32_t at, int columns, float f) {
+#pragma unroll 1
+  for (int i = 0; i < columns; i += 16) {
+    uint32_t o[16];
+    tmem_load16(at + i, o);
+    tmem_wait_ld();
+#pragma unroll
+    for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+    tmem_store16(at + i, o);
+  }
+}
+template <bool kBf16>
+__device__ __forceinline__ void scale_weights(uint32_t at, int columns, float f) {
+#pragma unroll 1
+  for (int i = 0; i < columns; i += 16) {
+    uint32_t p[16];
+    tmem_load16(at + i, p);
+    tmem_wait_ld();
+#pragma unroll
+    for (int e = 0; e < 16; e++) p[e] = pack<kBf16>(widen<kBf16>(p[e] & 0xffff) * f, widen<kBf16>(p[e] >> 16) * f);
+    tmem_store16(at + i, p);
+  }
+  tmem_wait_st();
+}
+
 // Scores of keys that a row does not see (their bit is clear): -inf.
 __device__ __forceinline__ void unseen(uint32_t* v, uint32_t seen) {
 #pragma unroll
@@ -462,7 +491,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
       bar_init(smem_addr(&ctl.q_full[i]), 2);
       bar_init(smem_addr(&ctl.q_empty[i]), 1);
       bar_init(smem_addr(&ctl.s_full[i]), 1);
-      bar_init(smem_addr(&ctl.p_half[i]), 4);
       bar_init(smem_addr(&ctl.p_full[i]), 4);
     }
     bar_init(smem_addr(&ctl.done), 1);
@@ -701,21 +729,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
             }
             // look for the next keys before P is there, not between its product and theirs
             if (j + 2 < n && (!kWide || s == 0)) k_ready = bar_poll(smem_addr(&ctl.full[k_slot]), k_turn & 1);
-            // the products with the first 64 keys run while the other weights are made
-            const uint32_t d = 2 * kTile + s * kDim, p = s * kTile, turn = p_turn >> s & 1;
-            ok = wait_alone(&ctl, &ctl.p_half[s], turn);
-            if (!ok) break;
-            tmem_after();
-#pragma unroll
-            for (int i = 0; i < kTile / 32; i++)
-              if (i < steps) mma_ts(d, p + i * 8, vd + i * (2048 / 16), o_inst, j >= 2 || i > 0);
-            ok = wait_alone(&ctl, &ctl.p_full[s], turn);
+            const uint32_t d = 2 * kTile + s * kDim, p = s * kTile;
+            ok = wait_alone(&ctl, &ctl.p_full[s], p_turn >> s & 1);
             if (!ok) break;
             p_turn ^= 1u << s;
             tmem_after();
 #pragma unroll
-            for (int i = kTile / 32; i < kTile / 16; i++)
-              if (i < steps) mma_ts(d, p + i * 8, vd + i * (2048 / 16), o_inst, 1);
+            for (int i = 0; i < kTile / 16; i++)
+              if (i < steps) mma_ts(d, p + i * 8, vd + i * (2048 / 16), o_inst, j >= 2 || i > 0);
             if (t > 0 && (!kWide || s == 1)) {
               tmem_commit(smem_addr(&ctl.empty[v_slot]));
               v_slot += 2;
@@ -814,19 +835,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
       const bool mine = r < rows, any = (r & ~31) < rows;  // this row, this warp's rows are there
       const int node = mine ? divide(rows0 + r, a.group_inverse) : 0, h = w.head * a.group + (mine ? rows0 + r - node * a.group : 0);
       uint64_t sees = 0;
-      float t_ref = -INFINITY, sum = 0.0f;
-      bool clear = segment == 0;
+      float t_ref = -INFINITY, sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      bool clear = segment == 0;  // the last segment's O has been read
       const int step = kWide ? 1 : 2;
       for (int t = w.t0 + (kWide ? 0 : g); ok && t < w.t1; t += step) {
         ok = wait(&ctl, &ctl.s_full[g], s_turn & 1);
         if (!ok) break;
         s_turn++;
-        // the last segment's O has been read before a product writes it again
-        if (!clear) {
-          ok = wait(&ctl, &ctl.read, (segment - 1) & 1);
-          if (!ok) break;
-          clear = true;
-        }
         if (t == 0 && mine) sees = sets[segment % kBuffers].of[node];
         tmem_after();
         const int keys = t > 0 ? min(kTile, w.len - (t - 1) * kTile) : kTreeTile;
@@ -842,77 +857,57 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
             *reinterpret_cast<uint4*>(raw + ring_at + slot * L::kSlot + (ch >> 3) * (kTile * 128) + j * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_async();
+          __syncwarp();
         }
         if (any) {
-          // The scores are read from TMEM twice, 64 at a time, in loops: for their maximum
-          // and for their exponentials.  All 128 at once, unrolled, make a step shorter but
-          // the whole a quarter slower: the code no longer fits the instruction caches
-          // beside the rest.
-          float m0 = -INFINITY, m1 = -INFINITY;
+          // 64 scores at a time: if their maximum exceeds the bound by more than the slack,
+          // the bound moves, and with it what the old one made (rare after a row's first
+          // scores); then their weights, which go over scores already read.  A loop, not
+          // unrolled over the tile: that did not fit the instruction caches beside the
+          // other roles.
           const int columns = t > 0 ? kTile : kTreeTile;
-          const auto scores = [&](int i, uint32_t* v) {
+#pragma unroll 1
+          for (int i = 0; i < columns; i += 64) {
+            uint32_t v[64];
             tmem_load32(s_at + i, v);
             tmem_load32(s_at + i + 32, v + 32);
             tmem_wait_ld();
-            const uint64_t seen = t == 0 ? sees : i + 64 <= keys ? ~0ull : i < keys ? (1ull << (keys - i)) - 1 : 0ull;
-            if (!__all_sync(~0u, seen == ~0ull)) {
+            if (t == 0 || keys < kTile) {
+              const uint64_t seen = t == 0 ? sees : i + 64 <= keys ? ~0ull : i < keys ? (1ull << (keys - i)) - 1 : 0ull;
               unseen(v, static_cast<uint32_t>(seen));
               unseen(v + 32, static_cast<uint32_t>(seen >> 32));
             }
-          };
-#pragma unroll 1
-          for (int i = 0; i < columns; i += 64) {
-            uint32_t v[64];
-            scores(i, v);
+            float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < 64; e += 2) {
-              m0 = fmaxf(m0, __uint_as_float(v[e]));
-              m1 = fmaxf(m1, __uint_as_float(v[e + 1]));
-            }
-          }
-          const float top = fmaxf(m0, m1) * cs;
-          const bool begun = t >= w.t0 + step;  // O holds something
-          const bool move = top > t_ref + kSlack;
-          if (__any_sync(~0u, move)) {
-            const float f = move ? exp2_fast(t_ref - top) : 1.0f;
-            if (move) t_ref = top;
-            sum *= f;
-            if (begun) {
-#pragma unroll 1
-              for (int i = 0; i < kDim; i += 32) {
-                uint32_t o[32];
-                tmem_load32(o_at + i, o);
-                tmem_wait_ld();
+            for (int e = 0; e < 64; e++) m[e & 3] = fmaxf(m[e & 3], __uint_as_float(v[e]));
+            const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * cs;
+            const bool move = top > t_ref + kSlack;
+            if (__any_sync(~0u, move)) {
+              const float f = move ? exp2_fast(t_ref - top) : 1.0f;
+              if (move) t_ref = top;
 #pragma unroll
-                for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                tmem_store32(o_at + i, o);
-              }
+              for (int e = 0; e < 4; e++) sum[e] *= f;
+              tmem_wait_st();
+              if (t >= w.t0 + step) scale_columns(o_at, kDim, f);
+              if (i > 0) scale_weights<kBf16>(s_at, i / 2, f);
             }
-          }
-          const float t_use = t_ref == -INFINITY ? 0.0f : t_ref;
-          float a0 = 0.0f, a1 = 0.0f;
-#pragma unroll 1
-          for (int i = 0; i < columns; i += 64) {
-            uint32_t v[64];
-            scores(i, v);
+            const float t_use = t_ref == -INFINITY ? 0.0f : t_ref;
 #pragma unroll
             for (int e = 0; e < 64; e += 2) {
               const float p0 = exp2_fast(__fmaf_rn(__uint_as_float(v[e]), cs, -t_use));
               const float p1 = exp2_fast(__fmaf_rn(__uint_as_float(v[e + 1]), cs, -t_use));
-              a0 += p0, a1 += p1;
+              sum[e & 3] += p0, sum[e + 1 & 3] += p1;
               v[e / 2] = pack<kBf16>(p0, p1);
             }
-            tmem_store32(s_at + i / 2, v);  // over scores already read
-            if (i == 0) {
-              tmem_wait_st();
-              tmem_before();
-              warp_arrive(&ctl.p_half[g]);
-            }
+            tmem_store16(s_at + i / 2, v);
+            tmem_store16(s_at + i / 2 + 16, v + 16);
           }
-          sum += a0 + a1;
           tmem_wait_st();
-        } else {
-          warp_arrive(&ctl.p_half[g]);
+        }
+        if (!clear) {  // the last segment's O has been read before a product writes it again
+          ok = wait(&ctl, &ctl.read, (segment - 1) & 1);
+          if (!ok) break;
+          clear = true;
         }
         tmem_before();
         warp_arrive(&ctl.p_full[g]);
@@ -921,7 +916,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
       if (!ok) break;
       loaded += 2 * (w.t1 - max(w.t0, 1));
       sums[segment % kBuffers].t[g][row] = t_ref;
-      sums[segment % kBuffers].sum[g][row] = sum;
+      sums[segment % kBuffers].sum[g][row] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
       warp_arrive(&ctl.stats);
       segment++;
       warp_arrive(&ctl.seg_empty[k.at]);
