@@ -291,10 +291,10 @@ struct Segment {
   int32_t slot, len, nodes;       // the sequence
   int32_t part;                   // the part that its rows make; -1: they are whole
 };
-constexpr int kSegments = 3;      // handed over ahead
+constexpr int kSegments = 2;      // in hand: this one and the next
 
 struct Control {
-  uint64_t full[kMaxSlots], empty[kMaxSlots], q_full[2], q_empty[2], s_full[2], p_full[2], stats, done, read, drain;
+  uint64_t full[kMaxSlots], empty[kMaxSlots], q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], half_done[2], stats, done, read, drain;
   uint64_t seg_full[kSegments], seg_empty[kSegments];
   uint64_t odd[4][2];  // nodes with a value that is not finite, by segment modulo 4 and loading warp
   int64_t total, run_off;
@@ -398,7 +398,7 @@ __device__ __forceinline__ uint4 load8(const uint16_t* row, int col, int dim, bo
   return vec ? *reinterpret_cast<const uint4*>(row + col) : load8_by_element(row, col);
 }
 
-// A row's fp32 columns in TMEM by f; its 16-bit weights by f.  By whole warps.
+// A row's fp32 columns in TMEM by f, by whole warps.
 __device__ __forceinline__ void scale_columns(uint32_t at, int columns, float f) {
 #pragma unroll 1
   for (int i = 0; i < columns; i += 16) {
@@ -409,19 +409,6 @@ __device__ __forceinline__ void scale_columns(uint32_t at, int columns, float f)
     for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
     tmem_store16(at + i, o);
   }
-}
-template <bool kBf16>
-__device__ __forceinline__ void scale_weights(uint32_t at, int columns, float f) {
-#pragma unroll 1
-  for (int i = 0; i < columns; i += 16) {
-    uint32_t p[16];
-    tmem_load16(at + i, p);
-    tmem_wait_ld();
-#pragma unroll
-    for (int e = 0; e < 16; e++) p[e] = pack<kBf16>(widen<kBf16>(p[e] & 0xffff) * f, widen<kBf16>(p[e] >> 16) * f);
-    tmem_store16(at + i, p);
-  }
-  tmem_wait_st();
 }
 
 // Scores of keys that a row does not see (their bit is clear): -inf.
@@ -491,7 +478,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
       bar_init(smem_addr(&ctl.q_full[i]), 2);
       bar_init(smem_addr(&ctl.q_empty[i]), 1);
       bar_init(smem_addr(&ctl.s_full[i]), 1);
+      bar_init(smem_addr(&ctl.p_half[i]), 4);
       bar_init(smem_addr(&ctl.p_full[i]), 4);
+      bar_init(smem_addr(&ctl.half_done[i]), 1);
     }
     bar_init(smem_addr(&ctl.done), 1);
     bar_init(smem_addr(&ctl.stats), 8);
@@ -714,30 +703,39 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
         ok = wait_alone(&ctl, &ctl.q_full[segment % kBuffers], segment / kBuffers & 1);
         tmem_after();
         bool k_ready = false;  // the next keys were seen in the ring
-        // step j makes the scores of step j + 2, after the output of its own; group s
+        // Step j, a tile for group s, makes the output of its tile, 64 keys as soon as their
+        // weights are there, then the scores of step j + 2, the group's next.
         for (int j = -2; ok && j < n; j++) {
           const int s = j & 1;
+          const bool last_use = !kWide || s == 1;  // of the tile's keys or values
           if (j >= 0) {
-            const int t = t0 + (kWide ? j >> 1 : j);
-            uint64_t vd = tv_desc;
-            int steps = max(1, (nodes + 15) / 16);
-            if (t > 0) {
-              ok = (kWide && s == 1) || wait_alone(&ctl, &ctl.full[v_slot], v_turn & 1);
+            const int t = t0 + (kWide ? j >> 1 : j), keys = t > 0 ? min(kTile, len - (t - 1) * kTile) : nodes;
+            if (t > 0 && !(kWide && s)) {
+              ok = wait_alone(&ctl, &ctl.full[v_slot], v_turn & 1);
               if (!ok) break;
-              vd = v_desc + v_slot * (L::kSlot / 16);
-              steps = (min(kTile, len - (t - 1) * kTile) + 15) / 16;
             }
             // look for the next keys before P is there, not between its product and theirs
-            if (j + 2 < n && (!kWide || s == 0)) k_ready = bar_poll(smem_addr(&ctl.full[k_slot]), k_turn & 1);
-            const uint32_t d = 2 * kTile + s * kDim, p = s * kTile;
-            ok = wait_alone(&ctl, &ctl.p_full[s], p_turn >> s & 1);
+            if (j + 2 < n && !(kWide && s)) k_ready = bar_poll(smem_addr(&ctl.full[k_slot]), k_turn & 1);
+            const uint64_t vd = t > 0 ? v_desc + v_slot * (L::kSlot / 16) : tv_desc;
+            const uint32_t d = 2 * kTile + s * kDim, p = s * kTile, turn = p_turn >> s & 1;
+            const int steps = max(1, (keys + 15) / 16);
+            ok = wait_alone(&ctl, &ctl.p_half[s], turn);
             if (!ok) break;
-            p_turn ^= 1u << s;
             tmem_after();
 #pragma unroll
-            for (int i = 0; i < kTile / 16; i++)
+            for (int i = 0; i < 4; i++)
               if (i < steps) mma_ts(d, p + i * 8, vd + i * (2048 / 16), o_inst, j >= 2 || i > 0);
-            if (t > 0 && (!kWide || s == 1)) {
+            tmem_commit(smem_addr(&ctl.half_done[s]));
+            ok = wait_alone(&ctl, &ctl.p_full[s], turn);
+            if (!ok) break;
+            p_turn ^= 1u << s;
+            if (steps > 4) {
+              tmem_after();
+#pragma unroll
+              for (int i = 4; i < 8; i++)
+                if (i < steps) mma_ts(d, p + i * 8, vd + i * (2048 / 16), o_inst, 1);
+            }
+            if (t > 0 && last_use) {
               tmem_commit(smem_addr(&ctl.empty[v_slot]));
               v_slot += 2;
               if (v_slot >= slots) v_slot -= slots, v_turn++;
@@ -749,21 +747,18 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
           }
           if (j + 2 < n) {
             const int t = t0 + (kWide ? (j + 2) >> 1 : j + 2);
-            const uint64_t qd = q_desc + (kWide ? s * (q_tile / 16) : 0);
-            const uint32_t d = s * kTile;
-            uint64_t kd = tk_desc;
-            uint32_t step = tree_step, inst = tree_inst;
             if (t > 0) {
               ok = k_ready || wait_alone(&ctl, &ctl.full[k_slot], k_turn & 1);
               if (!ok) break;
               k_ready = kWide && s == 0;
               tmem_after();
-              kd = k_desc + k_slot * (L::kSlot / 16), step = kTile * 128 / 16, inst = s_inst;
             }
+            const uint64_t qd = q_desc + (kWide ? s * (q_tile / 16) : 0), kd = t > 0 ? k_desc + k_slot * (L::kSlot / 16) : tk_desc;
+            const uint32_t d = s * kTile, step = t > 0 ? kTile * 128 / 16 : tree_step, inst = t > 0 ? s_inst : tree_inst;
 #pragma unroll
             for (int i = 0; i < kDim / 16; i++) mma_ss(d, qd + (i >> 2) * q_step + (i & 3) * 2, kd + (i >> 2) * step + (i & 3) * 2, inst, i > 0);
             tmem_commit(smem_addr(&ctl.s_full[s]));
-            if (t > 0 && (!kWide || s == 1)) {
+            if (t > 0 && last_use) {
               tmem_commit(smem_addr(&ctl.empty[k_slot]));
               k_slot += 2;
               if (k_slot >= slots) k_slot -= slots, k_turn++;
@@ -839,15 +834,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
       bool clear = segment == 0;  // the last segment's O has been read
       const int step = kWide ? 1 : 2;
       for (int t = w.t0 + (kWide ? 0 : g); ok && t < w.t1; t += step) {
+        const int keys = t > 0 ? min(kTile, w.len - (t - 1) * kTile) : w.nodes;
         ok = wait(&ctl, &ctl.s_full[g], s_turn & 1);
         if (!ok) break;
-        s_turn++;
         if (t == 0 && mine) sees = sets[segment % kBuffers].of[node];
         tmem_after();
-        const int keys = t > 0 ? min(kTile, w.len - (t - 1) * kTile) : kTreeTile;
         if (t > 0 && keys < kTile) {
-          // the rows of V past the sequence's end that the last 16-key step reads are
-          // not its tokens: zeros in their place
+          // the rows of V past the sequence's end that the last 16-key step reads are not
+          // its tokens: zeros in their place
           const uint32_t e = loaded + 2 * (t - max(w.t0, 1)) + 1, slot = e % a.slots;
           ok = wait(&ctl, &ctl.full[slot], (e / a.slots) & 1);
           if (!ok) break;
@@ -859,21 +853,21 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
           fence_async();
           __syncwarp();
         }
-        if (any) {
-          // 64 scores at a time: if their maximum exceeds the bound by more than the slack,
-          // the bound moves, and with it what the old one made (rare after a row's first
-          // scores); then their weights, which go over scores already read.  A loop, not
-          // unrolled over the tile: that did not fit the instruction caches beside the
-          // other roles.
-          const int columns = t > 0 ? kTile : kTreeTile;
 #pragma unroll 1
-          for (int i = 0; i < columns; i += 64) {
+        for (int half = 0; half < 2; half++) {
+          if (any && (!half || keys > 64)) {
+            // 64 scores: if their maximum exceeds the bound by more than the slack, the
+            // bound moves, and with it the output so far (rare after a row's first
+            // scores); then their weights, which go over the scores.  A loop, not unrolled
+            // over the tile: that did not fit the instruction caches beside the other roles.
+            const uint32_t at = s_at + half * 64;
             uint32_t v[64];
-            tmem_load32(s_at + i, v);
-            tmem_load32(s_at + i + 32, v + 32);
+            tmem_load32(at, v);
+            tmem_load32(at + 32, v + 32);
             tmem_wait_ld();
             if (t == 0 || keys < kTile) {
-              const uint64_t seen = t == 0 ? sees : i + 64 <= keys ? ~0ull : i < keys ? (1ull << (keys - i)) - 1 : 0ull;
+              const int here = keys - 64 * half;
+              const uint64_t seen = t == 0 ? sees : here >= 64 ? ~0ull : here > 0 ? (1ull << here) - 1 : 0ull;
               unseen(v, static_cast<uint32_t>(seen));
               unseen(v + 32, static_cast<uint32_t>(seen >> 32));
             }
@@ -887,30 +881,35 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
               if (move) t_ref = top;
 #pragma unroll
               for (int e = 0; e < 4; e++) sum[e] *= f;
-              tmem_wait_st();
-              if (t >= w.t0 + step) scale_columns(o_at, kDim, f);
-              if (i > 0) scale_weights<kBf16>(s_at, i / 2, f);
+              if (half) {  // the products with the first half's weights are to end first; those
+                           // of the tiles before had when this one's scores were made
+                ok = wait(&ctl, &ctl.half_done[g], s_turn & 1);
+                if (!ok) break;
+                tmem_after();
+              }
+              if (half || t >= w.t0 + step) scale_columns(o_at, kDim, f);
             }
             const float t_use = t_ref == -INFINITY ? 0.0f : t_ref;
 #pragma unroll
             for (int e = 0; e < 64; e += 2) {
               const float p0 = exp2_fast(__fmaf_rn(__uint_as_float(v[e]), cs, -t_use));
               const float p1 = exp2_fast(__fmaf_rn(__uint_as_float(v[e + 1]), cs, -t_use));
-              sum[e & 3] += p0, sum[e + 1 & 3] += p1;
+              sum[e & 3] += p0, sum[(e + 1) & 3] += p1;
               v[e / 2] = pack<kBf16>(p0, p1);
             }
-            tmem_store16(s_at + i / 2, v);
-            tmem_store16(s_at + i / 2 + 16, v + 16);
+            tmem_store16(s_at + half * 32, v);
+            tmem_store16(s_at + half * 32 + 16, v + 16);
+            tmem_wait_st();
           }
-          tmem_wait_st();
+          if (!clear) {  // the last segment's O has been read before a product writes it again
+            ok = wait(&ctl, &ctl.read, (segment - 1) & 1);
+            if (!ok) break;
+            clear = true;
+          }
+          tmem_before();
+          warp_arrive(half ? &ctl.p_full[g] : &ctl.p_half[g]);
         }
-        if (!clear) {  // the last segment's O has been read before a product writes it again
-          ok = wait(&ctl, &ctl.read, (segment - 1) & 1);
-          if (!ok) break;
-          clear = true;
-        }
-        tmem_before();
-        warp_arrive(&ctl.p_full[g]);
+        s_turn++;
       }
       if (ok && !clear) ok = wait(&ctl, &ctl.read, (segment - 1) & 1);
       if (!ok) break;
