@@ -60,8 +60,6 @@ struct TreeArgs {
   int32_t layer, n, nodes, q_heads, group, blocks, min_tiles, vec;  // vec: all rows are 16-byte aligned
   uint32_t group_inverse;  // ceil(2^32 / group)
   int32_t q_rows, tree_rows, slots;  // shared memory: rows of a row block, of the nodes' tile, ring slots
-  int32_t by_item;         // join_kernel: a block column per item, not per cut
-  int32_t run_blocks;      // blocks of tree_kernel's grid
   const int32_t* seqs;
   const int32_t* n_nodes;
   const uint64_t* masks;
@@ -69,9 +67,15 @@ struct TreeArgs {
   float scale;
   uint16_t* out;
   float* out_lse;
-  int64_t* total;          // all items' measure; for join_kernel, as starts
-  int64_t* starts;         // [n] where each sequence begins in it
+  struct CutItem* cuts;    // [blocks of the grid] for join_kernel
   float* partial;          // [runs, 2] parts of items (see part_floats)
+};
+
+// An item that runs cut, written by the block whose run has its first tile: its parts are
+// `part`, then the first ones of the runs after that up to `last`.
+struct CutItem {
+  int32_t b, head, block, nodes;  // b < 0: none in this run
+  int32_t part, last;
 };
 
 // ---- PTX -----------------------------------------------------------------------------
@@ -189,7 +193,7 @@ __device__ __forceinline__ int64_t quotient(int64_t x, int64_t d) {
 // A sequence's part of the work.  An item counts as its tiles and kOverhead more, for
 // what a block does once per item: runs are cut in this measure, so that a run of many
 // short items has as much to do as one of a few long ones.
-constexpr int kOverhead = 3;
+constexpr int kOverhead = 2;
 struct Seq {
   int slot, len, nodes;  // nodes 0 where the row cannot be served
   int ctx;               // tiles of cached tokens
@@ -533,14 +537,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
     int64_t at = before + inc - mine;
     const int64_t run = run_length(total, gridDim.x, a.min_tiles), first = run * blockIdx.x;
     if (tid == 0) ctl.total = total;
-    if (blockIdx.x == 0) {
-      if (bad) atomicOr(c.status, bad);
-      if (tid == 0) *a.total = total;
-    }
-    if ((first < total && first >= at && first < at + mine) || blockIdx.x == 0) {
+    if (blockIdx.x == 0 && bad) atomicOr(c.status, bad);
+    if (first < total && first >= at && first < at + mine) {
       for (int b = b0; b < b1; b++) {
         const int64_t n = static_cast<int64_t>(sequence<kRows>(c, a, b).per_head) * c.kv_heads;
-        if (blockIdx.x == 0) a.starts[b] = at;
         if (first >= at && first < at + n) {
           ctl.run_b = b;
           ctl.run_off = first - at;
@@ -553,6 +553,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
   constexpr uint32_t tmem = 0;  // where 512 columns start
   const bool work = ctl.run_b >= 0 && ctl.tmem == tmem;
   if (ctl.tmem != tmem && tid == 0) ctl.give_up = 1;
+  if (!work && tid == 0) a.cuts[blockIdx.x].b = -1;
 
   // Q of a segment and, with tile 0, the nodes' keys and values into a buffer, the nodes'
   // also into the cache: by the two warps 10 and 11.
@@ -785,6 +786,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
     w.start(ctl.run_b, ctl.run_off, min(run, ctl.total - first));
     uint32_t segment = 0;
     bool ok = true, more = true, opening = true;
+    CutItem cut;
+    cut.b = -1;
     for (Turn k; ok; k.next(), segment++) {
       if (warp == 10) {
         Segment g;
@@ -792,8 +795,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
         while (more && g.b < 0) {
           w.enter(c, a);
           const int t0 = w.t0(), t1 = w.t1();
-          if (t0 < t1)
-            g = Segment{w.b, w.head, w.block, t0, t1, w.q.slot, w.q.len, w.q.nodes, t0 == 0 && t1 == w.tiles ? -1 : static_cast<int32_t>(blockIdx.x) * 2 + (opening ? 0 : 1)};
+          if (t0 < t1) {
+            const int me = blockIdx.x, part = t0 == 0 && t1 == w.tiles ? -1 : 2 * me + (opening ? 0 : 1);
+            g = Segment{w.b, w.head, w.block, t0, t1, w.q.slot, w.q.len, w.q.nodes, part};
+            if (t0 == 0 && t1 < w.tiles) {  // the run's last segment
+              cut = CutItem{w.b, w.head, w.block, w.q.nodes, part, me + static_cast<int>(quotient(w.tiles - t1 + run - 1, run))};
+            }
+          }
           more = w.advance(c);
           opening = false;
         }
@@ -812,6 +820,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
       ok = load_rows(g, segment);
       warp_arrive(&ctl.seg_empty[k.at]);
     }
+    if (warp == 10 && lane == 0) a.cuts[blockIdx.x] = cut;
   } else if (work && warp < 8) {
     // ---- softmax warps: a thread per row
     const int g = warp >> 2, row = tid & (kTile - 1);       // group, row of its row block
@@ -1027,62 +1036,50 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
   }
 }
 
-// Joins the rows of items that runs cut: a thread per row and 4 columns, a warp per 32
-// rows, so that parts are read in whole lines.  Block x is an item when there are few
-// (by_item), else the cut between runs x and x + 1, and the first cut inside an item
-// does the item.  y: 32 rows, z: 32 columns.
+// Joins the rows of the items that runs cut: a thread per row and 4 columns, a warp per 32
+// rows, so that parts are read in whole lines, 8 parts at a time.  Grid: runs, 32 rows,
+// 32 columns.
 template <int kDim, bool kWide, bool kBf16>
 __global__ void __launch_bounds__(256) join_kernel(CacheView c, TreeArgs a) {
-  constexpr int kRows = Layout<kDim, kWide>::kRows;
+  constexpr int kRows = Layout<kDim, kWide>::kRows, kBatch = 8;
   after_previous_work();
-  const int64_t total = *a.total, run = run_length(total, a.run_blocks, a.min_tiles);
-  Walk<kRows> w;
-  int64_t begin;  // the item's in the measure
-  if (a.by_item) {
-    const int per = c.kv_heads * a.blocks, b = blockIdx.x / per, i = blockIdx.x % per;
-    w.q = sequence<kRows>(c, a, b);
-    w.b = b;
-    w.head = i / a.blocks;
-    w.block = i % a.blocks;
-    w.tiles = w.block < w.q.active ? w.q.ctx + 1 : 1;
-    begin = a.starts[b] + static_cast<int64_t>(w.head) * w.q.per_head + static_cast<int64_t>(min(w.block, w.q.active)) * (w.q.ctx + 1 + kOverhead) +
-            max(0, w.block - w.q.active) * (1 + kOverhead);
-  } else {
-    const int64_t cut = run * (blockIdx.x + 1);
-    if (cut >= total) return;
-    int lo = 0, hi = a.n - 1;  // the sequence that holds the cut
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (a.starts[mid] <= cut) lo = mid; else hi = mid - 1;
-    }
-    w.start(lo, cut - a.starts[lo], 1);
-    w.enter(c, a);
-    begin = cut - w.into;
-    if (cut <= begin + kOverhead || cut - run > begin + kOverhead) return;  // not the first cut between the item's tiles
-  }
-  // the runs that have tiles of it
-  const int64_t first = quotient(begin + kOverhead, run), last = quotient(begin + kOverhead + w.tiles - 1, run);
-  if (first == last) return;  // whole
-  const int rows0 = w.block * kRows, rows = min(kRows, w.q.nodes * a.group - rows0);
+  const CutItem w = a.cuts[blockIdx.x];
+  if (w.b < 0) return;
+  const int rows0 = w.block * kRows, rows = min(kRows, w.nodes * a.group - rows0);
   const int r = blockIdx.y * 32 + (threadIdx.x & 31), col4 = blockIdx.z * 8 + (threadIdx.x >> 5);
   if (r >= rows || col4 * 4 >= c.head_dim) return;
-  // in its first run the item is not the first of the run's unless the run starts in it
-  const int later = begin > run * first ? 1 : 0;
-  const auto part = [&](int64_t x) { return a.partial + (x * 2 + (x == first ? later : 0)) * part_floats<kDim, kRows>(); };
-  const auto stats = [&](int64_t x) { return __ldcg(reinterpret_cast<const float2*>(part(x) + kDim * kRows) + r); };
-  float t = -INFINITY;
-#pragma unroll 4
-  for (int64_t x = first; x <= last; x++) t = fmaxf(t, stats(x).x);
-  float sum = 0.0f;
+  const int first = blockIdx.x, n = w.last - first + 1;
+  const auto part = [&](int i) { return a.partial + static_cast<int64_t>(i == 0 ? w.part : 2 * (first + i)) * part_floats<kDim, kRows>(); };
+  float t = -INFINITY, sum = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-  for (int64_t x = first; x <= last; x++) {
-    const float2 ts = stats(x);
-    const float4 y = __ldcg(reinterpret_cast<const float4*>(part(x)) + col4 * kRows + r);
-    const float f = weight(ts.x, ts.y, t);
-    if (f != 0.0f) {
-      sum += f * ts.y;
-      o.x += f * y.x, o.y += f * y.y, o.z += f * y.z, o.w += f * y.w;
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += kBatch) {
+    float2 ts[kBatch];
+    float4 y[kBatch];
+    float top = t;
+#pragma unroll
+    for (int i = 0; i < kBatch; i++) {
+      ts[i] = make_float2(-INFINITY, 0.0f);
+      if (i0 + i < n) {
+        ts[i] = __ldcg(reinterpret_cast<const float2*>(part(i0 + i) + kDim * kRows) + r);
+        y[i] = __ldcg(reinterpret_cast<const float4*>(part(i0 + i)) + col4 * kRows + r);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; i++) top = fmaxf(top, ts[i].x);
+    const float before = weight(t, sum, top);
+    if (before != 1.0f) {
+      sum = before == 0.0f ? 0.0f : sum * before;
+      o.x *= before, o.y *= before, o.z *= before, o.w *= before;
+      t = top;
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; i++) {
+      const float f = weight(ts[i].x, ts[i].y, top);
+      if (f != 0.0f) {
+        sum += f * ts[i].y;
+        o.x += f * y[i].x, o.y += f * y[i].y, o.z += f * y[i].z, o.w += f * y[i].w;
+      }
     }
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -1105,16 +1102,13 @@ cudaError_t launch(tg_cache* c, TreeArgs a, cudaStream_t st) {
   const int rows = a.nodes * a.group < L::kRows ? a.nodes * a.group : L::kRows;
   a.q_rows = kWide ? kTile : (rows + 7) & ~7;
   a.tree_rows = (a.nodes + 15) & ~15;
-  a.run_blocks = c->sms;
   const int fixed = control_bytes<L::kBuffers>() + L::kBuffers * ((kWide ? 2 : 1) * a.q_rows + 2 * a.tree_rows) * kDim * 2;
   a.slots = (kMaxSmem - fixed) / L::kSlot;
   if (a.slots > kMaxSlots) a.slots = kMaxSlots;
   // the last row block's 128 rows, read from its start, end inside the block's memory:
   // at least 4 slots of 128 rows follow it
   cudaError_t e = launch_after(tree_kernel<kDim, kWide, kBf16>, dim3(c->sms), kThreads, fixed + a.slots * L::kSlot, st, 1, c->view, a, c->k_map, c->v_map);
-  const int64_t items = static_cast<int64_t>(a.n) * c->view.kv_heads * a.blocks;
-  a.by_item = items < c->sms;
-  const dim3 grid(static_cast<unsigned>(a.by_item ? items : c->sms - 1), (rows + 31) / 32, kDim / 32);
+  const dim3 grid(c->sms, (rows + 31) / 32, kDim / 32);
   if (e == cudaSuccess) e = launch_after(join_kernel<kDim, kWide, kBf16>, grid, 256, 0, st, 1, c->view, a);
   return e;
 }
@@ -1126,8 +1120,8 @@ cudaError_t launch_dim(tg_cache* c, const TreeArgs& a, bool wide, cudaStream_t s
   return bf16 ? launch<kDim, false, true>(c, a, st) : launch<kDim, false, false>(c, a, st);
 }
 
-// The workspace: total and starts, then the parts of cut items, two per run.
-constexpr size_t kStartBytes = (65536 + 64) * sizeof(int64_t);
+// The workspace: the cut items, then the parts, two per run.
+constexpr size_t cut_bytes(int sms) { return (static_cast<size_t>(sms) * sizeof(CutItem) + 255) / 256 * 256; }
 constexpr size_t part_bytes(int sms) { return static_cast<size_t>(sms) * 2 * 2 * kTile * (128 + 2) * sizeof(float); }
 
 }  // namespace
@@ -1158,7 +1152,7 @@ int32_t tree_setup(tg_cache* c) noexcept {
   TG_TRY((allow_smem<128, false, true>()));
   TG_TRY((allow_smem<128, true, false>()));
   TG_TRY((allow_smem<128, true, true>()));
-  TG_TRY(cudaMalloc(&c->partial, kStartBytes + part_bytes(c->sms)));
+  TG_TRY(cudaMalloc(&c->partial, cut_bytes(c->sms) + part_bytes(c->sms)));
   return TG_OK;
 }
 
@@ -1206,9 +1200,8 @@ int32_t tg_tree_attention(tg_cache* c, int32_t layer, int32_t n, const int32_t* 
   a.out = static_cast<uint16_t*>(out);
   a.out_lse = out_lse;
   char* space = static_cast<char*>(c->partial);
-  a.total = reinterpret_cast<int64_t*>(space);
-  a.starts = reinterpret_cast<int64_t*>(space + 128);
-  a.partial = reinterpret_cast<float*>(space + tg::kStartBytes);
+  a.cuts = reinterpret_cast<tg::CutItem*>(space);
+  a.partial = reinterpret_cast<float*>(space + tg::cut_bytes(c->sms));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   TG_TRY(c->view.head_dim <= 64 ? tg::launch_dim<64>(c, a, wide, st) : tg::launch_dim<128>(c, a, wide, st));
   return TG_OK;
