@@ -11,8 +11,9 @@ import ctypes
 from typing import NamedTuple
 
 from . import _lib
+from ._device import address, stream_address
 from ._lib import check
-from .sampler import _dtype_code, _ptr, _stream_ptr
+from .sampler import _dtype_code
 
 try:
     import torch
@@ -60,9 +61,8 @@ class BeamSearch:
         return bits.value
 
     def _of(self, t, name, dtype, shape):
-        if t is not None and (t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device.index != self.device):
-            raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on device {self.device}")
-        return t
+        if t is not None and (t.dtype is not dtype or t.shape != shape or t.get_device() != self.device or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on CUDA device {self.device}")
 
     def select(self, logits, scores, *, finished=None, eos_id: int = -1, pad_id: int = 0, mask_table=None, state_id=None,
                history=None, history_len=None, stream=None) -> Beams:
@@ -75,7 +75,7 @@ class BeamSearch:
             raise ValueError(f"logits must be [batch * {self.beams}, at least {self.vocab}] and scores [batch, {self.beams}]")
         if logits.stride(1) != 1 and self.vocab > 1:
             raise ValueError("logits rows must be contiguous")
-        if logits.device.index != self.device:
+        if logits.get_device() != self.device:
             raise ValueError(f"logits must be on device {self.device}")
         self._of(scores, "scores", torch.float32, (B, W))
         self._of(finished, "finished", torch.int32, (B, W))
@@ -84,11 +84,11 @@ class BeamSearch:
         if state_id is not None:
             words = (self.vocab + 31) // 32
             if mask_table is None or mask_table.dim() != 2 or mask_table.shape[1] != words or mask_table.element_size() != 4 or \
-                    not mask_table.is_contiguous() or mask_table.device.index != self.device:
+                    not mask_table.is_contiguous() or mask_table.get_device() != self.device:
                 raise ValueError(f"mask_table must be a contiguous 32-bit tensor [states, {words}] on device {self.device}")
             num_states = mask_table.shape[0]
-        ints = torch.empty((3, B, W), dtype=torch.int32, device=scores.device)
-        best = torch.empty((B, W), dtype=torch.float32, device=scores.device)
+        parents, tokens, done = (torch.empty_like(scores, dtype=torch.int32) for _ in range(3))
+        best = torch.empty_like(scores)
         new_history = new_len = None
         stride = 0
         if history is not None:
@@ -98,9 +98,8 @@ class BeamSearch:
                 raise ValueError("history given without history_len")
             self._of(history_len, "history_len", torch.int32, (rows,))
             new_history, new_len = torch.empty_like(history), torch.empty_like(history_len)
-        parents, tokens, done = ints.unbind(0)
-        check(self._L.tg_beam_select(self._h, _ptr(logits), _dtype_code(logits), logits.stride(0) if rows > 1 else logits.shape[1], B,
-                                     _ptr(scores), _ptr(finished), _ptr(mask_table), num_states, _ptr(state_id), eos_id, pad_id,
-                                     _ptr(history), _ptr(history_len), stride, _ptr(parents), _ptr(tokens), _ptr(best), _ptr(done),
-                                     _ptr(new_history), _ptr(new_len), _stream_ptr(stream)))
+        check(self._L.tg_beam_select(self._h, logits.data_ptr(), _dtype_code(logits), logits.stride(0) if rows > 1 else logits.shape[1], B,
+                                     scores.data_ptr(), address(finished), address(mask_table), num_states, address(state_id), eos_id, pad_id,
+                                     address(history), address(history_len), stride, parents.data_ptr(), tokens.data_ptr(), best.data_ptr(),
+                                     done.data_ptr(), address(new_history), address(new_len), stream_address(stream, self.device)))
         return Beams(parents, tokens, best, done, new_history, new_len)

@@ -19,8 +19,8 @@ import ctypes
 import math
 
 from . import _lib
+from ._device import address, stream_address
 from ._lib import check
-from .sampler import _ptr, _stream_ptr
 
 try:
     import torch
@@ -49,36 +49,35 @@ class _DeviceInts:
         self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": "<i4", "data": (ptr, False), "version": 2}
 
 
-def _rows(t, name: str, n: int | None = None, device: int | None = None):
-    """An int32 contiguous CUDA vector of n entries (None: not given)."""
+def _rows(t, name: str, n: int | None, device: int) -> int:
+    """The length of an int32 contiguous vector on the device, n entries if given (None: not given, 0)."""
     if t is None:
-        return None
-    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or not t.is_cuda:
-        raise ValueError(f"{name} must be a contiguous int32 CUDA vector")
-    if (n is not None and t.shape[0] != n) or (device is not None and t.device.index != device):
-        raise ValueError(f"{name} must have {n} entries on device {device}")
-    return t
+        return 0
+    shape = t.shape
+    if t.dtype is not torch.int32 or len(shape) != 1 or t.get_device() != device or not t.is_contiguous() or (n is not None and shape[0] != n):
+        raise ValueError(f"{name} must be a contiguous int32 vector{'' if n is None else f' of {n} entries'} on CUDA device {device}")
+    return shape[0]
 
 
-def _tree(t, name: str, shape, device: int, dtype=None):
-    if t.dtype != (dtype or torch.int32) or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device.index != device:
-        raise ValueError(f"{name} must be a contiguous {dtype or torch.int32} tensor of shape {tuple(shape)} on device {device}")
+def _dense(t, name: str, shape, device: int, dtype):
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on CUDA device {device}")
     return t
 
 
 def tree_masks(parents, n_nodes=None, *, out=None, stream=None):
     """tg_tree_masks: int64 [n, nodes] bit sets (a node and its ancestors) from int32 parents [n, nodes]."""
     n, nodes = parents.shape
-    dev = parents.device.index
-    if dev is None:
+    dev = parents.get_device()
+    if dev < 0:
         raise ValueError("parents must be a CUDA tensor")
-    _tree(parents, "parents", (n, nodes), dev)
+    _dense(parents, "parents", (n, nodes), dev, torch.int32)
     _rows(n_nodes, "n_nodes", n, dev)
     if out is None:
         out = torch.empty((n, nodes), dtype=torch.int64, device=parents.device)
-    _tree(out, "out", (n, nodes), dev, torch.int64)
+    _dense(out, "out", (n, nodes), dev, torch.int64)
     with torch.cuda.device(dev):
-        check(_lib.load().tg_tree_masks(n, nodes, _ptr(n_nodes), _ptr(parents), _ptr(out), _stream_ptr(stream)))
+        check(_lib.load().tg_tree_masks(n, nodes, address(n_nodes), address(parents), address(out), stream_address(stream, dev)))
     return out
 
 
@@ -102,9 +101,10 @@ class PagedCache:
         self.dtype = dtype
         self.layers, self.kv_heads, self.head_dim, self.page_size = int(layers), int(kv_heads), int(head_dim), int(page_size)
         self.num_pages, self.max_seqs, self.max_pages_per_seq = int(num_pages), int(max_seqs), int(max_pages_per_seq)
+        self._scale = 1.0 / math.sqrt(self.head_dim) if self.head_dim > 0 else 0.0
         if min(shape) <= 0:
             raise ValueError(f"the pools' shape {shape} must be positive")
-        where = torch.device("cuda", self.device)
+        self._where = where = torch.device("cuda", self.device)
         self.k = torch.empty(shape, dtype=dtype, device=where) if k is None else k
         self.v = torch.empty(shape, dtype=dtype, device=where) if v is None else v
         for name, t in (("k", self.k), ("v", self.v)):
@@ -113,7 +113,7 @@ class PagedCache:
         cfg = _lib.CacheConfig(self.layers, self.kv_heads, self.head_dim, self.page_size, self.num_pages, self.max_seqs,
                                self.max_pages_per_seq, code)
         h = ctypes.c_void_p()
-        check(self._L.tg_cache_create(self.device, ctypes.byref(cfg), _ptr(self.k), _ptr(self.v), ctypes.byref(h)))
+        check(self._L.tg_cache_create(self.device, ctypes.byref(cfg), address(self.k), address(self.v), ctypes.byref(h)))
         self._owner, self._h = _Handle(self._L, h), h
         st = _lib.CacheState()
         check(self._L.tg_cache_get_state(self._h, ctypes.byref(st)))
@@ -139,92 +139,97 @@ class PagedCache:
 
     def extend(self, seqs, counts, *, stream=None) -> None:
         """Pages for counts[i] tokens past slot seqs[i]'s length; a shared last page is copied first."""
-        n = _rows(seqs, "seqs", None, self.device).shape[0]
+        n = _rows(seqs, "seqs", None, self.device)
         _rows(counts, "counts", n, self.device)
-        check(self._L.tg_cache_extend(self._h, n, _ptr(seqs), _ptr(counts), _stream_ptr(stream)))
+        check(self._L.tg_cache_extend(self._h, n, seqs.data_ptr(), counts.data_ptr(), stream_address(stream, self.device)))
 
     def fork(self, src, dst, *, stream=None) -> None:
         """Slots dst[i] become copies of slots src[i] (-1: empty), all at once, sharing pages."""
-        n = _rows(src, "src", None, self.device).shape[0]
+        n = _rows(src, "src", None, self.device)
         _rows(dst, "dst", n, self.device)
-        check(self._L.tg_cache_fork(self._h, n, _ptr(src), _ptr(dst), _stream_ptr(stream)))
+        check(self._L.tg_cache_fork(self._h, n, src.data_ptr(), dst.data_ptr(), stream_address(stream, self.device)))
 
     def truncate(self, seqs, lens, *, stream=None) -> None:
         """Sets lengths back to lens[i]; pages past them are freed."""
-        n = _rows(seqs, "seqs", None, self.device).shape[0]
+        n = _rows(seqs, "seqs", None, self.device)
         _rows(lens, "lens", n, self.device)
-        check(self._L.tg_cache_truncate(self._h, n, _ptr(seqs), _ptr(lens), _stream_ptr(stream)))
+        check(self._L.tg_cache_truncate(self._h, n, seqs.data_ptr(), lens.data_ptr(), stream_address(stream, self.device)))
 
     def free(self, seqs, *, stream=None) -> None:
         """Empties slots."""
-        n = _rows(seqs, "seqs", None, self.device).shape[0]
-        check(self._L.tg_cache_truncate(self._h, n, _ptr(seqs), None, _stream_ptr(stream)))
+        n = _rows(seqs, "seqs", None, self.device)
+        check(self._L.tg_cache_truncate(self._h, n, seqs.data_ptr(), None, stream_address(stream, self.device)))
 
     def commit(self, seqs, counts, *, stream=None) -> None:
         """Advances lengths by counts[i] stored tokens."""
-        n = _rows(seqs, "seqs", None, self.device).shape[0]
+        n = _rows(seqs, "seqs", None, self.device)
         _rows(counts, "counts", n, self.device)
-        check(self._L.tg_cache_commit(self._h, n, _ptr(seqs), _ptr(counts), _stream_ptr(stream)))
+        check(self._L.tg_cache_commit(self._h, n, seqs.data_ptr(), counts.data_ptr(), stream_address(stream, self.device)))
 
-    def _tokens(self, t, name: str, n: int, tokens: int, heads: int):
-        if t.dtype != self.dtype or tuple(t.shape) != (n, tokens, heads, self.head_dim) or t.device.index != self.device:
-            raise ValueError(f"{name} must be a {self.dtype} tensor of shape {(n, tokens, heads, self.head_dim)} on device {self.device}")
+    def _strides(self, t, name: str, shape):
         st = t.stride()
-        if st[3] != 1:
-            raise ValueError(f"{name}: the last dimension must be contiguous")
+        if t.dtype is not self.dtype or t.shape != shape or t.get_device() != self.device or (st[3] != 1 and shape[3] != 1):
+            raise ValueError(f"{name} must be a {self.dtype} tensor of shape {shape} on CUDA device {self.device}, its last dimension contiguous")
         return st
 
     def append(self, layer: int, seqs, k, v, counts=None, *, stream=None) -> None:
         """Stores keys and values [n, tokens, kv_heads, head_dim] of one layer past the lengths (reserve with
         extend, advance with commit)."""
-        n, tokens = _rows(seqs, "seqs", None, self.device).shape[0], k.shape[1]
-        ks, vs = self._tokens(k, "k", n, tokens, self.kv_heads), self._tokens(v, "v", n, tokens, self.kv_heads)
+        n = _rows(seqs, "seqs", None, self.device)
+        if k.dim() != 4:
+            raise ValueError("k must be [n, tokens, kv_heads, head_dim]")
+        shape = (n, k.shape[1], self.kv_heads, self.head_dim)
+        ks, vs = self._strides(k, "k", shape), self._strides(v, "v", shape)
         _rows(counts, "counts", n, self.device)
-        check(self._L.tg_cache_append(self._h, layer, n, _ptr(seqs), _ptr(counts), tokens, _ptr(k), ks[0], ks[1], ks[2],
-                                      _ptr(v), vs[0], vs[1], vs[2], _stream_ptr(stream)))
+        check(self._L.tg_cache_append(self._h, layer, n, seqs.data_ptr(), address(counts), shape[1], k.data_ptr(), ks[0], ks[1], ks[2],
+                                      v.data_ptr(), vs[0], vs[1], vs[2], stream_address(stream, self.device)))
 
     def tree_attention(self, layer: int, seqs, q, k, v, masks=None, *, n_nodes=None, scale: float | None = None, out=None,
                        want_lse: bool = False, lse=None, stream=None):
         """tg_tree_attention: q [n, nodes, q_heads, head_dim] over the slots' cached tokens and the nodes' own k, v
         [n, nodes, kv_heads, head_dim], which are also stored past the lengths.  masks: int64 [n, nodes] bit sets
         (tree_masks; None: a chain).  Returns out, or (out, lse) with want_lse or lse given."""
-        n = _rows(seqs, "seqs", None, self.device).shape[0]
+        device, dim = self.device, self.head_dim
+        n = _rows(seqs, "seqs", None, device)
         if q.dim() != 4:
             raise ValueError("q must be [n, nodes, q_heads, head_dim]")
-        nodes, heads = q.shape[1], q.shape[2]
-        qs = self._tokens(q, "q", n, nodes, heads)
-        ks, vs = self._tokens(k, "k", n, nodes, self.kv_heads), self._tokens(v, "v", n, nodes, self.kv_heads)
+        _, nodes, heads, _ = q.shape
+        shape, kv = (n, nodes, heads, dim), (n, nodes, self.kv_heads, dim)
+        qs, ks, vs = self._strides(q, "q", shape), self._strides(k, "k", kv), self._strides(v, "v", kv)
         if masks is not None:
-            _tree(masks, "masks", (n, nodes), self.device, torch.int64)
-        _rows(n_nodes, "n_nodes", n, self.device)
+            _dense(masks, "masks", (n, nodes), device, torch.int64)
+        _rows(n_nodes, "n_nodes", n, device)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = torch.empty(shape, dtype=self.dtype, device=self._where)
         else:
-            _tree(out, "out", q.shape, self.device, self.dtype)
+            _dense(out, "out", shape, device, self.dtype)
         if lse is not None:
-            _tree(lse, "lse", q.shape[:3], self.device, torch.float32)
+            _dense(lse, "lse", shape[:3], device, torch.float32)
         elif want_lse:
-            lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
-        check(self._L.tg_tree_attention(self._h, layer, n, _ptr(seqs), nodes, _ptr(n_nodes), _ptr(masks), heads,
-                                        _ptr(q), qs[0], qs[1], qs[2], _ptr(k), ks[0], ks[1], ks[2], _ptr(v), vs[0], vs[1], vs[2],
-                                        1.0 / math.sqrt(self.head_dim) if scale is None else scale, _ptr(out), _ptr(lse),
-                                        _stream_ptr(stream)))
+            lse = torch.empty(shape[:3], dtype=torch.float32, device=self._where)
+        check(self._L.tg_tree_attention(self._h, layer, n, seqs.data_ptr(), nodes, address(n_nodes), address(masks), heads,
+                                        q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2],
+                                        self._scale if scale is None else scale, out.data_ptr(), address(lse),
+                                        stream_address(stream, device)))
         return out if lse is None else (out, lse)
 
     def accept(self, seqs, parents, tokens, ids, *, n_nodes=None, out_ids=None, out_n=None, stream=None):
         """tg_cache_accept: walks each tree (parents, drafted tokens [n, nodes]) with the target's ids [n, nodes] and
         keeps the accepted path in the cache.  Returns (out_ids int32 [n, nodes], out_n int32 [n])."""
-        n = _rows(seqs, "seqs", None, self.device).shape[0]
+        device = self.device
+        n = _rows(seqs, "seqs", None, device)
         shape = (n, parents.shape[1])
         for name, t in (("parents", parents), ("tokens", tokens), ("ids", ids)):
-            _tree(t, name, shape, self.device)
-        _rows(n_nodes, "n_nodes", n, self.device)
+            _dense(t, name, shape, device, torch.int32)
+        _rows(n_nodes, "n_nodes", n, device)
         if out_ids is None:
-            out_ids = torch.empty(shape, dtype=torch.int32, device=ids.device)
+            out_ids = torch.empty(shape, dtype=torch.int32, device=self._where)
+        else:
+            _dense(out_ids, "out_ids", shape, device, torch.int32)
         if out_n is None:
-            out_n = torch.empty(n, dtype=torch.int32, device=ids.device)
-        _tree(out_ids, "out_ids", shape, self.device)
-        _rows(out_n, "out_n", n, self.device)
-        check(self._L.tg_cache_accept(self._h, n, _ptr(seqs), shape[1], _ptr(n_nodes), _ptr(parents), _ptr(tokens), _ptr(ids),
-                                      _ptr(out_ids), _ptr(out_n), _stream_ptr(stream)))
+            out_n = torch.empty(n, dtype=torch.int32, device=self._where)
+        else:
+            _rows(out_n, "out_n", n, device)
+        check(self._L.tg_cache_accept(self._h, n, seqs.data_ptr(), shape[1], address(n_nodes), parents.data_ptr(), tokens.data_ptr(),
+                                      ids.data_ptr(), out_ids.data_ptr(), out_n.data_ptr(), stream_address(stream, device)))
         return out_ids, out_n

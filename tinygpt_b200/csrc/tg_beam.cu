@@ -7,8 +7,9 @@
 //
 // The candidates of a part cost the stream almost nothing: each thread keeps the
 // maximum of every 4 vectors it reads in shared memory.  The (beams + 4)-th largest of
-// the threads' own maxima bounds the part's (beams + 4)-th largest logit from below, so
-// only the few groups that reach it (about beams + 4 of thousands) are read again.
+// the maxima of 64 sets of threads bounds the part's (beams + 4)-th largest logit from
+// below, so only the few groups that reach it (1.2 to 1.5 times beams + 4, of thousands)
+// are read again.
 //
 // Order is by score in fp32, then index, while a part's list is cut by logit.  The two
 // differ only where rounding gives two different logits one score; merge_kernel looks
@@ -29,12 +30,14 @@ namespace tg {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kQuads = kThreads / 4;
 constexpr int kVecs = 4;         // 16-byte vectors of a group
 constexpr int kMaxGroups = 32;   // groups of a thread in a part
 constexpr int kListMax = 1024;   // candidates of a part before its cut
 constexpr int kExtra = 4;        // candidates past `beams`: the first one cut is then known exactly
-constexpr int kParts = 1184;     // blocks that fill the GPU: 148 SMs x 8
+constexpr int kWave = 592;       // blocks that run at a time: 148 SMs x 4
 constexpr float kLog2e = 1.44269504f;
+constexpr int kMergeSmem = 200 * 1024;
 
 constexpr uint32_t kBadState = 1, kBadHistory = 2;
 
@@ -170,7 +173,7 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(BeamArgs a) {
   using E = Elem<DT>;
   constexpr int kPer = E::kPer;
   __shared__ float group_max[kMaxGroups + 1][kThreads];
-  __shared__ float thread_max[kThreads];
+  __shared__ __align__(16) float quad_max[kQuads];
   __shared__ Candidate list[kListMax];
   __shared__ float warp_t[kThreads / 32], warp_l[kThreads / 32];
   __shared__ int n_list;
@@ -240,12 +243,7 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(BeamArgs a) {
 #pragma unroll
       for (int e = 1; e < kPer; e++) m = fmaxf(m, x[e]);
       top = fmaxf(top, m);
-    }
-#pragma unroll
-    for (int u = 0; u < kVecs; u++) {
-      float x[kPer];
-      values(g, u, now[u], x);
-      sum.add<kPer>(x, top);
+      sum.add<kPer>(x, m);
     }
     group_max[g][tid] = top;
     most = fmaxf(most, top);
@@ -260,19 +258,27 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(BeamArgs a) {
     t = s.t, l = s.l;
   }
   if ((tid & 31) == 0) warp_t[tid >> 5] = t, warp_l[tid >> 5] = l;
-  thread_max[tid] = most;
+  // the maxima of 4 threads each, 64 in all
+  float quad = fmaxf(most, __shfl_xor_sync(~0u, most, 1));
+  quad = fmaxf(quad, __shfl_xor_sync(~0u, quad, 2));
+  if ((tid & 3) == 0) quad_max[tid >> 2] = quad;
   if (tid == 0) {
     n_list = 0;
     bound = -INFINITY;
   }
   __syncthreads();
-  // the (beams + kExtra)-th largest thread maximum: each thread counts those before its own
-  int rank = 0;
-  for (int i = 0; i < kThreads; i += 4) {
-    const float4 o = *reinterpret_cast<const float4*>(&thread_max[i]);
-    rank += before(o.x, i, most, tid) + before(o.y, i + 1, most, tid) + before(o.z, i + 2, most, tid) + before(o.w, i + 3, most, tid);
+  // the (beams + kExtra)-th largest of them, which as many logits reach: each thread
+  // counts those before its own
+  if (tid < kQuads) {
+    const float mine = quad_max[tid];
+    int rank = 0;
+#pragma unroll 4
+    for (int i = 0; i < kQuads; i += 4) {
+      const float4 o = *reinterpret_cast<const float4*>(&quad_max[i]);
+      rank += before(o.x, i, mine, tid) + before(o.y, i + 1, mine, tid) + before(o.z, i + 2, mine, tid) + before(o.w, i + 3, mine, tid);
+    }
+    if (rank == a.beams + kExtra - 1) bound = mine;
   }
-  if (rank == a.beams + kExtra - 1) bound = most;
   __syncthreads();
   const float low = bound;
   const auto put = [&](float x, int id) {
@@ -405,48 +411,62 @@ __device__ void row_exact(const BeamArgs& a, int row, int w, float* lse_out, uin
 // Key 0: no candidate.
 template <int DT>
 __global__ void __launch_bounds__(kThreads) merge_kernel(BeamArgs a) {
-  extern __shared__ uint64_t keys[];  // [beams, parts, beams]
+  extern __shared__ uint64_t keys[];  // [beams, parts, beams], then PartHead [beams, parts]
   __shared__ uint64_t warp_keys[kThreads / 32], best[TG_MAX_BEAMS];
-  __shared__ float lse[TG_MAX_BEAMS];
-  __shared__ int exact[TG_MAX_BEAMS];  // 1: the row needs row_exact, 2: it had it
-  const int b = blockIdx.x, tid = threadIdx.x, W = a.beams, P = a.parts, row0 = b * W;
+  __shared__ float lse[TG_MAX_BEAMS], beam[TG_MAX_BEAMS];
+  __shared__ int live[TG_MAX_BEAMS];    // 1: the row adds candidates, 2: it goes on as it is, 0: neither
+  __shared__ int exact[TG_MAX_BEAMS];   // 1: the row needs row_exact, 2: it had it
+  __shared__ int from_row[TG_MAX_BEAMS], from_len[TG_MAX_BEAMS], grow[TG_MAX_BEAMS];
+  const int b = blockIdx.x, tid = threadIdx.x, W = a.beams, P = a.parts, row0 = b * W, lane = tid & 31;
   after_previous_work();
   const int per_row = P * W, total = W * per_row;
-  // lse of each row: a thread merges a row's parts in order, in 64 bits
+  PartHead* heads = reinterpret_cast<PartHead*>(keys + total);
   if (tid < W) {
     const int row = row0 + tid;
-    int ex = 0;
-    double top = -INFINITY, sum = 0.0;
-    if (row_scores(a, row)) {
-      if (a.state_id && a.state_id[row] >= a.num_states) atomicOr(a.status, kBadState);
-      const PartHead* h = a.heads + static_cast<int64_t>(row) * P;
-      for (int p = 0; p < P; p++) {
-        if (h[p].count < 0) ex = 1;
-        top = fmax(top, static_cast<double>(h[p].t));
-      }
-      for (int p = 0; p < P; p++)
-        if (h[p].t > -INFINITY) sum += static_cast<double>(h[p].l) * exp2(static_cast<double>(h[p].t) - top);
-    }
-    lse[tid] = top > -INFINITY ? static_cast<float>(top / static_cast<double>(kLog2e) + log(sum)) : -INFINITY;
-    exact[tid] = ex;
+    const float s = a.scores[row];
+    const bool done = a.finished && a.finished[row];
+    beam[tid] = s;
+    live[tid] = s > -INFINITY ? (done ? 2 : 1) : 0;
+    exact[tid] = 0;
+    if (a.state_id && live[tid] == 1 && a.state_id[row] >= a.num_states) atomicOr(a.status, kBadState);
   }
   __syncthreads();
+  for (int i = tid; i < W * P; i += kThreads) {
+    PartHead h{-INFINITY, 0.0f, -INFINITY, 0};
+    if (live[i / P] == 1) h = a.heads[static_cast<int64_t>(row0) * P + i];
+    heads[i] = h;
+    if (h.count < 0) exact[i / P] = 1;
+  }
+  __syncthreads();
+  // lse of a row: a warp over its parts
+  for (int w = tid >> 5; w < W; w += kThreads / 32) {
+    float top = -INFINITY, sum = 0.0f;
+    for (int p = lane; p < P; p += 32) top = fmaxf(top, heads[w * P + p].t);
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+    for (int p = lane; p < P; p += 32)
+      if (heads[w * P + p].t > -INFINITY) sum += heads[w * P + p].l * exp2_fast(heads[w * P + p].t - top);
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+    if (lane == 0) lse[w] = top > -INFINITY ? static_cast<float>(static_cast<double>(top) * (1.0 / static_cast<double>(kLog2e)) + log(static_cast<double>(sum))) : -INFINITY;
+  }
+  __syncthreads();
+  int mixed = 0;  // a list whose keys do not fall: rounding made scores equal
   for (int i = tid; i < total; i += kThreads) {
-    const int w = i / per_row, p = i % per_row / W, r = i % W, row = row0 + w;
+    const int w = i / per_row, list = i / W, r = i - list * W;
+    const auto key = [&](int at) -> uint64_t {
+      const Candidate c = a.candidates[static_cast<int64_t>(row0) * per_row + at];
+      const float s = score(c.x, lse[w], beam[w]);
+      return s > -INFINITY ? key_of(s, static_cast<uint32_t>(w) * a.vocab + c.id) : 0;
+    };
     uint64_t k = 0;
-    if (row_scores(a, row)) {
-      const int64_t at = static_cast<int64_t>(row) * P + p;
-      if (r < a.heads[at].count) {
-        const Candidate c = a.candidates[at * W + r];
-        const float s = score(c.x, lse[w], a.scores[row]);
-        if (s > -INFINITY) k = key_of(s, static_cast<uint32_t>(w) * a.vocab + c.id);
-      }
-    } else if (i % per_row == 0 && a.scores[row] > -INFINITY) {  // finished: it stays as it is
-      k = key_of(a.scores[row] + 0.0f, static_cast<uint32_t>(w) * a.vocab + a.pad_id);
+    if (live[w] == 1) {
+      if (r < heads[list].count) k = key(i);
+      if (r + 1 < heads[list].count) mixed |= key(i + 1) > k;
+    } else if (live[w] == 2 && i == w * per_row) {  // finished: it stays as it is
+      k = key_of(beam[w] + 0.0f, static_cast<uint32_t>(w) * a.vocab + a.pad_id);
     }
     keys[i] = k;
   }
-  __syncthreads();
+  mixed = __syncthreads_or(mixed);
   for (bool again = true; again;) {
     again = false;
     for (int w = 0; w < W; w++)
@@ -456,33 +476,59 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(BeamArgs a) {
         if (tid == 0) exact[w] = 2;
         __syncthreads();
       }
-    uint64_t prev = ~0ull;
-    for (int r = 0; r < W; r++) {
-      uint64_t k = 0;
-      for (int i = tid; i < total; i += kThreads) {
-        const uint64_t o = keys[i];
-        if (o < prev && o > k) k = o;
+    if (mixed) {
+      uint64_t prev = ~0ull;
+      for (int r = 0; r < W; r++) {
+        uint64_t k = 0;
+        for (int i = tid; i < total; i += kThreads) {
+          const uint64_t o = keys[i];
+          if (o < prev && o > k) k = o;
+        }
+        k = block_max(k, warp_keys);
+        if (tid == 0) best[r] = k;
+        prev = k;
       }
-      k = block_max(k, warp_keys);
-      if (tid == 0) best[r] = k;
-      prev = k;
+    } else if (tid < 32) {
+      // one warp merges the falling lists: a lane knows the best head of its lists, and
+      // looks again after one of them gave the round's winner
+      uint64_t mine = 0, prev = ~0ull;
+      bool look = true;
+      for (int r = 0; r < W; r++) {
+        if (look) {
+          mine = 0;
+          for (int list = lane; list < W * P; list += 32) {
+            int i = list * W;
+            const int end = i + W;
+            while (i < end && keys[i] >= prev) i++;  // taken
+            if (i < end && keys[i] > mine) mine = keys[i];
+          }
+        }
+        const uint32_t hi = __reduce_max_sync(~0u, static_cast<uint32_t>(mine >> 32));
+        const uint32_t lo = __reduce_max_sync(~0u, static_cast<uint32_t>(mine >> 32) == hi ? static_cast<uint32_t>(mine) : 0u);
+        prev = static_cast<uint64_t>(hi) << 32 | lo;
+        if (lane == 0) best[r] = prev;
+        if (prev == 0) {  // no more
+          if (lane == 0)
+            for (int i = r + 1; i < W; i++) best[i] = 0;
+          break;
+        }
+        look = mine == prev;
+      }
     }
     __syncthreads();
     // A logit that a list left out matters only if it has the score of one that the
     // list kept with a larger logit, and that score reaches the selection.
     const uint64_t last = best[W - 1];
     for (int i = tid; i < W * P; i += kThreads) {
-      const int w = i / P, row = row0 + w;
-      if (exact[w] || !row_scores(a, row)) continue;
-      const int64_t at = static_cast<int64_t>(row) * P + i % P;
-      const PartHead h = a.heads[at];
-      if (h.cut == -INFINITY || h.count <= 0) continue;
+      const int w = i / P;
+      const PartHead h = heads[i];
+      if (exact[w] || live[w] != 1 || h.cut == -INFINITY || h.count <= 0) continue;
       // the list's kept logits with the cut one's score, if any, are at its end
-      const float s = score(h.cut, lse[w], a.scores[row]);
+      const float s = score(h.cut, lse[w], beam[w]);
       if (!(s > -INFINITY) || (last != 0 && s < score_of(last))) continue;
       for (int r = h.count - 1; r >= 0; r--) {
-        const Candidate c = a.candidates[at * W + r];
-        if (score(c.x, lse[w], a.scores[row]) != s) break;
+        const Candidate c = a.candidates[(static_cast<int64_t>(row0) * P + i) * W + r];
+        if (score(c.x, lse[w], beam[w]) != s) break;
         if (c.x != h.cut) {
           exact[w] = 1;
           break;
@@ -501,33 +547,53 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(BeamArgs a) {
     a.out_parent[at] = parent;
     a.out_token[at] = token;
     a.out_score[at] = k ? score_of(k) : -INFINITY;
-    const bool was = k && a.finished && a.finished[row0 + parent];
+    const bool was = k && live[parent] == 2;
     if (a.out_finished) a.out_finished[at] = !k || was || (a.eos_id >= 0 && token == a.eos_id);
+    if (a.history) {
+      int len = k ? a.history_len[row0 + parent] : 0;
+      if (len < 0 || len > a.history_stride) {
+        atomicOr(a.status, kBadHistory);
+        len = min(max(len, 0), a.history_stride);
+      }
+      const bool more = k && len < a.history_stride && !was;
+      a.out_history_len[at] = len + more;
+      from_row[tid] = row0 + max(parent, 0);
+      from_len[tid] = len;
+      grow[tid] = more ? token : -1;
+    }
   }
   if (!a.history) return;
-  for (int w = 0; w < W; w++) {
-    const uint64_t k = best[w];
-    const uint32_t index = index_of(k);
-    const int parent = k ? static_cast<int>(index / a.vocab) : 0, token = static_cast<int>(index % a.vocab);
-    const int32_t* from = a.history + static_cast<int64_t>(row0 + parent) * a.history_stride;
+  __syncthreads();
+  // a warp per 512 entries of a history, 16 loads on their way per lane
+  const int pieces = (a.history_stride + 511) / 512;
+  for (int u = tid >> 5; u < W * pieces; u += kThreads / 32) {
+    const int w = u / pieces, j0 = (u - w * pieces) * 512 + lane, len = from_len[w];
+    const int32_t* from = a.history + static_cast<int64_t>(from_row[w]) * a.history_stride;
     int32_t* to = a.out_history + static_cast<int64_t>(row0 + w) * a.history_stride;
-    int len = k ? a.history_len[row0 + parent] : 0;
-    if (len < 0 || len > a.history_stride) {
-      if (tid == 0) atomicOr(a.status, kBadHistory);
-      len = min(max(len, 0), a.history_stride);
-    }
-    const bool grow = k && len < a.history_stride && !(a.finished && a.finished[row0 + parent]);
-    for (int j = tid; j < a.history_stride; j += kThreads) to[j] = j < len ? from[j] : (j == len && grow ? token : -1);
-    if (tid == 0) a.out_history_len[row0 + w] = len + grow;
+    int32_t x[16];
+#pragma unroll
+    for (int e = 0; e < 16; e++) x[e] = j0 + 32 * e < len ? from[j0 + 32 * e] : j0 + 32 * e == len ? grow[w] : -1;
+#pragma unroll
+    for (int e = 0; e < 16; e++)
+      if (j0 + 32 * e < a.history_stride) to[j0 + 32 * e] = x[e];
   }
 }
 
-// Parts of a row: enough blocks to fill the GPU, none with less than one group per
-// thread, and no more groups than a block keeps.
+// Parts of a row.  Few rows: as many as fill one wave of blocks, none with less than one
+// group per thread.  More rows than that: the number from 1 to 4 that leaves the last wave
+// fullest.  Never more groups than a block keeps.
 int parts_of(int vocab, int per, int rows) {
   const int step = kThreads * kVecs * per;  // elements of one group of every thread
   const int most = (vocab + step - 1) / step, least = (most + kMaxGroups - 1) / kMaxGroups;
-  int p = kParts / rows;
+  int p = kWave / rows;
+  if (rows > kWave / 4) {
+    double fullest = 0.0;
+    for (int i = 1; i <= 4; i++) {
+      const int waves = (rows * i + kWave - 1) / kWave;
+      const double full = static_cast<double>(rows) * i / (static_cast<double>(waves) * kWave);
+      if (full > fullest + 0.02) fullest = full, p = i;
+    }
+  }
   if (p > most) p = most;
   if (p < least) p = least;
   return p < 1 ? 1 : p;
@@ -578,8 +644,9 @@ int32_t tg_beam_create(int32_t device, int32_t vocab, int32_t beams, int32_t max
   h->beams = beams;
   h->max_batch = max_batch;
   const size_t rows = static_cast<size_t>(max_batch) * beams;
-  const size_t least = tg::parts_of(vocab, 4, tg::kParts * 2);  // the parts of a row when rows are many
-  h->slots = rows * least > tg::kParts + rows ? rows * least : tg::kParts + rows;
+  // the parts of any number of rows up to `rows`: at most 4 each, or one wave, or what a block's groups ask for
+  const size_t least = tg::parts_of(vocab, 4, 1 << 20);
+  h->slots = rows * (least > 4 ? least : 4) + tg::kWave;
   char* base = nullptr;
   const size_t list_bytes = h->slots * beams * sizeof(tg::Candidate);
   cudaError_t e = cudaMalloc(&base, h->slots * sizeof(tg::PartHead) + list_bytes + 4);
@@ -589,9 +656,8 @@ int32_t tg_beam_create(int32_t device, int32_t vocab, int32_t beams, int32_t max
     h->status = reinterpret_cast<uint32_t*>(base + h->slots * sizeof(tg::PartHead) + list_bytes);
     e = cudaMemset(h->status, 0, 4);
   }
-  const int smem = TG_MAX_BEAMS * 1024 * 8 > 200 * 1024 ? 200 * 1024 : TG_MAX_BEAMS * 1024 * 8;
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(tg::merge_kernel<TG_DTYPE_F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(tg::merge_kernel<TG_DTYPE_BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(tg::merge_kernel<TG_DTYPE_F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, tg::kMergeSmem);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(tg::merge_kernel<TG_DTYPE_BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, tg::kMergeSmem);
   if (e == cudaSuccess) e = cudaDeviceSynchronize();  // calls may come on any stream
   if (e != cudaSuccess) {
     tg_beam_destroy(h);
@@ -658,10 +724,10 @@ int32_t tg_beam_select(tg_beam* h, const void* logits, int32_t dtype, int64_t ro
   a.heads = h->heads;
   a.candidates = h->candidates;
   a.status = h->status;
-  // the merge holds beams x parts x beams keys in shared memory
-  const size_t most = 200 * 1024 / 8 / (static_cast<size_t>(h->beams) * h->beams);
+  // the merge holds beams x parts x beams keys, and the parts' heads, in shared memory
+  const size_t per_part = static_cast<size_t>(a.beams) * a.beams * 8 + a.beams * sizeof(tg::PartHead), most = tg::kMergeSmem / per_part;
   if (static_cast<size_t>(a.parts) > most) a.parts = static_cast<int>(most);
-  const size_t smem = static_cast<size_t>(a.beams) * a.parts * a.beams * 8;
+  const size_t smem = a.parts * per_part;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 grid(a.parts, batch * h->beams);
   if (dtype == TG_DTYPE_F32) {
