@@ -30,6 +30,7 @@ namespace tg {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kMergeThreads = 512;
 constexpr int kQuads = kThreads / 4;
 constexpr int kVecs = 4;         // 16-byte vectors of a group
 constexpr int kMaxGroups = 32;   // groups of a thread in a part
@@ -37,6 +38,7 @@ constexpr int kListMax = 1024;   // candidates of a part before its cut
 constexpr int kExtra = 4;        // candidates past `beams`: the first one cut is then known exactly
 constexpr int kWave = 592;       // blocks that run at a time: 148 SMs x 4
 constexpr float kLog2e = 1.44269504f;
+constexpr int kKeep = TG_MAX_BEAMS * TG_MAX_BEAMS;  // keys that the merge ranks
 constexpr int kMergeSmem = 200 * 1024;
 
 constexpr uint32_t kBadState = 1, kBadHistory = 2;
@@ -102,6 +104,21 @@ struct Elem<TG_DTYPE_F32> {
     x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
   }
   static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+  static __device__ __forceinline__ uint4 masked(const uint4& v, uint32_t bits) {
+    return make_uint4(bits & 1 ? v.x : 0xff800000u, bits & 2 ? v.y : 0xff800000u, bits & 4 ? v.z : 0xff800000u, bits & 8 ? v.w : 0xff800000u);
+  }
+  // the largest of N vectors; NaN does not count
+  template <int N>
+  static __device__ __forceinline__ float most(const uint4* d) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < N; v++) {
+      float x[4];
+      unpack(d[v], x);
+      m = fmaxf(fmaxf(m, fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
+    }
+    return m;
+  }
 };
 template <>
 struct Elem<TG_DTYPE_BF16> {
@@ -117,6 +134,24 @@ struct Elem<TG_DTYPE_BF16> {
     }
   }
   static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+  static __device__ __forceinline__ uint32_t masked_word(uint32_t w, uint32_t bits) {
+    return (bits & 1 ? w & 0xffffu : 0xff80u) | (bits & 2 ? w & 0xffff0000u : 0xff800000u);
+  }
+  static __device__ __forceinline__ uint4 masked(const uint4& v, uint32_t bits) {
+    return make_uint4(masked_word(v.x, bits), masked_word(v.y, bits >> 2), masked_word(v.z, bits >> 4), masked_word(v.w, bits >> 6));
+  }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t m;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+    return m;
+  }
+  template <int N>
+  static __device__ __forceinline__ float most(const uint4* d) {
+    uint32_t m = 0xff80ff80u;
+#pragma unroll
+    for (int v = 0; v < N; v++) m = max2(max2(m, max2(d[v].x, d[v].y)), max2(d[v].z, d[v].w));
+    return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+  }
 };
 
 __device__ __forceinline__ uint4 load_stream(const uint4* p) {
@@ -133,38 +168,66 @@ __device__ __forceinline__ uint32_t mask_bits(const uint32_t* mask, int v) {
   return __funnelshift_r(lo, hi, v & 31);
 }
 
+__device__ __forceinline__ uint64_t two(float lo, float hi) { return static_cast<uint64_t>(__float_as_uint(hi)) << 32 | __float_as_uint(lo); }
+__device__ __forceinline__ float low_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float high_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // sum 2^(x log2e - t), rescaled when a group exceeds t: t is a rounded x log2e, so
 // every term is at most about 1, and lse = t / log2e + ln(sum) has no error from the
 // rounding of t.
 struct Sum {
   float t = -INFINITY, l = 0.0f;
-  template <int N>
-  __device__ __forceinline__ void add(const float* x, float top) {
+  __device__ __forceinline__ void raise(float top) {
     const float at = top * kLog2e;
     if (at > t) {
       l *= exp2_fast(t - at);
       t = at;
     }
-    if (top > -INFINITY) {
-      float s0 = 0.0f, s1 = 0.0f;
-#pragma unroll
-      for (int i = 0; i < N; i += 2) {
-        s0 += exp2_fast(__fmaf_rn(x[i], kLog2e, -t));
-        s1 += exp2_fast(__fmaf_rn(x[i + 1], kLog2e, -t));
-      }
-      l += s0 + s1;
-    }
   }
-  __device__ __forceinline__ void merge(float t2, float l2) {
-    if (t2 == -INFINITY) return;
-    if (t2 > t) {
-      l = l * exp2_fast(t - t2) + l2;
-      t = t2;
-    } else {
-      l += l2 * exp2_fast(t2 - t);
+  __device__ __forceinline__ void add(float x, float top) {
+    raise(top);
+    if (top > -INFINITY) l += exp2_fast(__fmaf_rn(x, kLog2e, -t));
+  }
+  // N vectors, whose largest is `top`; two elements an instruction where it exists
+  template <typename E, int N>
+  __device__ __forceinline__ void add(const uint4* d, float top) {
+    raise(top);
+    if (!(top > -INFINITY)) return;
+    const uint64_t scale = two(kLog2e, kLog2e), from = two(-t, -t);
+    uint64_t s[2] = {0, 0};
+#pragma unroll
+    for (int v = 0; v < N; v++) {
+      float x[E::kPer];
+      E::unpack(d[v], x);
+#pragma unroll
+      for (int i = 0; i < E::kPer; i += 2) {
+        const uint64_t y = fma2(two(x[i], x[i + 1]), scale, from);
+        s[i / 2 & 1] = add2(s[i / 2 & 1], two(exp2_fast(low_of(y)), exp2_fast(high_of(y))));
+      }
     }
+    s[0] = add2(s[0], s[1]);
+    l += low_of(s[0]) + high_of(s[0]);
   }
 };
+
+// The 32 lanes' sums as one, in every lane.
+__device__ __forceinline__ void join_lanes(Sum& s) {
+  float t = s.t;
+  for (int d = 16; d; d >>= 1) t = fmaxf(t, __shfl_xor_sync(~0u, t, d));
+  float l = s.t > -INFINITY ? s.l * exp2_fast(s.t - t) : 0.0f;
+  for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(~0u, l, d);
+  s.t = t, s.l = l;
+}
 
 __device__ __forceinline__ bool before(float xa, int ia, float xb, int ib) { return xa > xb || (xa == xb && ia < ib); }
 
@@ -175,8 +238,9 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(BeamArgs a) {
   __shared__ float group_max[kMaxGroups + 1][kThreads];
   __shared__ __align__(16) float quad_max[kQuads];
   __shared__ Candidate list[kListMax];
+  __shared__ int32_t hits[kListMax];  // groups to read again: group * kThreads + thread
   __shared__ float warp_t[kThreads / 32], warp_l[kThreads / 32];
-  __shared__ int n_list;
+  __shared__ int n_list, n_hits;
   __shared__ float bound;
   const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
   after_previous_work();
@@ -205,8 +269,7 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(BeamArgs a) {
   if (odd >= 0 && allowed(mask, odd)) {
     odd_x = fmaxf(E::get(p + odd), -INFINITY);  // NaN: -inf
     const float raw = E::get(p + odd);
-    const float two[2] = {raw, -INFINITY};
-    sum.add<2>(two, odd_x);
+    sum.add(raw, odd_x);
   }
   group_max[groups][tid] = odd_x;
   most = odd_x;
@@ -218,14 +281,16 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(BeamArgs a) {
       d[u] = i < v1 ? load_stream(pv + i) : E::nothing();
     }
   };
-  const auto values = [&](int g, int u, const uint4& d, float* x) {
-    E::unpack(d, x);
-    if (kMasked && mask) {
-      const int i = v0 + (g * kVecs + u) * kThreads + tid;
-      const uint32_t bits = i < v1 ? mask_bits<kPer>(mask, head + i * kPer) : 0;
+  const auto mask_group = [&](int g, uint4* d) {
+    if (!kMasked || !mask) return;
+    uint32_t bits[kVecs];
 #pragma unroll
-      for (int e = 0; e < kPer; e++) x[e] = bits >> e & 1 ? x[e] : -INFINITY;
+    for (int u = 0; u < kVecs; u++) {
+      const int i = v0 + (g * kVecs + u) * kThreads + tid;
+      bits[u] = i < v1 ? mask_bits<kPer>(mask, head + i * kPer) : 0;
     }
+#pragma unroll
+    for (int u = 0; u < kVecs; u++) d[u] = E::masked(d[u], bits[u]);
   };
   uint4 next[kVecs];
   if (groups > 0) fetch(0, next);
@@ -234,36 +299,20 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(BeamArgs a) {
 #pragma unroll
     for (int u = 0; u < kVecs; u++) now[u] = next[u];
     if (g + 1 < groups) fetch(g + 1, next);
-    float top = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < kVecs; u++) {
-      float x[kPer];
-      values(g, u, now[u], x);
-      float m = x[0];
-#pragma unroll
-      for (int e = 1; e < kPer; e++) m = fmaxf(m, x[e]);
-      top = fmaxf(top, m);
-      sum.add<kPer>(x, m);
-    }
+    mask_group(g, now);
+    const float top = E::template most<kVecs>(now);
+    sum.add<E, kVecs>(now, top);
     group_max[g][tid] = top;
     most = fmaxf(most, top);
   }
-  // the part's sum
-  float t = sum.t, l = sum.l;
-  for (int d = 16; d; d >>= 1) {
-    const float t2 = __shfl_xor_sync(~0u, t, d), l2 = __shfl_xor_sync(~0u, l, d);
-    Sum s;
-    s.t = t, s.l = l;
-    s.merge(t2, l2);
-    t = s.t, l = s.l;
-  }
-  if ((tid & 31) == 0) warp_t[tid >> 5] = t, warp_l[tid >> 5] = l;
+  join_lanes(sum);
+  if ((tid & 31) == 0) warp_t[tid >> 5] = sum.t, warp_l[tid >> 5] = sum.l;
   // the maxima of 4 threads each, 64 in all
   float quad = fmaxf(most, __shfl_xor_sync(~0u, most, 1));
   quad = fmaxf(quad, __shfl_xor_sync(~0u, quad, 2));
   if ((tid & 3) == 0) quad_max[tid >> 2] = quad;
   if (tid == 0) {
-    n_list = 0;
+    n_list = n_hits = 0;
     bound = -INFINITY;
   }
   __syncthreads();
@@ -280,31 +329,37 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(BeamArgs a) {
     if (rank == a.beams + kExtra - 1) bound = mine;
   }
   __syncthreads();
+  // the groups that reach it, then their vectors, one per thread: all re-reads at once
   const float low = bound;
+  if (most >= low && most > -INFINITY)
+    for (int g = 0; g < groups; g++) {
+      const float top = group_max[g][tid];
+      if (top >= low && top > -INFINITY) {
+        const int at = atomicAdd(&n_hits, 1);
+        if (at < kListMax) hits[at] = g * kThreads + tid;
+      }
+    }
+  __syncthreads();
   const auto put = [&](float x, int id) {
     const int at = atomicAdd(&n_list, 1);
     if (at < kListMax) list[at] = Candidate{x, id};
   };
-  if (most >= low && most > -INFINITY) {
-    for (int g = 0; g < groups; g++) {
-      const float top = group_max[g][tid];
-      if (!(top >= low && top > -INFINITY)) continue;
-      uint4 d[kVecs];
-      fetch(g, d);
+  const int n_groups = min(n_hits, kListMax);
+  for (int h = tid; h < n_groups * kVecs; h += kThreads) {
+    const int hit = hits[h / kVecs], i = v0 + (hit / kThreads * kVecs + h % kVecs) * kThreads + hit % kThreads;
+    if (i >= v1) continue;
+    uint4 d = load_stream(pv + i);
+    const int id = head + i * kPer;
+    if (kMasked && mask) d = E::masked(d, mask_bits<kPer>(mask, id));
+    float x[kPer];
+    E::unpack(d, x);
 #pragma unroll
-      for (int u = 0; u < kVecs; u++) {
-        float x[kPer];
-        values(g, u, d[u], x);
-        const int id = head + (v0 + (g * kVecs + u) * kThreads + tid) * kPer;
-#pragma unroll
-        for (int e = 0; e < kPer; e++)
-          if (x[e] >= low && x[e] > -INFINITY) put(x[e], id + e);
-      }
-    }
-    if (odd_x >= low && odd_x > -INFINITY) put(odd_x, odd);
+    for (int e = 0; e < kPer; e++)
+      if (x[e] >= low && x[e] > -INFINITY) put(x[e], id + e);
   }
+  if (odd_x >= low && odd_x > -INFINITY) put(odd_x, odd);
   __syncthreads();
-  const int n = n_list, kept = min(n, a.beams);
+  const int n = n_hits > kListMax ? kListMax + 1 : n_list, kept = min(n, a.beams);  // a group has one at least
   const int64_t at = static_cast<int64_t>(row) * a.parts + part;
   if (n <= kListMax) {
     for (int i = tid; i < n; i += kThreads) {
@@ -316,14 +371,16 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(BeamArgs a) {
     }
     if (tid == 0 && n <= a.beams) a.heads[at].cut = -INFINITY;
   }
-  if (tid == 0) {
+  if (tid < 32) {
     Sum s;
-    s.t = warp_t[0], s.l = warp_l[0];
-    for (int w = 1; w < kThreads / 32; w++) s.merge(warp_t[w], warp_l[w]);
-    a.heads[at].t = s.t;
-    a.heads[at].l = s.l;
-    // NaN, +inf or logits beyond the range of x log2e in the part: its sum is not finite
-    a.heads[at].count = n <= kListMax && s.l < INFINITY && s.t < INFINITY ? kept : -1;
+    if (tid < kThreads / 32) s.t = warp_t[tid], s.l = warp_l[tid];
+    join_lanes(s);
+    if (tid == 0) {
+      a.heads[at].t = s.t;
+      a.heads[at].l = s.l;
+      // NaN, +inf or logits beyond the range of x log2e in the part: its sum is not finite
+      a.heads[at].count = n <= kListMax && s.l < INFINITY && s.t < INFINITY ? kept : -1;
+    }
   }
 }
 
@@ -352,7 +409,7 @@ __device__ uint64_t block_max(uint64_t k, uint64_t* warp_keys) {
   if ((threadIdx.x & 31) == 0) warp_keys[threadIdx.x >> 5] = k;
   __syncthreads();
   uint64_t best = 0;
-  for (int w = 0; w < kThreads / 32; w++) best = warp_keys[w] > best ? warp_keys[w] : best;
+  for (int w = 0; w < kMergeThreads / 32; w++) best = warp_keys[w] > best ? warp_keys[w] : best;
   return best;
 }
 
@@ -370,25 +427,25 @@ __device__ void row_exact(const BeamArgs& a, int row, int w, float* lse_out, uin
   const uint32_t* mask = row_mask(a, row);
   const int tid = threadIdx.x;
   float top = -INFINITY;
-  for (int v = tid; v < a.vocab; v += kThreads) top = fmaxf(top, logit<DT>(p, mask, v));
+  for (int v = tid; v < a.vocab; v += kMergeThreads) top = fmaxf(top, logit<DT>(p, mask, v));
   top = score_of(block_max(key_of(top, 0), warp_keys));
   double sum = 0.0;
   if (top > -INFINITY)
-    for (int v = tid; v < a.vocab; v += kThreads) sum += exp(static_cast<double>(logit<DT>(p, mask, v)) - static_cast<double>(top));
+    for (int v = tid; v < a.vocab; v += kMergeThreads) sum += exp(static_cast<double>(logit<DT>(p, mask, v)) - static_cast<double>(top));
   // the block's sum, in a fixed order
   for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
   __syncthreads();
   if ((tid & 31) == 0) warp_keys[tid >> 5] = __double_as_longlong(sum);
   __syncthreads();
   sum = 0.0;
-  for (int i = 0; i < kThreads / 32; i++) sum += __longlong_as_double(warp_keys[i]);
+  for (int i = 0; i < kMergeThreads / 32; i++) sum += __longlong_as_double(warp_keys[i]);
   const float lse = static_cast<float>(static_cast<double>(top) + log(sum));
   const float beam = a.scores[row];
   uint64_t prev = ~0ull;
   for (int r = 0; r < a.beams; r++) {
     uint64_t best = 0;
     if (top > -INFINITY)
-      for (int v = tid; v < a.vocab; v += kThreads) {
+      for (int v = tid; v < a.vocab; v += kMergeThreads) {
         const float x = logit<DT>(p, mask, v);
         if (x == -INFINITY) continue;
         const float s = score(x, lse, beam);
@@ -400,7 +457,7 @@ __device__ void row_exact(const BeamArgs& a, int row, int w, float* lse_out, uin
     if (tid == 0) keys[r] = best;
     prev = best;
     if (best == 0) {  // no more: the same for every thread
-      for (int i = r + 1 + tid; i < a.beams; i += kThreads) keys[i] = 0;
+      for (int i = r + 1 + tid; i < a.beams; i += kMergeThreads) keys[i] = 0;
       break;
     }
   }
@@ -410,10 +467,11 @@ __device__ void row_exact(const BeamArgs& a, int row, int w, float* lse_out, uin
 
 // Key 0: no candidate.
 template <int DT>
-__global__ void __launch_bounds__(kThreads) merge_kernel(BeamArgs a) {
+__global__ void __launch_bounds__(kMergeThreads) merge_kernel(BeamArgs a) {
   extern __shared__ uint64_t keys[];  // [beams, parts, beams], then PartHead [beams, parts]
-  __shared__ uint64_t warp_keys[kThreads / 32], best[TG_MAX_BEAMS];
-  __shared__ float lse[TG_MAX_BEAMS], beam[TG_MAX_BEAMS];
+  __shared__ uint64_t warp_keys[kMergeThreads / 32], best[TG_MAX_BEAMS], keep[kKeep], bound;
+  __shared__ int n_keys;
+  __shared__ float lse[TG_MAX_BEAMS], row_sum[TG_MAX_BEAMS], beam[TG_MAX_BEAMS];
   __shared__ int live[TG_MAX_BEAMS];    // 1: the row adds candidates, 2: it goes on as it is, 0: neither
   __shared__ int exact[TG_MAX_BEAMS];   // 1: the row needs row_exact, 2: it had it
   __shared__ int from_row[TG_MAX_BEAMS], from_len[TG_MAX_BEAMS], grow[TG_MAX_BEAMS];
@@ -421,6 +479,9 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(BeamArgs a) {
   after_previous_work();
   const int per_row = P * W, total = W * per_row;
   PartHead* heads = reinterpret_cast<PartHead*>(keys + total);
+  // what the first key of each thread needs, on its way while the heads are read
+  Candidate first{0.0f, 0};
+  if (tid < total) first = a.candidates[static_cast<int64_t>(row0) * per_row + tid];
   if (tid < W) {
     const int row = row0 + tid;
     const float s = a.scores[row];
@@ -430,57 +491,89 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(BeamArgs a) {
     exact[tid] = 0;
     if (a.state_id && live[tid] == 1 && a.state_id[row] >= a.num_states) atomicOr(a.status, kBadState);
   }
+  for (int i = tid; i < W * P; i += kMergeThreads) heads[i] = a.heads[static_cast<int64_t>(row0) * P + i];
   __syncthreads();
-  for (int i = tid; i < W * P; i += kThreads) {
-    PartHead h{-INFINITY, 0.0f, -INFINITY, 0};
-    if (live[i / P] == 1) h = a.heads[static_cast<int64_t>(row0) * P + i];
-    heads[i] = h;
-    if (h.count < 0) exact[i / P] = 1;
+  for (int i = tid; i < W * P; i += kMergeThreads) {
+    if (live[i / P] != 1) heads[i] = PartHead{-INFINITY, 0.0f, -INFINITY, 0};
+    if (heads[i].count < 0) exact[i / P] = 1;
   }
   __syncthreads();
-  // lse of a row: a warp over its parts
-  for (int w = tid >> 5; w < W; w += kThreads / 32) {
+  // lse of a row: a warp adds its parts, a thread takes the logarithm
+  for (int w = tid >> 5; w < W; w += kMergeThreads / 32) {
     float top = -INFINITY, sum = 0.0f;
     for (int p = lane; p < P; p += 32) top = fmaxf(top, heads[w * P + p].t);
     for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
     for (int p = lane; p < P; p += 32)
       if (heads[w * P + p].t > -INFINITY) sum += heads[w * P + p].l * exp2_fast(heads[w * P + p].t - top);
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-    if (lane == 0) lse[w] = top > -INFINITY ? static_cast<float>(static_cast<double>(top) * (1.0 / static_cast<double>(kLog2e)) + log(static_cast<double>(sum))) : -INFINITY;
+    if (lane == 0) lse[w] = top, row_sum[w] = sum;
   }
   __syncthreads();
-  int mixed = 0;  // a list whose keys do not fall: rounding made scores equal
-  for (int i = tid; i < total; i += kThreads) {
+  if (tid < W && lse[tid] > -INFINITY)
+    lse[tid] = static_cast<float>(static_cast<double>(lse[tid]) * (1.0 / static_cast<double>(kLog2e)) + log(static_cast<double>(row_sum[tid])));
+  __syncthreads();
+  for (int i = tid; i < total; i += kMergeThreads) {
     const int w = i / per_row, list = i / W, r = i - list * W;
-    const auto key = [&](int at) -> uint64_t {
-      const Candidate c = a.candidates[static_cast<int64_t>(row0) * per_row + at];
-      const float s = score(c.x, lse[w], beam[w]);
-      return s > -INFINITY ? key_of(s, static_cast<uint32_t>(w) * a.vocab + c.id) : 0;
-    };
     uint64_t k = 0;
     if (live[w] == 1) {
-      if (r < heads[list].count) k = key(i);
-      if (r + 1 < heads[list].count) mixed |= key(i + 1) > k;
+      if (r < heads[list].count) {
+        const Candidate c = i == tid ? first : a.candidates[static_cast<int64_t>(row0) * per_row + i];
+        const float s = score(c.x, lse[w], beam[w]);
+        if (s > -INFINITY) k = key_of(s, static_cast<uint32_t>(w) * a.vocab + c.id);
+      }
     } else if (live[w] == 2 && i == w * per_row) {  // finished: it stays as it is
       k = key_of(beam[w] + 0.0f, static_cast<uint32_t>(w) * a.vocab + a.pad_id);
     }
     keys[i] = k;
   }
-  mixed = __syncthreads_or(mixed);
+  __syncthreads();
   for (bool again = true; again;) {
     again = false;
     for (int w = 0; w < W; w++)
       if (exact[w] == 1) {  // the same for every thread
-        for (int i = W + tid; i < per_row; i += kThreads) keys[w * per_row + i] = 0;
+        for (int i = W + tid; i < per_row; i += kMergeThreads) keys[w * per_row + i] = 0;
         row_exact<DT>(a, row0 + w, w, &lse[w], keys + w * per_row, warp_keys);
         if (tid == 0) exact[w] = 2;
         __syncthreads();
       }
-    if (mixed) {
+    // The beams-th best of the lists' first keys is a bound: lists fall but for rounding,
+    // so at most about beams * beams keys reach it.  Each counts those before it.
+    if (tid == 0) n_keys = 0, bound = 0;
+    if (tid < W) best[tid] = 0;
+    __syncthreads();
+    for (int i = tid; i < W * P; i += kMergeThreads) {
+      const uint64_t k = keys[i * W];
+      int r = 0;
+      if (k != 0) {
+#pragma unroll 4
+        for (int j = 0; j < W * P; j++) r += keys[j * W] > k;
+        if (r == W - 1) bound = k;
+      }
+    }
+    __syncthreads();
+    for (int i0 = 0; i0 < total; i0 += kMergeThreads) {
+      const uint64_t k = i0 + tid < total ? keys[i0 + tid] : 0;
+      const bool in = k != 0 && k >= bound;
+      const uint32_t all = __ballot_sync(~0u, in);
+      int at = 0;
+      if (lane == 0 && all) at = atomicAdd(&n_keys, __popc(all));
+      at = __shfl_sync(~0u, at, 0) + __popc(all & ((1u << lane) - 1));
+      if (in && at < kKeep) keep[at] = k;
+    }
+    __syncthreads();
+    if (n_keys <= kKeep) {
+      for (int i = tid; i < n_keys; i += kMergeThreads) {
+        const uint64_t k = keep[i];
+        int r = 0;
+#pragma unroll 4
+        for (int j = 0; j < n_keys; j++) r += keep[j] > k;
+        if (r < W) best[r] = k;
+      }
+    } else {
       uint64_t prev = ~0ull;
       for (int r = 0; r < W; r++) {
         uint64_t k = 0;
-        for (int i = tid; i < total; i += kThreads) {
+        for (int i = tid; i < total; i += kMergeThreads) {
           const uint64_t o = keys[i];
           if (o < prev && o > k) k = o;
         }
@@ -488,38 +581,12 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(BeamArgs a) {
         if (tid == 0) best[r] = k;
         prev = k;
       }
-    } else if (tid < 32) {
-      // one warp merges the falling lists: a lane knows the best head of its lists, and
-      // looks again after one of them gave the round's winner
-      uint64_t mine = 0, prev = ~0ull;
-      bool look = true;
-      for (int r = 0; r < W; r++) {
-        if (look) {
-          mine = 0;
-          for (int list = lane; list < W * P; list += 32) {
-            int i = list * W;
-            const int end = i + W;
-            while (i < end && keys[i] >= prev) i++;  // taken
-            if (i < end && keys[i] > mine) mine = keys[i];
-          }
-        }
-        const uint32_t hi = __reduce_max_sync(~0u, static_cast<uint32_t>(mine >> 32));
-        const uint32_t lo = __reduce_max_sync(~0u, static_cast<uint32_t>(mine >> 32) == hi ? static_cast<uint32_t>(mine) : 0u);
-        prev = static_cast<uint64_t>(hi) << 32 | lo;
-        if (lane == 0) best[r] = prev;
-        if (prev == 0) {  // no more
-          if (lane == 0)
-            for (int i = r + 1; i < W; i++) best[i] = 0;
-          break;
-        }
-        look = mine == prev;
-      }
     }
     __syncthreads();
     // A logit that a list left out matters only if it has the score of one that the
     // list kept with a larger logit, and that score reaches the selection.
     const uint64_t last = best[W - 1];
-    for (int i = tid; i < W * P; i += kThreads) {
+    for (int i = tid; i < W * P; i += kMergeThreads) {
       const int w = i / P;
       const PartHead h = heads[i];
       if (exact[w] || live[w] != 1 || h.cut == -INFINITY || h.count <= 0) continue;
@@ -527,8 +594,9 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(BeamArgs a) {
       const float s = score(h.cut, lse[w], beam[w]);
       if (!(s > -INFINITY) || (last != 0 && s < score_of(last))) continue;
       for (int r = h.count - 1; r >= 0; r--) {
+        const uint64_t k = keys[i * W + r];
+        if (k == 0 || score_of(k) != s) break;
         const Candidate c = a.candidates[(static_cast<int64_t>(row0) * P + i) * W + r];
-        if (score(c.x, lse[w], beam[w]) != s) break;
         if (c.x != h.cut) {
           exact[w] = 1;
           break;
@@ -566,7 +634,7 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(BeamArgs a) {
   __syncthreads();
   // a warp per 512 entries of a history, 16 loads on their way per lane
   const int pieces = (a.history_stride + 511) / 512;
-  for (int u = tid >> 5; u < W * pieces; u += kThreads / 32) {
+  for (int u = tid >> 5; u < W * pieces; u += kMergeThreads / 32) {
     const int w = u / pieces, j0 = (u - w * pieces) * 512 + lane, len = from_len[w];
     const int32_t* from = a.history + static_cast<int64_t>(from_row[w]) * a.history_stride;
     int32_t* to = a.out_history + static_cast<int64_t>(row0 + w) * a.history_stride;
@@ -579,24 +647,22 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(BeamArgs a) {
   }
 }
 
-// Parts of a row.  Few rows: as many as fill one wave of blocks, none with less than one
-// group per thread.  More rows than that: the number from 1 to 4 that leaves the last wave
-// fullest.  Never more groups than a block keeps.
+// Parts of a row: the number with the least waves x (groups of a part + 3.5), since what
+// follows a part's last group takes as long as 3.5 groups (9,000 of 2,700 cycles with 4
+// blocks on an SM).  1024 rows of 16 groups: 64 us in one part, 87 in four; 4 rows of 7
+// groups: 10.3 us in 7 parts.  Never more groups than a block keeps.
 int parts_of(int vocab, int per, int rows) {
   const int step = kThreads * kVecs * per;  // elements of one group of every thread
   const int most = (vocab + step - 1) / step, least = (most + kMaxGroups - 1) / kMaxGroups;
-  int p = kWave / rows;
-  if (rows > kWave / 4) {
-    double fullest = 0.0;
-    for (int i = 1; i <= 4; i++) {
-      const int waves = (rows * i + kWave - 1) / kWave;
-      const double full = static_cast<double>(rows) * i / (static_cast<double>(waves) * kWave);
-      if (full > fullest + 0.02) fullest = full, p = i;
-    }
+  const int limit = kWave / rows > 4 ? kWave / rows : 4;
+  int best = least;
+  float cost = FLT_MAX;
+  for (int p = least; p <= most && (p <= limit || p == least); p++) {
+    const float waves = static_cast<float>((static_cast<int64_t>(rows) * p + kWave - 1) / kWave);
+    const float c = waves * (static_cast<float>((most + p - 1) / p) + 3.5f);
+    if (c < cost) cost = c, best = p;
   }
-  if (p > most) p = most;
-  if (p < least) p = least;
-  return p < 1 ? 1 : p;
+  return best;
 }
 
 }  // namespace
@@ -732,10 +798,10 @@ int32_t tg_beam_select(tg_beam* h, const void* logits, int32_t dtype, int64_t ro
   const dim3 grid(a.parts, batch * h->beams);
   if (dtype == TG_DTYPE_F32) {
     TG_TRY(tg::launch_after(state_id ? tg::scan_kernel<TG_DTYPE_F32, true> : tg::scan_kernel<TG_DTYPE_F32, false>, grid, tg::kThreads, 0, st, 1, a));
-    TG_TRY(tg::launch_after(tg::merge_kernel<TG_DTYPE_F32>, dim3(batch), tg::kThreads, smem, st, 1, a));
+    TG_TRY(tg::launch_after(tg::merge_kernel<TG_DTYPE_F32>, dim3(batch), tg::kMergeThreads, smem, st, 1, a));
   } else {
     TG_TRY(tg::launch_after(state_id ? tg::scan_kernel<TG_DTYPE_BF16, true> : tg::scan_kernel<TG_DTYPE_BF16, false>, grid, tg::kThreads, 0, st, 1, a));
-    TG_TRY(tg::launch_after(tg::merge_kernel<TG_DTYPE_BF16>, dim3(batch), tg::kThreads, smem, st, 1, a));
+    TG_TRY(tg::launch_after(tg::merge_kernel<TG_DTYPE_BF16>, dim3(batch), tg::kMergeThreads, smem, st, 1, a));
   }
   return TG_OK;
 }
