@@ -457,7 +457,8 @@ int32_t tg_cache_extend(tg_cache* c, int32_t n, const int32_t* seqs, const int32
  * empty), sharing its pages; pages that dst[i] alone held are freed.  All rows at
  * once: src may repeat, and src and dst may overlap, as when a beam search's
  * parents replace the beams.  dst's slots are distinct.  Tokens reserved but not
- * committed are not taken along. */
+ * committed are not taken along; a row of the pair that stores tokens next reserves
+ * them again (tg_cache_extend), since its last page may now be shared. */
 int32_t tg_cache_fork(tg_cache* c, int32_t n, const int32_t* src, const int32_t* dst, void* stream);
 
 /* Sets row i's length back to lens[i] (NULL: to 0) and frees its pages past it,

@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(kCopyThreads) truncate_kernel(CacheView c, int
     return;
   }
   __syncwarp();
-  if (lane == 0) c.lens[s] = len;
+  if (lane == 0) atomicMin(&c.lens[s], len);  // a slot given twice: the shorter, as its pages
   release_from(c, s, (len + c.page_size - 1) >> c.page_log2, lane);
 }
 
@@ -380,7 +380,11 @@ __global__ void __launch_bounds__(kCopyThreads) accept_kernel(CacheView c, int n
   const int s = seqs[i];
   int count = n_nodes ? n_nodes[i] : nodes;
   uint32_t bad = 0;
-  if (s < 0 || s >= c.max_seqs) {
+  // a slot given twice is served once: of two warps on one row, one would follow page
+  // ids that the other gives back.  move_kernel ends the claim.
+  int claimed = 1;
+  if (lane == 0 && s >= 0 && s < c.max_seqs) claimed = atomicExch(&c.claim[s], 1);
+  if (__shfl_sync(~0u, claimed, 0) != 0) {
     bad |= kBadSlot;
     count = 0;
   } else if (count < 0 || count > nodes) {
@@ -452,9 +456,13 @@ __global__ void __launch_bounds__(kCopyThreads) accept_kernel(CacheView c, int n
 // the path's tokens in ascending order, up to 8 loads ahead of the stores.  The path
 // ascends, so a source is never a place stored to by an earlier move of the same
 // thread, and no other thread touches the column.
-__global__ void __launch_bounds__(kCopyThreads) move_kernel(CacheView c) {
+__global__ void __launch_bounds__(kCopyThreads) move_kernel(CacheView c, const int32_t* seqs) {
   after_previous_work();
   const int i = blockIdx.y, n = c.n_moves[i];
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    const int s = seqs[i];
+    if (s >= 0 && s < c.max_seqs) c.claim[s] = 0;
+  }
   if (n == 0) return;
   const int cols = c.head_dim >> 3;
   const int u = blockIdx.x * kCopyThreads + threadIdx.x;
@@ -711,7 +719,7 @@ int32_t tg_cache_accept(tg_cache* c, int32_t n, const int32_t* seqs, int32_t nod
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   TG_TRY(tg::launch_after(tg::accept_kernel, dim3(tg::blocks_of_warps(n)), tg::kCopyThreads, 0, st, 1, c->view, n, seqs, nodes, n_nodes, parents, tokens, ids, out_ids, out_n));
   const int columns = c->view.layers * 2 * c->view.kv_heads * (c->view.head_dim / 8);
-  TG_TRY(tg::launch_after(tg::move_kernel, dim3((columns + tg::kCopyThreads - 1) / tg::kCopyThreads, n), tg::kCopyThreads, 0, st, 1, c->view));
+  TG_TRY(tg::launch_after(tg::move_kernel, dim3((columns + tg::kCopyThreads - 1) / tg::kCopyThreads, n), tg::kCopyThreads, 0, st, 1, c->view, seqs));
   return TG_OK;
 }
 
