@@ -87,7 +87,8 @@ class BeamSearch:
                     not mask_table.is_contiguous() or mask_table.get_device() != self.device:
                 raise ValueError(f"mask_table must be a contiguous 32-bit tensor [states, {words}] on device {self.device}")
             num_states = mask_table.shape[0]
-        parents, tokens, done = (torch.empty_like(scores, dtype=torch.int32) for _ in range(3))
+        ints = torch.empty_like(scores, dtype=torch.int32) if finished is None else torch.empty_like(finished)
+        parents, tokens, done = ints, torch.empty_like(ints), torch.empty_like(ints)
         best = torch.empty_like(scores)
         new_history = new_len = None
         stride = 0

@@ -200,13 +200,13 @@ class PagedCache:
             _dense(masks, "masks", (n, nodes), device, torch.int64)
         _rows(n_nodes, "n_nodes", n, device)
         if out is None:
-            out = torch.empty(shape, dtype=self.dtype, device=self._where)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         else:
             _dense(out, "out", shape, device, self.dtype)
         if lse is not None:
             _dense(lse, "lse", shape[:3], device, torch.float32)
         elif want_lse:
-            lse = torch.empty(shape[:3], dtype=torch.float32, device=self._where)
+            lse = q.new_empty(shape[:3], dtype=torch.float32)
         check(self._L.tg_tree_attention(self._h, layer, n, seqs.data_ptr(), nodes, address(n_nodes), address(masks), heads,
                                         q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2],
                                         self._scale if scale is None else scale, out.data_ptr(), address(lse),
@@ -223,11 +223,11 @@ class PagedCache:
             _dense(t, name, shape, device, torch.int32)
         _rows(n_nodes, "n_nodes", n, device)
         if out_ids is None:
-            out_ids = torch.empty(shape, dtype=torch.int32, device=self._where)
+            out_ids = torch.empty_like(ids)
         else:
             _dense(out_ids, "out_ids", shape, device, torch.int32)
         if out_n is None:
-            out_n = torch.empty(n, dtype=torch.int32, device=self._where)
+            out_n = torch.empty_like(seqs)
         else:
             _rows(out_n, "out_n", n, device)
         check(self._L.tg_cache_accept(self._h, n, seqs.data_ptr(), shape[1], address(n_nodes), parents.data_ptr(), tokens.data_ptr(),

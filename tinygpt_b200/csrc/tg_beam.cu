@@ -469,7 +469,8 @@ __device__ void row_exact(const BeamArgs& a, int row, int w, float* lse_out, uin
 template <int DT>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(BeamArgs a) {
   extern __shared__ uint64_t keys[];  // [beams, parts, beams], then PartHead [beams, parts]
-  __shared__ uint64_t warp_keys[kMergeThreads / 32], best[TG_MAX_BEAMS], keep[kKeep], bound;
+  __shared__ uint64_t warp_keys[kMergeThreads / 32], best[TG_MAX_BEAMS], keep[kKeep];
+  __shared__ unsigned long long bound;
   __shared__ int n_keys;
   __shared__ float lse[TG_MAX_BEAMS], row_sum[TG_MAX_BEAMS], beam[TG_MAX_BEAMS];
   __shared__ int live[TG_MAX_BEAMS];    // 1: the row adds candidates, 2: it goes on as it is, 0: neither
@@ -536,18 +537,26 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(BeamArgs a) {
         if (tid == 0) exact[w] = 2;
         __syncthreads();
       }
-    // The beams-th best of the lists' first keys is a bound: lists fall but for rounding,
-    // so at most about beams * beams keys reach it.  Each counts those before it.
+    // Bounds of the beams-th best key: the beams-th best of the lists' first keys, and the
+    // beams/2-th best of the lists' pairs of first keys, by the lesser.  Lists fall but for
+    // rounding, so at most about beams * beams keys reach them.  Each of these counts those
+    // before it.
     if (tid == 0) n_keys = 0, bound = 0;
     if (tid < W) best[tid] = 0;
     __syncthreads();
-    for (int i = tid; i < W * P; i += kMergeThreads) {
-      const uint64_t k = keys[i * W];
+    const int lists = W * P;
+    const auto front = [&](int list, bool pair) {
+      const uint64_t k = keys[list * W];
+      return pair ? min(k, keys[list * W + 1]) : k;
+    };
+    for (int i = tid; i < (W > 1 ? 2 * lists : lists); i += kMergeThreads) {
+      const bool pair = i >= lists;
+      const uint64_t k = front(pair ? i - lists : i, pair);
       int r = 0;
       if (k != 0) {
 #pragma unroll 4
-        for (int j = 0; j < W * P; j++) r += keys[j * W] > k;
-        if (r == W - 1) bound = k;
+        for (int j = 0; j < lists; j++) r += front(j, pair) > k;
+        if (r + 1 == (pair ? (W + 1) / 2 : W)) atomicMax(&bound, static_cast<unsigned long long>(k));
       }
     }
     __syncthreads();
@@ -632,19 +641,34 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(BeamArgs a) {
   }
   if (!a.history) return;
   __syncthreads();
-  // a warp per 512 entries of a history, 16 loads on their way per lane
-  const int pieces = (a.history_stride + 511) / 512;
-  for (int u = tid >> 5; u < W * pieces; u += kMergeThreads / 32) {
-    const int w = u / pieces, j0 = (u - w * pieces) * 512 + lane, len = from_len[w];
-    const int32_t* from = a.history + static_cast<int64_t>(from_row[w]) * a.history_stride;
-    int32_t* to = a.out_history + static_cast<int64_t>(row0 + w) * a.history_stride;
-    int32_t x[16];
+  // 8 loads of 4 entries on their way per lane where rows are aligned, 16 of one where not
+  const auto copy = [&](auto type) {
+    using T = decltype(type);
+    constexpr int kPer = sizeof(T) / 4, kLoads = kPer > 1 ? 8 : 16, kStep = 32 * kPer * kLoads;
+    const int pieces = (a.history_stride + kStep - 1) / kStep;
+    for (int u = tid >> 5; u < W * pieces; u += kMergeThreads / 32) {
+      const int w = u / pieces, j0 = (u - w * pieces) * kStep + lane * kPer, len = from_len[w];
+      const int32_t* from = a.history + static_cast<int64_t>(from_row[w]) * a.history_stride;
+      int32_t* to = a.out_history + static_cast<int64_t>(row0 + w) * a.history_stride;
+      __align__(16) int32_t x[kPer * kLoads];
 #pragma unroll
-    for (int e = 0; e < 16; e++) x[e] = j0 + 32 * e < len ? from[j0 + 32 * e] : j0 + 32 * e == len ? grow[w] : -1;
+      for (int e = 0; e < kLoads; e++) {
+        const int j = j0 + 32 * kPer * e;
+        if (j < len) *reinterpret_cast<T*>(x + e * kPer) = *reinterpret_cast<const T*>(from + j);
+      }
 #pragma unroll
-    for (int e = 0; e < 16; e++)
-      if (j0 + 32 * e < a.history_stride) to[j0 + 32 * e] = x[e];
-  }
+      for (int e = 0; e < kLoads; e++) {
+        const int j = j0 + 32 * kPer * e;
+        if (j >= a.history_stride) break;
+#pragma unroll
+        for (int i = 0; i < kPer; i++)
+          if (j + i >= len) x[e * kPer + i] = j + i == len ? grow[w] : -1;
+        *reinterpret_cast<T*>(to + j) = *reinterpret_cast<const T*>(x + e * kPer);
+      }
+    }
+  };
+  if (a.history_stride % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.history) | reinterpret_cast<uintptr_t>(a.out_history)) & 15) == 0) copy(int4{});
+  else copy(int32_t{});
 }
 
 // Parts of a row: the number with the least waves x (groups of a part + 3.5), since what
