@@ -60,6 +60,7 @@ struct TreeArgs {
   int32_t layer, n, nodes, q_heads, group, blocks, min_tiles, vec;  // vec: all rows are 16-byte aligned
   uint32_t group_inverse;  // ceil(2^32 / group)
   int32_t q_rows, tree_rows, slots;  // shared memory: rows of a row block, of the nodes' tile, ring slots
+  uint32_t ring_block, ring_group;   // bytes from one 64-column block of a slot to the next, from 8 tokens to the next 8
   const int32_t* seqs;
   const int32_t* n_nodes;
   const uint64_t* masks;
@@ -107,10 +108,10 @@ __device__ __forceinline__ bool bar_poll_lane0(uint32_t bar, uint32_t parity, ui
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ void tma_load(uint32_t to, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int w) {
+__device__ __forceinline__ void tma_load(uint32_t to, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(to), "l"(map), "r"(bar), "r"(x), "r"(y),
-      "r"(z), "r"(w)
+      "cp.async.bulk.tensor.5d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %4, %5, %6}], [%2];" ::"r"(to), "l"(map), "r"(bar), "r"(x), "r"(0),
+      "r"(y), "r"(z)
       : "memory");
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -655,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
         const int token = (t - 1) * kTile, here = min(kTile, g.len - token), n = (here + box - 1) / box;
         int page = 0;
         if (lane < n) page = c.tables[static_cast<size_t>(g.slot) * c.width + ((token + lane * box) >> c.page_log2)];
-        const int z = a.layer * c.num_pages + page, y = (token + lane * box) & (c.page_size - 1);
+        const int z = (a.layer * c.num_pages + page) * c.kv_heads + g.head, y = ((token + lane * box) & (c.page_size - 1)) >> 3;
         // past the first tile the run's first Q goes before: behind a full ring of
         // copies its loads would wait for all of them
         if (tiles >= 0 && ++tiles == 2) ok = wait(&ctl, &ctl.q_full[0], 0);
@@ -667,9 +668,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
           if (lane == 0) bar_expect(bar, n * box * L::kBlocks * 128);
           __syncwarp();
           if (lane < n) {
-#pragma unroll
-            for (int x = 0; x < L::kBlocks; x++)
-              tma_load(to + x * (kTile * 128) + lane * box * 128, kv ? &v_map : &k_map, bar, x * 64, y, g.head, z);
+            for (uint32_t x = 0; x < L::kBlocks; x += a.ring_block == 1024 ? 2 : 1)
+              tma_load(to + x * a.ring_block + lane * (box >> 3) * a.ring_group, kv ? &v_map : &k_map, bar, x * 64, y, z);
           }
           __syncwarp();
           if (++slot == static_cast<uint32_t>(a.slots)) slot = 0, turn++;
@@ -690,7 +690,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
     if (elect()) {
       constexpr uint32_t s_inst = instruction(kBf16, kTile, 0), o_inst = instruction(kBf16, kDim, 1);
       const uint32_t tree_inst = s_inst - (static_cast<uint32_t>((kTile - a.tree_rows) >> 3) << 17);
-      const uint64_t k_desc = operand(base + ring_at, 16, 1024), v_desc = operand(base + ring_at, kTile * 128, 1024);
+      const uint64_t k_desc = operand(base + ring_at, 16, a.ring_group), v_desc = operand(base + ring_at, a.ring_block, a.ring_group);
+      const uint32_t ring_step = a.ring_block / 16, ring_keys = a.ring_group / 8;
       uint64_t q_desc = operand(base + q_at, 16, 1024), tk_desc = operand(base + tk_at, 16, 1024), tv_desc = operand(base + tv_at, tree_block, 1024);
       const uint32_t slots = a.slots, q_step = q_block / 16, tree_step = tree_block / 16;
       uint32_t k_slot = 0, k_turn = 0, v_slot = 1, v_turn = 0;  // the next keys and values in the ring
@@ -718,6 +719,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
             // look for the next keys before P is there, not between its product and theirs
             if (j + 2 < n && !(kWide && s)) k_ready = bar_poll(smem_addr(&ctl.full[k_slot]), k_turn & 1);
             const uint64_t vd = t > 0 ? v_desc + v_slot * (L::kSlot / 16) : tv_desc;
+            const uint32_t step = t > 0 ? ring_keys : 2048 / 16;  // 16 keys
             const uint32_t d = 2 * kTile + s * kDim, p = s * kTile, turn = p_turn >> s & 1;
             const int steps = max(1, (keys + 15) / 16);
             ok = wait_alone(&ctl, &ctl.p_half[s], turn);
@@ -725,7 +727,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
             tmem_after();
 #pragma unroll
             for (int i = 0; i < 4; i++)
-              if (i < steps) mma_ts(d, p + i * 8, vd + i * (2048 / 16), o_inst, j >= 2 || i > 0);
+              if (i < steps) mma_ts(d, p + i * 8, vd + i * step, o_inst, j >= 2 || i > 0);
             tmem_commit(smem_addr(&ctl.half_done[s]));
             ok = wait_alone(&ctl, &ctl.p_full[s], turn);
             if (!ok) break;
@@ -734,7 +736,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
               tmem_after();
 #pragma unroll
               for (int i = 4; i < 8; i++)
-                if (i < steps) mma_ts(d, p + i * 8, vd + i * (2048 / 16), o_inst, 1);
+                if (i < steps) mma_ts(d, p + i * 8, vd + i * step, o_inst, 1);
             }
             if (t > 0 && last_use) {
               tmem_commit(smem_addr(&ctl.empty[v_slot]));
@@ -755,7 +757,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
               tmem_after();
             }
             const uint64_t qd = q_desc + (kWide ? s * (q_tile / 16) : 0), kd = t > 0 ? k_desc + k_slot * (L::kSlot / 16) : tk_desc;
-            const uint32_t d = s * kTile, step = t > 0 ? kTile * 128 / 16 : tree_step, inst = t > 0 ? s_inst : tree_inst;
+            const uint32_t d = s * kTile, step = t > 0 ? ring_step : tree_step, inst = t > 0 ? s_inst : tree_inst;
 #pragma unroll
             for (int i = 0; i < kDim / 16; i++) mma_ss(d, qd + (i >> 2) * q_step + (i & 3) * 2, kd + (i >> 2) * step + (i & 3) * 2, inst, i > 0);
             tmem_commit(smem_addr(&ctl.s_full[s]));
@@ -857,7 +859,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
           const int end = (keys + 15) & ~15;
           for (int i = row; i < (end - keys) * kChunks; i += kTile) {
             const int j = keys + i / kChunks, ch = i % kChunks;
-            *reinterpret_cast<uint4*>(raw + ring_at + slot * L::kSlot + (ch >> 3) * (kTile * 128) + j * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(raw + ring_at + slot * L::kSlot + (ch >> 3) * a.ring_block + (j >> 3) * a.ring_group + (j & 7) * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_async();
           __syncwarp();
@@ -1104,6 +1106,9 @@ cudaError_t launch(tg_cache* c, TreeArgs a, cudaStream_t st) {
   a.tree_rows = (a.nodes + 15) & ~15;
   const int fixed = control_bytes<L::kBuffers>() + L::kBuffers * ((kWide ? 2 : 1) * a.q_rows + 2 * a.tree_rows) * kDim * 2;
   a.slots = (kMaxSmem - fixed) / L::kSlot;
+  const bool joined = c->view.head_dim == 128;  // as tree_setup's boxes
+  a.ring_block = joined ? 1024 : kTile * 128;
+  a.ring_group = joined ? 2048 : 1024;
   if (a.slots > kMaxSlots) a.slots = kMaxSlots;
   // the last row block's 128 rows, read from its start, end inside the block's memory:
   // at least 4 slots of 128 rows follow it
@@ -1134,12 +1139,16 @@ int32_t tree_setup(tg_cache* c) noexcept {
   TG_TRY(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found));
   if (found != cudaDriverEntryPointSuccess || !fn) return set_error(TG_ERR_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
   const CacheView& v = c->view;
-  const cuuint64_t d = v.head_dim, ps = v.page_size, heads = v.kv_heads;
-  const cuuint64_t dims[4] = {d, ps, heads, static_cast<cuuint64_t>(v.num_pages) * v.layers};
-  const cuuint64_t strides[3] = {d * 2, d * 2 * ps, d * 2 * ps * heads};
-  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(ps < kTile ? ps : kTile), 1, 1}, ones[4] = {1, 1, 1, 1};
+  // A box is what a tile needs of a page: 8-token groups of 64-column blocks, as they lie in
+  // a slot.  A head dimension of 128 comes as one box of both blocks (dimension 2), since
+  // the copy engine takes about 75 cycles a box whatever its size; other dimensions past
+  // 64 take a box per block, for the columns past the end to read as zeros.
+  const cuuint64_t d = v.head_dim, ps = v.page_size, joined = d == 128 ? 2 : 1;
+  const cuuint64_t dims[5] = {joined == 2 ? 64 : d, 8, joined, ps / 8, static_cast<cuuint64_t>(v.num_pages) * v.layers * v.kv_heads};
+  const cuuint64_t strides[4] = {d * 2, 128, d * 16, d * 2 * ps};
+  const cuuint32_t box[5] = {64, 8, static_cast<cuuint32_t>(joined), static_cast<cuuint32_t>((ps < kTile ? ps : kTile) / 8), 1}, ones[5] = {1, 1, 1, 1, 1};
   for (int i = 0; i < 2; i++) {
-    const CUresult r = reinterpret_cast<EncodeFn>(fn)(i ? &c->v_map : &c->k_map, c->dtype == TG_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+    const CUresult r = reinterpret_cast<EncodeFn>(fn)(i ? &c->v_map : &c->k_map, c->dtype == TG_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
                                                       i ? v.v : v.k, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return set_error(TG_ERR_CUDA, "cuTensorMapEncodeTiled failed");
