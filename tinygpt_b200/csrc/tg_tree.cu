@@ -174,6 +174,17 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+// The sign bits of the halves of w that are not finite: an exponent of ones carries into it.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t odd_halves(uint32_t w) {
+  return kBf16 ? ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u : ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+}
+// w with zeros in their place.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
+  const uint32_t odd = odd_halves<kBf16>(w);
+  return w & ~((odd >> 15) * 0xffffu);
+}
 template <bool kBf16>
 __device__ __forceinline__ bool not_finite(uint16_t x) {
   return kBf16 ? (x & 0x7f80) == 0x7f80 : (x & 0x7c00) == 0x7c00;
@@ -391,18 +402,13 @@ __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
 
-// 8 elements of a row from column `col` on, zeros past the head's dimension.
+// 8 elements of a row from column `col` on.
 __device__ __noinline__ uint4 load8_by_element(const uint16_t* row, int col) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) w[i] = row[col + 2 * i] | static_cast<uint32_t>(row[col + 2 * i + 1]) << 16;
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ uint4 load8(const uint16_t* row, int col, int dim, bool vec) {
-  if (col >= dim) return make_uint4(0, 0, 0, 0);
-  return vec ? *reinterpret_cast<const uint4*>(row + col) : load8_by_element(row, col);
-}
-
 // A row's fp32 columns in TMEM by f, by whole warps.
 __device__ __forceinline__ void scale_columns(uint32_t at, int columns, float f) {
 #pragma unroll 1
@@ -565,70 +571,64 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
     const int rows0 = w.block * kRows, rows = min(kRows, w.nodes * a.group - rows0);  // rows that are there
     const bool tree = w.t0 == 0;
     const int me = tid - 320, ch = me % kChunks, first_row = me / kChunks;  // a thread keeps its column of chunks
-    constexpr int kRowStep = 64 / kChunks, kAhead = 4;                      // nodes' rows of a thread on their way at a time
-    if (a.vec) {
-      for (int r = first_row; r < rows; r += kRowStep) {
-        const int node = divide(rows0 + r, a.group_inverse), h = w.head * a.group + rows0 + r - node * a.group, rr = r & (kTile - 1);
-        copy16(base + q_at + to + (r / kTile) * q_tile + (ch >> 3) * q_block + rr * 128 + ((ch ^ rr) & 7) * 16,
-               a.q.p + w.b * a.q.row + node * a.q.node + h * a.q.head + (ch * 8 < c.head_dim ? ch * 8 : 0), ch * 8 < c.head_dim);
-      }
-    } else {
-      for (int r = first_row; r < rows; r += kRowStep) {
-        const int node = divide(rows0 + r, a.group_inverse), h = w.head * a.group + rows0 + r - node * a.group, rr = r & (kTile - 1);
-        *reinterpret_cast<uint4*>(raw + q_at + to + (r / kTile) * q_tile + (ch >> 3) * q_block + rr * 128 + ((ch ^ rr) & 7) * 16) =
-            load8(a.q.p + w.b * a.q.row + node * a.q.node + h * a.q.head, ch * 8, c.head_dim, false);
-      }
+    constexpr int kRowStep = 64 / kChunks;
+    // 8 columns of a row to shared memory; zeros past the head's dimension and where the row is not there
+    const auto bring = [&](uint32_t at, const uint16_t* row, bool there) {
+      there = there && ch * 8 < c.head_dim;
+      if (a.vec) copy16(base + at, row + (there ? ch * 8 : 0), there);
+      else *reinterpret_cast<uint4*>(raw + at) = there ? load8_by_element(row, ch * 8) : make_uint4(0, 0, 0, 0);
+    };
+    const uint16_t* q_from = a.q.p + w.b * a.q.row + static_cast<int64_t>(w.head) * a.group * a.q.head;
+#pragma unroll 4
+    for (int r = first_row; r < rows; r += kRowStep) {
+      const int node = divide(rows0 + r, a.group_inverse), h = rows0 + r - node * a.group, rr = r & (kTile - 1);
+      bring(q_at + to + (r / kTile) * q_tile + (ch >> 3) * q_block + rr * 128 + ((ch ^ rr) & 7) * 16, q_from + node * a.q.node + h * a.q.head, true);
     }
-    uint32_t odd_lo = 0, odd_hi = 0;
+    const int room = w.nodes > 0 ? (c.counts[w.slot] << c.page_log2) - w.len : 0, keep = tree && w.block == 0 ? min(w.nodes, room) : 0;
+    int page = -1;  // of this lane's page among those that the nodes go to: 64 nodes reach 9 at most
     if (tree) {
+      const uint16_t* k_from = a.k.p + w.b * a.k.row + w.head * a.k.head;
+      const uint16_t* v_from = a.v.p + w.b * a.v.row + w.head * a.v.head;
+#pragma unroll 4
+      for (int j = first_row; j < a.tree_rows; j += kRowStep) {
+        const uint32_t at = to + (ch >> 3) * tree_block + j * 128 + ((ch ^ j) & 7) * 16;
+        const int node = j < w.nodes ? j : 0;
+        bring(tk_at + at, k_from + node * a.k.node, j < w.nodes);
+        bring(tv_at + at, v_from + node * a.v.node, j < w.nodes);
+      }
       if (me < w.nodes) {
         const uint64_t all = w.nodes < 64 ? (1ull << w.nodes) - 1 : ~0ull;
         sets[buffer].of[me] = (a.masks ? a.masks[static_cast<int64_t>(w.b) * a.nodes + me] : ~0ull >> (63 - me)) & all;
       }
-      const int room = w.nodes > 0 ? (c.counts[w.slot] << c.page_log2) - w.len : 0, keep = w.block == 0 ? min(w.nodes, room) : 0;
+      const int first_page = w.len >> c.page_log2;
+      if (keep > 0 && first_page + lane <= (w.len + keep - 1) >> c.page_log2) page = c.tables[static_cast<size_t>(w.slot) * c.width + first_page + lane];
       if (me == 0 && w.block == 0 && w.head == 0 && w.nodes > room) atomicOr(c.status, kNotReserved);
-#pragma unroll 1
-      for (int j0 = first_row; j0 < a.tree_rows; j0 += kAhead * kRowStep) {
-        uint4 x[kAhead], y[kAhead];
-        int page[kAhead];
-#pragma unroll
-        for (int u = 0; u < kAhead; u++) {
-          const int j = j0 + u * kRowStep;
-          x[u] = y[u] = make_uint4(0, 0, 0, 0);
-          if (j < w.nodes) {
-            x[u] = load8(a.k.p + w.b * a.k.row + j * a.k.node + w.head * a.k.head, ch * 8, c.head_dim, a.vec);
-            y[u] = load8(a.v.p + w.b * a.v.row + j * a.v.node + w.head * a.v.head, ch * 8, c.head_dim, a.vec);
-          }
-          page[u] = j < keep ? c.tables[static_cast<size_t>(w.slot) * c.width + ((w.len + j) >> c.page_log2)] : -1;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    uint32_t odd_lo = 0, odd_hi = 0;
+    if (tree) {
+      const int64_t pages = static_cast<int64_t>(a.layer) * c.num_pages;
+#pragma unroll 2
+      for (int j = first_row; j < a.tree_rows; j += kRowStep) {  // as often in every lane
+        const uint32_t at = to + (ch >> 3) * tree_block + j * 128 + ((ch ^ j) & 7) * 16;
+        const int there = __shfl_sync(~0u, page, ((w.len & (c.page_size - 1)) + j) >> c.page_log2 & 31);
+        uint4 v = *reinterpret_cast<const uint4*>(raw + tv_at + at);
+        if (j < keep && ch * 8 < c.head_dim) {
+          const int64_t in_pool = (((pages + there) * c.kv_heads + w.head) << c.page_log2) + ((w.len + j) & (c.page_size - 1));
+          *reinterpret_cast<uint4*>(c.k + in_pool * c.head_dim * 2 + ch * 16) = *reinterpret_cast<const uint4*>(raw + tk_at + at);
+          *reinterpret_cast<uint4*>(c.v + in_pool * c.head_dim * 2 + ch * 16) = v;
         }
-#pragma unroll
-        for (int u = 0; u < kAhead; u++) {
-          const int j = j0 + u * kRowStep, at = to + (ch >> 3) * tree_block + j * 128 + ((ch ^ j) & 7) * 16;
-          if (j >= a.tree_rows) continue;
-          if (page[u] >= 0 && ch * 8 < c.head_dim) {
-            const int64_t in_pool = (((static_cast<int64_t>(a.layer) * c.num_pages + page[u]) * c.kv_heads + w.head) << c.page_log2) + ((w.len + j) & (c.page_size - 1));
-            *reinterpret_cast<uint4*>(c.k + in_pool * c.head_dim * 2 + ch * 16) = x[u];
-            *reinterpret_cast<uint4*>(c.v + in_pool * c.head_dim * 2 + ch * 16) = y[u];
-          }
-          // a value that is not finite would reach every row as 0 * inf: it is taken out
-          // here and added to the rows that see it at the end
-          uint32_t ws[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
-          bool odd = false;
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            if (not_finite<kBf16>(ws[e] & 0xffff)) ws[e] &= 0xffff0000u, odd = true;
-            if (not_finite<kBf16>(ws[e] >> 16)) ws[e] &= 0xffffu, odd = true;
-          }
-          if (odd) (j < 32 ? odd_lo : odd_hi) |= 1u << (j & 31);
-          *reinterpret_cast<uint4*>(raw + tk_at + at) = x[u];
-          *reinterpret_cast<uint4*>(raw + tv_at + at) = make_uint4(ws[0], ws[1], ws[2], ws[3]);
+        // a value that is not finite would reach every row as 0 * inf: it is taken out
+        // here and added to the rows that see it at the end
+        if (odd_halves<kBf16>(v.x) | odd_halves<kBf16>(v.y) | odd_halves<kBf16>(v.z) | odd_halves<kBf16>(v.w)) {
+          (j < 32 ? odd_lo : odd_hi) |= 1u << (j & 31);
+          *reinterpret_cast<uint4*>(raw + tv_at + at) = make_uint4(finite_halves<kBf16>(v.x), finite_halves<kBf16>(v.y), finite_halves<kBf16>(v.z), finite_halves<kBf16>(v.w));
         }
       }
     }
     odd_lo = __reduce_or_sync(~0u, odd_lo);
     odd_hi = __reduce_or_sync(~0u, odd_hi);
     if (lane == 0) ctl.odd[segment % 4][warp & 1] = static_cast<uint64_t>(odd_hi) << 32 | odd_lo;
-    asm volatile("cp.async.wait_all;" ::: "memory");
     if (a.scale < 0.0f) {  // scale's sign goes into Q
       for (int r = first_row; r < rows; r += kRowStep) {
         const int rr = r & (kTile - 1);
@@ -695,6 +695,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
       uint64_t q_desc = operand(base + q_at, 16, 1024), tk_desc = operand(base + tk_at, 16, 1024), tv_desc = operand(base + tv_at, tree_block, 1024);
       const uint32_t slots = a.slots, q_step = q_block / 16, tree_step = tree_block / 16;
       uint32_t k_slot = 0, k_turn = 0, v_slot = 1, v_turn = 0;  // the next keys and values in the ring
+      // steps of a segment from which on the last scores come after the nodes' products, and
+      // so Q and the nodes are free with them
+      constexpr int kEarly = kWide ? 4 : 3;
       uint32_t segment = 0, p_turn = 0;  // p_turn: bit s is group s's parity
       bool ok = true;
       for (Turn k; ok; k.next()) {
@@ -745,7 +748,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
             }
             if (j == n - 1) {
               tmem_commit(smem_addr(&ctl.done));
-              tmem_commit(smem_addr(&ctl.q_empty[segment % kBuffers]));
+              if (n < kEarly) tmem_commit(smem_addr(&ctl.q_empty[segment % kBuffers]));
             }
           }
           if (j + 2 < n) {
@@ -761,6 +764,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
 #pragma unroll
             for (int i = 0; i < kDim / 16; i++) mma_ss(d, qd + (i >> 2) * q_step + (i & 3) * 2, kd + (i >> 2) * step + (i & 3) * 2, inst, i > 0);
             tmem_commit(smem_addr(&ctl.s_full[s]));
+            if (j == n - 3 && n >= kEarly) tmem_commit(smem_addr(&ctl.q_empty[segment % kBuffers]));
             if (t > 0 && last_use) {
               tmem_commit(smem_addr(&ctl.empty[k_slot]));
               k_slot += 2;
