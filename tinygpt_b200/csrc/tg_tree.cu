@@ -88,6 +88,30 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Two floats an instruction.
+__device__ __forceinline__ uint64_t two(float lo, float hi) { return static_cast<uint64_t>(__float_as_uint(hi)) << 32 | __float_as_uint(lo); }
+__device__ __forceinline__ float low_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float high_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
 __device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
@@ -845,7 +869,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
       const bool mine = r < rows, any = (r & ~31) < rows;  // this row, this warp's rows are there
       const int node = mine ? divide(rows0 + r, a.group_inverse) : 0, h = w.head * a.group + (mine ? rows0 + r - node * a.group : 0);
       uint64_t sees = 0;
-      float t_ref = -INFINITY, sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      float t_ref = -INFINITY;
+      uint64_t sum[2] = {0, 0};
       bool clear = segment == 0;  // the last segment's O has been read
       const int step = kWide ? 1 : 2;
       for (int t = w.t0 + (kWide ? 0 : g); ok && t < w.t1; t += step) {
@@ -888,14 +913,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
             }
             float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < 64; e++) m[e & 3] = fmaxf(m[e & 3], __uint_as_float(v[e]));
+            for (int e = 0; e < 64; e += 2) m[e >> 1 & 3] = max3(m[e >> 1 & 3], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
             const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * cs;
             const bool move = top > t_ref + kSlack;
             if (__any_sync(~0u, move)) {
               const float f = move ? exp2_fast(t_ref - top) : 1.0f;
               if (move) t_ref = top;
-#pragma unroll
-              for (int e = 0; e < 4; e++) sum[e] *= f;
+              sum[0] = mul2(sum[0], two(f, f)), sum[1] = mul2(sum[1], two(f, f));
               if (half) {  // the products with the first half's weights are to end first; those
                            // of the tiles before had when this one's scores were made
                 ok = wait(&ctl, &ctl.half_done[g], s_turn & 1);
@@ -905,11 +929,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
               if (half || t >= w.t0 + step) scale_columns(o_at, kDim, f);
             }
             const float t_use = t_ref == -INFINITY ? 0.0f : t_ref;
+            const uint64_t scale = two(cs, cs), from = two(-t_use, -t_use);
 #pragma unroll
             for (int e = 0; e < 64; e += 2) {
-              const float p0 = exp2_fast(__fmaf_rn(__uint_as_float(v[e]), cs, -t_use));
-              const float p1 = exp2_fast(__fmaf_rn(__uint_as_float(v[e + 1]), cs, -t_use));
-              sum[e & 3] += p0, sum[(e + 1) & 3] += p1;
+              const uint64_t x = fma2(two(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), scale, from);
+              const float p0 = exp2_fast(low_of(x)), p1 = exp2_fast(high_of(x));
+              sum[e >> 1 & 1] = add2(sum[e >> 1 & 1], two(p0, p1));
               v[e / 2] = pack<kBf16>(p0, p1);
             }
             tmem_store16(s_at + half * 32, v);
@@ -930,7 +955,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
       if (!ok) break;
       loaded += 2 * (w.t1 - max(w.t0, 1));
       sums[segment % kBuffers].t[g][row] = t_ref;
-      sums[segment % kBuffers].sum[g][row] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      sums[segment % kBuffers].sum[g][row] = (low_of(sum[0]) + high_of(sum[0])) + (low_of(sum[1]) + high_of(sum[1]));
       warp_arrive(&ctl.stats);
       segment++;
       warp_arrive(&ctl.seg_empty[k.at]);
