@@ -17,6 +17,11 @@
  *   tg_spec_verify   <- SpeculativeDecode.stepStochastic  native-mac/Sources/TinyGPT/SpeculativeDecode.swift:121-210
  *                    <- SpeculativeDecode.step (greedy)   native-mac/Sources/TinyGPT/SpeculativeDecode.swift:41-98
  *
+ * Beyond the reference (it keeps one sequence's contiguous cache and samples only):
+ *   tg_cache_*, tg_tree_attention, tg_tree_masks   a paged key/value cache and the
+ *                       attention of drafted trees over it
+ *   tg_beam_*           beam search's selection over beams and vocabulary
+ *
  * Memory: all array arguments of tg_sample / tg_spec_verify are DEVICE pointers
  * on the sampler's device, owned by the caller.  The *_host variants take host
  * pointers and stage through buffers the handle owns.  Threading: one handle
@@ -438,7 +443,9 @@ typedef struct tg_cache_state {
 } tg_cache_state;
 
 /* k_pool, v_pool: device memory, 16-byte aligned, owned by the caller and kept
- * while the handle lives.  Every slot starts empty. */
+ * while the handle lives.  Every slot starts empty.  The handle's own memory: about
+ * 16 bytes a page, 12 a table entry, 1.1 KB a slot, and 39 MB in which
+ * tg_tree_attention joins what its blocks leave. */
 int32_t tg_cache_create(int32_t device, const tg_cache_config* config, void* k_pool, void* v_pool,
                         tg_cache** out);
 int32_t tg_cache_destroy(tg_cache* c);

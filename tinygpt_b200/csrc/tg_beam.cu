@@ -16,8 +16,15 @@
 // for that at every list's cut and then, as for rows with NaN or +inf or with more ties
 // than a list holds, finds the row's list from the logits themselves (row_exact).
 //
-// Bound: HBM bytes (each logit once) for many rows, launch and reduction latency for
-// few.
+// Bound and figures (B200): HBM bytes for many rows, each logit once; 1024 rows of 128,256
+// bf16 logits take 61 us (263 MB, 4.4 TB/s): the stream itself runs at 6.4 TB/s, the lists
+// at its blocks' ends and merge_kernel take a third of the time.  Latency for few: 4 rows
+// of 50,257 fp32 logits 10.5 us, half of it the merge.
+//
+// One launch instead of two, the last block of a batch row merging it, was slower on the
+// device (66 and 12 us: every block waits for its fence and its arrival, and the merge
+// has fewer threads).  Persistent blocks with a ring of bulk copies were slower too (86 us:
+// a block per SM hides the ends of its rows less well than 4).
 #include "tg_host.h"
 
 #include <cuda_bf16.h>
@@ -673,8 +680,9 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(BeamArgs a) {
 
 // Parts of a row: the number with the least waves x (groups of a part + 3.5), since what
 // follows a part's last group takes as long as 3.5 groups (9,000 of 2,700 cycles with 4
-// blocks on an SM).  1024 rows of 16 groups: 64 us in one part, 87 in four; 4 rows of 7
-// groups: 10.3 us in 7 parts.  Never more groups than a block keeps.
+// blocks on an SM).  1024 rows of 16 groups: 62 us in one part, 66 in two, 73 in four; 128
+// rows: 22.7 us in 4 parts, 24.6 in 3, 26.1 in 2; 4 rows of 13 groups: 10.5 us in 13 parts,
+// 12.1 in 2, 14.0 in one.  Never more groups than a block keeps.
 int parts_of(int vocab, int per, int rows) {
   const int step = kThreads * kVecs * per;  // elements of one group of every thread
   const int most = (vocab + step - 1) / step, least = (most + kMaxGroups - 1) / kMaxGroups;

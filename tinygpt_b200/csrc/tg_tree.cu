@@ -8,21 +8,39 @@
 // the rows of one matrix: row = node * group + head in group.  A work item is (sequence,
 // key head, block of rows); its tiles are the nodes themselves (up to 64 keys, tile 0)
 // and 128 cached tokens each.  Keys and values are read once per item; a single
-// token with 4 heads per key head uses 4 of a tile's 128 rows, which costs nothing while
-// the bytes bound the time (128 rows need 1050 tensor cycles a tile, its 64 KB 2800).
+// token with 4 heads per key head uses 4 of a tile's 128 rows, which costs no time while
+// the bytes bound it (128 rows need 1050 tensor cycles a tile, its 64 KB 2800).
 //
 // Split.  The tiles of all items, in order, are cut into equal runs, one per block, one
 // block per SM: any mix of lengths is balanced to a tile.  An item that is cut
 // leaves (t, sum, unnormalised o) of its runs in a workspace, and join_kernel puts
 // them together in the order of the runs: the result does not depend on timing.
 //
-// A block.  Warp 8 brings pages with tiled TMA into a ring of 128-byte-swizzled slots;
-// warp 9 issues tcgen05.mma: S = Q K^T into TMEM, and O += P V with P read from TMEM;
-// two groups of four warps turn S into P, a thread per row, so no row needs a
-// shuffle.  The two groups work on two S buffers: on two blocks of 128 rows of the same
-// tile when the item has more than 128 rows (kWide), else on alternate tiles of
-// the same rows, joined at the item's end.  While one group exponentiates, the tensor
-// cores work for the other.
+// A block.  16 warps with roles that meet at mbarriers only:
+//   8       pages by tiled TMA into a ring of 128-byte-swizzled slots, 128 keys or values each
+//   9       one lane issues tcgen05.mma: S = Q K^T into TMEM, O += P V with P read from TMEM
+//   0-7     two groups that turn S into P, a thread per row, so no row needs a shuffle; they
+//           work on two S buffers: on two blocks of 128 rows of the same tile when the item
+//           has more than 128 rows (kWide), else on alternate tiles of the same rows, joined
+//           at the item's end.  While one group exponentiates, the tensor cores work for
+//           the other
+//   10, 11  walk over the run's segments (the part of an item that is in it), Q and the
+//           nodes of a segment ahead, the nodes also into the cache
+//   12-15   join a segment's two groups and write its rows, while the others go on
+//
+// Bound and figures (B200; 6.5 TB/s and 1.65 PFLOP/s by the card's own copy and GEMM):
+//   HBM for decoding: 64 sequences, 1 node, 114 us for 622 MB, 5.4 TB/s.  Pages below 64
+//   tokens cost more: the copy engine takes about 75 cycles a box and a box is a page's
+//   part of a tile (16,000 tokens, 32 sequences: 93 us, in pages of 16 118, of 8 153)
+//   the chain S -> P -> O -> S of a group for many rows: 4300 cycles a tile, of which the
+//   weights take 2400 (the exponentials' unit 1024 of them), the products 770, and the waits
+//   between warps the rest: 1 sequence, 64 nodes x 4 heads, 102 us, 0.67 PFLOP/s
+//   the card's power limit for the largest call (64 sequences, 16 nodes): 264 to 290 us, by
+//   the clock that the card holds, 1.66 to 1.75 GHz of 1.96
+//   latency for small calls: 14 us, of which join_kernel's launch takes 3
+// Tried and slower: exponentials of 32 scores beside the next 32's maxima (one vote more a
+// half tile: +5%), a tile's loop unrolled with more registers (the code left the
+// instruction caches: twice as slow), runs handed out in small pieces by a counter.
 //
 // Rounding: S, the sums and O are fp32; P is rounded to the cache's type for the tensor
 // cores (the products with V take 16-bit operands), relative 2^-8 (bf16) or 2^-11
