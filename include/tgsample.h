@@ -413,8 +413,8 @@ int32_t tg_grammar_table(tg_grammar* g, const uint32_t** words, int32_t* rows);
  *   bit 1: not enough free pages (extend: rows are served in order until one
  *          does not fit; that row and the later ones that need pages get none)
  *   bit 2: a length past max_pages_per_seq pages, or a negative count or length
- *   bit 3: keys and values past the pages reserved by tg_cache_extend (not stored),
- *          or an advance past them
+ *   bit 3: keys and values past the pages reserved by tg_cache_extend, or into a
+ *          page that a fork still shares (not stored), or an advance past them
  *   bit 4: a bounded wait of tg_tree_attention gave up (its output is unreliable)
  *   bit 5: a tree whose node count is outside [0, nodes]
  * Threading and streams: as tg_sampler, one handle serves one stream at a time. */

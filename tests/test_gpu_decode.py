@@ -120,3 +120,51 @@ def test_truncate_of_a_repeated_slot_takes_the_shorter():
     c.commit(i32([0]), i32([60]))
     c.truncate(i32([0, 0]), i32([50, 9]))
     assert c.lens[0] == 9 and c.counts[0] == 2 and c.refs.sum() == 2
+
+
+def forked(nodes):
+    """Slot 0 with 11 tokens of value 1, forked to slot 1: both end in one page."""
+    import torch
+    from tinygpt_b200 import PagedCache
+    c = PagedCache(1, 1, 16, 8, 16, 2, 8)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    c.extend(i32([0]), i32([11 + nodes]))
+    ones = torch.ones((1, 11, 1, 16), dtype=torch.bfloat16, device="cuda")
+    c.append(0, i32([0]), ones, ones)
+    c.commit(i32([0]), i32([11]))
+    c.fork(i32([0]), i32([1]))
+    c.k[c.k != 1], c.v[c.v != 1] = 0, 0
+    assert c.device_status() == 0
+    return c, i32, c.k.clone()
+
+
+@pytest.mark.parametrize("call", ["append", "attention", "accept"])
+def test_nothing_is_stored_into_a_shared_page(call):
+    """Until one of a forked pair is extended, neither may store into the page that both end in."""
+    import torch
+    c, i32, before = forked(3)
+    new = torch.full((1, 3, 1, 16), 2.0, dtype=torch.bfloat16, device="cuda")
+    for slot in ([0], [1]):
+        if call == "append":
+            c.append(0, i32(slot), new, new)
+        elif call == "attention":
+            out = c.tree_attention(0, i32(slot), new, new, new)
+            assert out.isfinite().all() and (out > 1).all()  # the nodes are attended to all the same
+        else:
+            _, taken = c.accept(i32(slot), i32([[-1, 0, 0]]), i32([[5, 6, 7]]), i32([[7, 0, 8]]))
+            assert taken.tolist() == [0]
+        assert c.device_status() == 8
+    assert torch.equal(c.k, before) and c.lens.tolist() == [11, 11]
+    # extended, slot 1 has a page of its own, and slot 0 has its page alone again
+    c.extend(i32([1]), i32([3]))
+    for slot in ([0], [1]):
+        if call == "append":
+            c.append(0, i32(slot), new, new)
+        elif call == "attention":
+            c.tree_attention(0, i32(slot), new, new, new)
+        else:
+            _, taken = c.accept(i32(slot), i32([[-1, 0, 0]]), i32([[5, 6, 7]]), i32([[7, 0, 8]]))
+            assert taken.tolist() == [2]
+        assert c.device_status() == 0
+    if call != "accept":
+        assert (c.k == 2).sum() == 2 * 3 * 16

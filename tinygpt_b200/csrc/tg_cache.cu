@@ -210,6 +210,12 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(CacheView c) {
   }
 }
 
+// Whether the page that slot s's length ends in is its alone: a fork shares it until one of
+// the two is extended, and what one stored there the other would read.
+__device__ __forceinline__ bool owns_end(const CacheView& c, int s, int len) {
+  return !(len & (c.page_size - 1)) || c.refs[c.tables[static_cast<size_t>(s) * c.width + (len >> c.page_log2)]] == 1;
+}
+
 __device__ __forceinline__ void release_page(const CacheView& c, int p) {
   if (atomicSub(&c.refs[p], 1) == 1) atomicOr(&c.free_map[p >> 5], 1u << (p & 31));
 }
@@ -348,6 +354,10 @@ __global__ void __launch_bounds__(kCopyThreads) append_kernel(CacheView c, int l
     bad |= kNotReserved;
     count = static_cast<int>(room);
   }
+  if (count > 0 && !owns_end(c, s, c.lens[s])) {
+    bad |= kNotReserved;
+    count = 0;
+  }
   if (threadIdx.x == 0 && blockIdx.x == 0) report(c, bad);
   const int64_t work = static_cast<int64_t>(count) * c.kv_heads * cols, step = static_cast<int64_t>(gridDim.x) * kCopyThreads;
   for (int64_t u = static_cast<int64_t>(blockIdx.x) * kCopyThreads + threadIdx.x; u < work; u += step) {
@@ -428,7 +438,7 @@ __global__ void __launch_bounds__(kCopyThreads) accept_kernel(CacheView c, int n
   if (!(bad & kBadSlot)) {
     const int len = c.lens[s];
     const int64_t room = static_cast<int64_t>(c.counts[s]) << c.page_log2;
-    if (len + static_cast<int64_t>(count) > room) {  // the tree was not reserved: nothing of it is kept
+    if (len + static_cast<int64_t>(count) > room || (count > 0 && !owns_end(c, s, len))) {  // the tree was not reserved: nothing of it is kept
       bad |= kNotReserved;
       taken = 0;
       mine[0] = mine[1] = out[0] = out[1] = -1;

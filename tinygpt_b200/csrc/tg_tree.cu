@@ -620,14 +620,22 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
       if (a.vec) copy16(base + at, row + (there ? ch * 8 : 0), there);
       else *reinterpret_cast<uint4*>(raw + at) = there ? load8_by_element(row, ch * 8) : make_uint4(0, 0, 0, 0);
     };
+    // what the nodes' places in the cache take to find is on its way before the copies are
+    const bool stores = tree && w.block == 0 && w.nodes > 0;
+    const int first_page = w.len >> c.page_log2, in_page = w.len & (c.page_size - 1);
+    int page = -1, room = 0, holders = 1;  // page: this lane's among those that the nodes go to; 64 nodes reach 9 at most
+    uint64_t seen = 0;
+    if (stores) {
+      room = (c.counts[w.slot] << c.page_log2) - w.len;
+      if (lane < 9 && first_page + lane < c.width) page = c.tables[static_cast<size_t>(w.slot) * c.width + first_page + lane];
+    }
+    if (tree && me < w.nodes) seen = a.masks ? a.masks[static_cast<int64_t>(w.b) * a.nodes + me] : ~0ull >> (63 - me);
     const uint16_t* q_from = a.q.p + w.b * a.q.row + static_cast<int64_t>(w.head) * a.group * a.q.head;
 #pragma unroll 4
     for (int r = first_row; r < rows; r += kRowStep) {
       const int node = divide(rows0 + r, a.group_inverse), h = rows0 + r - node * a.group, rr = r & (kTile - 1);
       bring(q_at + to + (r / kTile) * q_tile + (ch >> 3) * q_block + rr * 128 + ((ch ^ rr) & 7) * 16, q_from + node * a.q.node + h * a.q.head, true);
     }
-    const int room = w.nodes > 0 ? (c.counts[w.slot] << c.page_log2) - w.len : 0, keep = tree && w.block == 0 ? min(w.nodes, room) : 0;
-    int page = -1;  // of this lane's page among those that the nodes go to: 64 nodes reach 9 at most
     if (tree) {
       const uint16_t* k_from = a.k.p + w.b * a.k.row + w.head * a.k.head;
       const uint16_t* v_from = a.v.p + w.b * a.v.row + w.head * a.v.head;
@@ -638,22 +646,21 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
         bring(tk_at + at, k_from + node * a.k.node, j < w.nodes);
         bring(tv_at + at, v_from + node * a.v.node, j < w.nodes);
       }
-      if (me < w.nodes) {
-        const uint64_t all = w.nodes < 64 ? (1ull << w.nodes) - 1 : ~0ull;
-        sets[buffer].of[me] = (a.masks ? a.masks[static_cast<int64_t>(w.b) * a.nodes + me] : ~0ull >> (63 - me)) & all;
-      }
-      const int first_page = w.len >> c.page_log2;
-      if (keep > 0 && first_page + lane <= (w.len + keep - 1) >> c.page_log2) page = c.tables[static_cast<size_t>(w.slot) * c.width + first_page + lane];
-      if (me == 0 && w.block == 0 && w.head == 0 && w.nodes > room) atomicOr(c.status, kNotReserved);
+      if (me < w.nodes) sets[buffer].of[me] = seen & (w.nodes < 64 ? (1ull << w.nodes) - 1 : ~0ull);
+      // the page that the length ends in may be another row's too, forked and not yet copied
+      if (lane == 0 && page >= 0 && in_page) holders = c.refs[page];
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     uint32_t odd_lo = 0, odd_hi = 0;
     if (tree) {
+      holders = __shfl_sync(~0u, holders, 0);
+      const int keep = stores && holders == 1 ? min(w.nodes, room) : 0;
+      if (me == 0 && stores && w.head == 0 && keep < w.nodes) atomicOr(c.status, kNotReserved);
       const int64_t pages = static_cast<int64_t>(a.layer) * c.num_pages;
 #pragma unroll 2
       for (int j = first_row; j < a.tree_rows; j += kRowStep) {  // as often in every lane
         const uint32_t at = to + (ch >> 3) * tree_block + j * 128 + ((ch ^ j) & 7) * 16;
-        const int there = __shfl_sync(~0u, page, ((w.len & (c.page_size - 1)) + j) >> c.page_log2 & 31);
+        const int there = __shfl_sync(~0u, page, (in_page + j) >> c.page_log2 & 31);
         uint4 v = *reinterpret_cast<const uint4*>(raw + tv_at + at);
         if (j < keep && ch * 8 < c.head_dim) {
           const int64_t in_pool = (((pages + there) * c.kv_heads + w.head) << c.page_log2) + ((w.len + j) & (c.page_size - 1));
