@@ -43,6 +43,10 @@ struct CacheView {
 
 }  // namespace tg
 
+// cuTensorMapEncodeTiled
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
 struct tg_cache {
   int device = 0;
   int sms = 0;
@@ -51,6 +55,7 @@ struct tg_cache {
   void* arena = nullptr;   // every device array of the view
   void* partial = nullptr; // attention: outputs of split rows (tg_tree.cu)
   CUtensorMap k_map{}, v_map{};
+  EncodeTiled encode = nullptr;
 };
 
 namespace tg {

@@ -78,6 +78,7 @@ struct TreeArgs {
   int32_t layer, n, nodes, q_heads, group, blocks, min_tiles, vec;  // vec: all rows are 16-byte aligned
   uint32_t group_inverse;  // ceil(2^32 / group)
   int32_t q_rows, tree_rows, slots;  // shared memory: rows of a row block, of the nodes' tile, ring slots
+  int32_t q_box;                     // nodes of a box of Q's tensor map; 0: Q comes by 16-byte copies
   uint32_t ring_block, ring_group;   // bytes from one 64-column block of a slot to the next, from 8 tokens to the next 8
   const int32_t* seqs;
   const int32_t* n_nodes;
@@ -155,6 +156,16 @@ __device__ __forceinline__ void tma_load(uint32_t to, const CUtensorMap* map, ui
       "cp.async.bulk.tensor.5d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %4, %5, %6}], [%2];" ::"r"(to), "l"(map), "r"(bar), "r"(x), "r"(0),
       "r"(y), "r"(z)
       : "memory");
+}
+__device__ __forceinline__ void tma_load_q(uint32_t to, const CUtensorMap* map, uint32_t bar, int x, int head, int node, int b) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(to), "l"(map), "r"(bar), "r"(x), "r"(head),
+      "r"(node), "r"(b)
+      : "memory");
+}
+// Bytes that the phase waits for, beside its arrivals.
+__device__ __forceinline__ void bar_more_bytes(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tmem_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -503,7 +514,8 @@ __device__ __forceinline__ float log_sum(float t, float sum) {
 }
 
 template <int kDim, bool kWide, bool kBf16>
-__global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+__global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                                                            const __grid_constant__ CUtensorMap q_map) {
   using L = Layout<kDim, kWide>;
   constexpr int kRows = L::kRows, kChunks = kDim / 8;
   extern __shared__ __align__(1024) uint8_t raw[];
@@ -631,6 +643,20 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
     }
     if (tree && me < w.nodes) seen = a.masks ? a.masks[static_cast<int64_t>(w.b) * a.nodes + me] : ~0ull >> (63 - me);
     const uint16_t* q_from = a.q.p + w.b * a.q.row + static_cast<int64_t>(w.head) * a.group * a.q.head;
+    if (a.q_box) {
+      if (warp == 10) {
+        const uint32_t bar = smem_addr(&ctl.q_full[buffer]);
+        const int blocks = (rows + kTile - 1) / kTile, node0 = rows0 >= kTile ? rows0 / a.group : 0;
+        if (elect()) {
+          bar_more_bytes(bar, blocks * L::kBlocks * a.q_box * a.group * 128);
+          for (int block = 0; block < blocks; block++)
+#pragma unroll
+            for (int x = 0; x < L::kBlocks; x++)
+              tma_load_q(base + q_at + to + block * q_tile + x * q_block, &q_map, bar, x * 64, w.head * a.group, node0 + block * a.q_box, w.b);
+        }
+        __syncwarp();
+      }
+    } else
 #pragma unroll 4
     for (int r = first_row; r < rows; r += kRowStep) {
       const int node = divide(rows0 + r, a.group_inverse), h = rows0 + r - node * a.group, rr = r & (kTile - 1);
@@ -678,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
     odd_lo = __reduce_or_sync(~0u, odd_lo);
     odd_hi = __reduce_or_sync(~0u, odd_hi);
     if (lane == 0) ctl.odd[segment % 4][warp & 1] = static_cast<uint64_t>(odd_hi) << 32 | odd_lo;
-    if (a.scale < 0.0f) {  // scale's sign goes into Q
+    if (a.scale < 0.0f) {  // scale's sign goes into Q (by copies then)
       for (int r = first_row; r < rows; r += kRowStep) {
         const int rr = r & (kTile - 1);
         uint4* q = reinterpret_cast<uint4*>(raw + q_at + to + (r / kTile) * q_tile + (ch >> 3) * q_block + rr * 128 + ((ch ^ rr) & 7) * 16);
@@ -875,7 +901,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
       ok = load_rows(g, segment);
       warp_arrive(&ctl.seg_empty[k.at]);
     }
-    if (warp == 10 && lane == 0) a.cuts[blockIdx.x] = cut;
+    if (warp == 10 && lane == 0) {
+      a.cuts[blockIdx.x] = cut;
+      if (a.q_box && *reinterpret_cast<volatile int32_t*>(&ctl.give_up))  // no copy may be under way when the block ends
+        for (uint32_t i = 0; i < kBuffers && i < segment; i++) wait_out(&ctl.q_full[i], (segment - 1 - i) / kBuffers & 1);
+    }
   } else if (work && warp < 8) {
     // ---- softmax warps: a thread per row
     const int g = warp >> 2, row = tid & (kTile - 1);       // group, row of its row block
@@ -1153,7 +1183,7 @@ cudaError_t allow_smem() {
 }
 
 template <int kDim, bool kWide, bool kBf16>
-cudaError_t launch(tg_cache* c, TreeArgs a, cudaStream_t st) {
+cudaError_t launch(tg_cache* c, TreeArgs a, const CUtensorMap& q_map, cudaStream_t st) {
   using L = Layout<kDim, kWide>;
   const int rows = a.nodes * a.group < L::kRows ? a.nodes * a.group : L::kRows;
   a.q_rows = kWide ? kTile : (rows + 7) & ~7;
@@ -1166,17 +1196,17 @@ cudaError_t launch(tg_cache* c, TreeArgs a, cudaStream_t st) {
   if (a.slots > kMaxSlots) a.slots = kMaxSlots;
   // the last row block's 128 rows, read from its start, end inside the block's memory:
   // at least 4 slots of 128 rows follow it
-  cudaError_t e = launch_after(tree_kernel<kDim, kWide, kBf16>, dim3(c->sms), kThreads, fixed + a.slots * L::kSlot, st, 1, c->view, a, c->k_map, c->v_map);
+  cudaError_t e = launch_after(tree_kernel<kDim, kWide, kBf16>, dim3(c->sms), kThreads, fixed + a.slots * L::kSlot, st, 1, c->view, a, c->k_map, c->v_map, q_map);
   const dim3 grid(c->sms, (rows + 31) / 32, kDim / 32);
   if (e == cudaSuccess) e = launch_after(join_kernel<kDim, kWide, kBf16>, grid, 256, 0, st, 1, c->view, a);
   return e;
 }
 
 template <int kDim>
-cudaError_t launch_dim(tg_cache* c, const TreeArgs& a, bool wide, cudaStream_t st) {
+cudaError_t launch_dim(tg_cache* c, const TreeArgs& a, const CUtensorMap& q, bool wide, cudaStream_t st) {
   const bool bf16 = c->dtype == TG_DTYPE_BF16;
-  if (wide) return bf16 ? launch<kDim, true, true>(c, a, st) : launch<kDim, true, false>(c, a, st);
-  return bf16 ? launch<kDim, false, true>(c, a, st) : launch<kDim, false, false>(c, a, st);
+  if (wide) return bf16 ? launch<kDim, true, true>(c, a, q, st) : launch<kDim, true, false>(c, a, q, st);
+  return bf16 ? launch<kDim, false, true>(c, a, q, st) : launch<kDim, false, false>(c, a, q, st);
 }
 
 // The workspace: the cut items, then the parts, two per run.
@@ -1186,12 +1216,11 @@ constexpr size_t part_bytes(int sms) { return static_cast<size_t>(sms) * 2 * 2 *
 }  // namespace
 
 int32_t tree_setup(tg_cache* c) noexcept {
-  typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                               CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
   void* fn = nullptr;
   cudaDriverEntryPointQueryResult found;
   TG_TRY(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found));
   if (found != cudaDriverEntryPointSuccess || !fn) return set_error(TG_ERR_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
+  c->encode = reinterpret_cast<EncodeTiled>(fn);
   const CacheView& v = c->view;
   // A box is what a tile needs of a page: 8-token groups of 64-column blocks, as they lie in
   // a slot.  A head dimension of 128 comes as one box of both blocks (dimension 2), since
@@ -1202,9 +1231,9 @@ int32_t tree_setup(tg_cache* c) noexcept {
   const cuuint64_t strides[4] = {d * 2, 128, d * 16, d * 2 * ps};
   const cuuint32_t box[5] = {64, 8, static_cast<cuuint32_t>(joined), static_cast<cuuint32_t>((ps < kTile ? ps : kTile) / 8), 1}, ones[5] = {1, 1, 1, 1, 1};
   for (int i = 0; i < 2; i++) {
-    const CUresult r = reinterpret_cast<EncodeFn>(fn)(i ? &c->v_map : &c->k_map, c->dtype == TG_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
-                                                      i ? v.v : v.k, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                                                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUresult r = c->encode(i ? &c->v_map : &c->k_map, c->dtype == TG_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
+                                 i ? v.v : v.k, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return set_error(TG_ERR_CUDA, "cuTensorMapEncodeTiled failed");
   }
   TG_TRY((allow_smem<64, false, false>()));
@@ -1265,8 +1294,21 @@ int32_t tg_tree_attention(tg_cache* c, int32_t layer, int32_t n, const int32_t* 
   char* space = static_cast<char*>(c->partial);
   a.cuts = reinterpret_cast<tg::CutItem*>(space);
   a.partial = reinterpret_cast<float*>(space + tg::cut_bytes(c->sms));
+  // Q of many rows comes in boxes of whole nodes, heads inside nodes, as its rows lie in shared
+  // memory.  Two warps' 16-byte copies take 170 cycles an instruction of 512 bytes, 11,000 for
+  // 256 rows (91 short sequences of 64 nodes x 8 heads: 88 us by copies, 68 by boxes).
+  CUtensorMap q_map{};
+  if (a.vec && scale >= 0.0f && nodes * a.group > 32 && tg::kTile % a.group == 0 && q_row > 0 && q_node > 0 && q_head > 0) {
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c->view.head_dim), static_cast<cuuint64_t>(q_heads), static_cast<cuuint64_t>(nodes), static_cast<cuuint64_t>(n)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(q_head) * 2, static_cast<cuuint64_t>(q_node) * 2, static_cast<cuuint64_t>(q_row) * 2};
+    const int box_nodes = nodes < tg::kTile / a.group ? nodes : tg::kTile / a.group;
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(a.group), static_cast<cuuint32_t>(box_nodes), 1}, ones[4] = {1, 1, 1, 1};
+    if (c->encode(&q_map, c->dtype == TG_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(q), dims, strides, box, ones,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS)
+      a.q_box = box_nodes;
+  }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  TG_TRY(c->view.head_dim <= 64 ? tg::launch_dim<64>(c, a, wide, st) : tg::launch_dim<128>(c, a, wide, st));
+  TG_TRY(c->view.head_dim <= 64 ? tg::launch_dim<64>(c, a, q_map, wide, st) : tg::launch_dim<128>(c, a, q_map, wide, st));
   return TG_OK;
 }
 
