@@ -34,8 +34,8 @@
 //   part of a tile (16,000 tokens, 32 sequences: 93 us, in pages of 16 118, of 8 153)
 //   the chain S -> P -> O -> S of a group for many rows: 4300 cycles a tile, of which the
 //   weights take 2400 (the exponentials' unit 1024 of them), the products 770, and the waits
-//   between warps the rest: 1 sequence, 64 nodes x 4 heads, 102 us, 0.67 PFLOP/s
-//   the card's power limit for the largest call (64 sequences, 16 nodes): 264 to 290 us, by
+//   between warps the rest: 1 sequence, 64 nodes x 4 heads, 94 us, 0.73 PFLOP/s
+//   the card's power limit for the largest call (64 sequences, 16 nodes): 247 to 275 us, by
 //   the clock that the card holds, 1.66 to 1.75 GHz of 1.96
 //   latency for small calls: 14 us, of which join_kernel's launch takes 3
 // Tried and slower: exponentials of 32 scores beside the next 32's maxima (one vote more a
@@ -1294,11 +1294,13 @@ int32_t tg_tree_attention(tg_cache* c, int32_t layer, int32_t n, const int32_t* 
   char* space = static_cast<char*>(c->partial);
   a.cuts = reinterpret_cast<tg::CutItem*>(space);
   a.partial = reinterpret_cast<float*>(space + tg::cut_bytes(c->sms));
-  // Q of many rows comes in boxes of whole nodes, heads inside nodes, as its rows lie in shared
-  // memory.  Two warps' 16-byte copies take 170 cycles an instruction of 512 bytes, 11,000 for
-  // 256 rows (91 short sequences of 64 nodes x 8 heads: 88 us by copies, 68 by boxes).
+  // Q comes in boxes of whole nodes, heads inside nodes, as its rows lie in shared memory: two
+  // warps' 16-byte copies take 170 cycles an instruction of 512 bytes, 11,000 for 256 rows
+  // (91 short sequences of 64 nodes x 8 heads: 88 us by copies, 67 by boxes; with 4 rows both
+  // take the same).  Copies stay for rows that a map cannot describe (not 16-byte aligned,
+  // a stride of 0, heads that do not fill 128 rows evenly) and for a negative scale.
   CUtensorMap q_map{};
-  if (a.vec && scale >= 0.0f && nodes * a.group > 32 && tg::kTile % a.group == 0 && q_row > 0 && q_node > 0 && q_head > 0) {
+  if (a.vec && scale >= 0.0f && tg::kTile % a.group == 0 && q_row > 0 && q_node > 0 && q_head > 0) {
     const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c->view.head_dim), static_cast<cuuint64_t>(q_heads), static_cast<cuuint64_t>(nodes), static_cast<cuuint64_t>(n)};
     const cuuint64_t strides[3] = {static_cast<cuuint64_t>(q_head) * 2, static_cast<cuuint64_t>(q_node) * 2, static_cast<cuuint64_t>(q_row) * 2};
     const int box_nodes = nodes < tg::kTile / a.group ? nodes : tg::kTile / a.group;
