@@ -646,8 +646,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
     if (a.q_box) {
       if (warp == 10) {
         const uint32_t bar = smem_addr(&ctl.q_full[buffer]);
-        const int blocks = (rows + kTile - 1) / kTile, node0 = rows0 >= kTile ? rows0 / a.group : 0;
-        if (elect()) {
+        // no rows are there where a row block is all past the sequence's nodes
+        const int blocks = rows > 0 ? (rows + kTile - 1) / kTile : 0, node0 = rows0 >= kTile ? rows0 / a.group : 0;
+        if (blocks > 0 && elect()) {
           bar_more_bytes(bar, blocks * L::kBlocks * a.q_box * a.group * 128);
           for (int block = 0; block < blocks; block++)
 #pragma unroll
