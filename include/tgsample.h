@@ -444,7 +444,7 @@ typedef struct tg_cache_state {
 
 /* k_pool, v_pool: device memory, 16-byte aligned, owned by the caller and kept
  * while the handle lives.  Every slot starts empty.  The handle's own memory: about
- * 16 bytes a page, 12 a table entry, 1.1 KB a slot, and 39 MB in which
+ * 16 bytes a page, 8 a table entry, 1.1 KB a slot, and 39 MB in which
  * tg_tree_attention joins what its blocks leave. */
 int32_t tg_cache_create(int32_t device, const tg_cache_config* config, void* k_pool, void* v_pool,
                         tg_cache** out);
