@@ -822,6 +822,8 @@ int32_t tg_beam_select(tg_beam* h, const void* logits, int32_t dtype, int64_t ro
   a.heads = h->heads;
   a.candidates = h->candidates;
   a.status = h->status;
+  static_assert((TG_MAX_VOCAB - 1) / (tg::kThreads * tg::kVecs * 4 * tg::kMaxGroups) + 1 <= tg::kMergeSmem / (TG_MAX_BEAMS * TG_MAX_BEAMS * 8 + TG_MAX_BEAMS * sizeof(tg::PartHead)),
+                "the parts that the longest row asks for fit the merge");
   // the merge holds beams x parts x beams keys, and the parts' heads, in shared memory
   const size_t per_part = static_cast<size_t>(a.beams) * a.beams * 8 + a.beams * sizeof(tg::PartHead), most = tg::kMergeSmem / per_part;
   if (static_cast<size_t>(a.parts) > most) a.parts = static_cast<int>(most);

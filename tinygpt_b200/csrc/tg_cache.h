@@ -5,8 +5,6 @@
 
 #include <cuda.h>
 
-#include <mutex>
-
 #include "tg_host.h"
 
 namespace tg {
