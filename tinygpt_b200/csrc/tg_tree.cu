@@ -78,6 +78,7 @@ struct TreeArgs {
   int32_t layer, n, nodes, q_heads, group, blocks, min_tiles, vec;  // vec: all rows are 16-byte aligned
   uint32_t group_inverse;  // ceil(2^32 / group)
   int32_t q_rows, tree_rows, slots;  // shared memory: rows of a row block, of the nodes' tile, ring slots
+  int32_t buffers;                   // of Q and the nodes: 1 or 2
   int32_t q_box;                     // nodes of a box of Q's tensor map; 0: Q comes by 16-byte copies
   uint32_t ring_block, ring_group;   // bytes from one 64-column block of a slot to the next, from 8 tokens to the next 8
   const int32_t* seqs;
@@ -336,8 +337,8 @@ __device__ __forceinline__ int64_t run_length(int64_t total, int blocks, int min
 
 // In front the control block, then Q (each row block [64-column blocks][q_rows][128 bytes])
 // and the nodes' keys and values ([64-column blocks][tree_rows][128 bytes] each), twice
-// where there is room (the next segment's are loaded while this one runs), and the
-// ring ([64-column blocks][128][128 bytes] per slot).  Q takes only the rows that the call
+// in a narrow block that keeps kMinSlots slots then (the next segment's are loaded while
+// this one runs), and the ring ([64-column blocks][128][128 bytes] per slot).  Q takes only the rows that the call
 // has: the products read 128 rows from its start, and what the rows past the last hold
 // reaches only results that nothing reads.  The space saved is ring: bytes in flight.
 template <int kDim, bool kWide>
@@ -345,9 +346,14 @@ struct Layout {
   static constexpr int kBlocks = kDim / 64;       // 64-column blocks of a row
   static constexpr int kSlot = kTile * kDim * 2;  // 128 keys or values
   static constexpr int kRows = kWide ? 2 * kTile : kTile;
-  static constexpr int kBuffers = kWide ? 1 : 2;  // of Q and the nodes
+  static constexpr int kBuffers = kWide ? 1 : 2;  // of Q and the nodes at most; of the sets and the sums
 };
 constexpr int kMaxSlots = 9;
+// Keys and values take the slots in turn.  A softmax group waits for the last tile's values
+// by parity, which tells a slot's load from the one two before it only if the one before is
+// known to have landed.  From 3 slots on that was a load whose product came before the tile's
+// scores; of 2 slots all values take the second, and the load before may be under way.
+constexpr int kMinSlots = 3;
 
 // A part of an item in the workspace: float4 o[kDim / 4][kRows], float2 (t, sum)[kRows].
 template <int kDim, int kRows>
@@ -371,9 +377,9 @@ struct Control {
   int32_t run_b, give_up;
   uint32_t tmem;
 };
-// After it, by Q buffer: the nodes' sets, and t and sum of each row in each group.  All in
-// front of the 1024-byte-aligned tiles, within 3 KB for a wide block, which leaves it 4
-// ring slots with 64 nodes.
+// After it, by segment modulo kBuffers: the nodes' sets, and t and sum of each row in each
+// group.  All in front of the 1024-byte-aligned tiles, within 3 KB for a wide block, which
+// leaves it 4 ring slots with 64 nodes.
 struct Sets {
   uint64_t of[TG_MAX_TREE_NODES];
 };
@@ -524,9 +530,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
   Sums* sums = reinterpret_cast<Sums*>(raw + kSetsAt + L::kBuffers * sizeof(Sets));
   int64_t* scan = reinterpret_cast<int64_t*>(sums);  // before the roles begin
   constexpr int kBuffers = L::kBuffers;
+  const uint32_t buffers = kWide ? 1 : a.buffers, buffers_log2 = buffers - 1;
   const uint32_t q_block = a.q_rows * 128, q_tile = L::kBlocks * q_block, tree_block = a.tree_rows * 128;  // bytes
   const uint32_t q_at = control_bytes<L::kBuffers>(), tk_at = q_at + (kWide ? 2 : 1) * q_tile, tv_at = tk_at + L::kBlocks * tree_block;
-  const uint32_t q_size = tv_at + L::kBlocks * tree_block - q_at, ring_at = q_at + kBuffers * q_size;  // of a buffer: Q and the nodes
+  const uint32_t q_size = tv_at + L::kBlocks * tree_block - q_at, ring_at = q_at + buffers * q_size;  // of a buffer: Q and the nodes
   const uint32_t base = smem_addr(raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (base & 1023) {  // the swizzle needs it; shared memory starts on such a boundary
@@ -619,8 +626,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
   // Q of a segment and, with tile 0, the nodes' keys and values into a buffer, the nodes'
   // also into the cache: by the two warps 10 and 11.
   const auto load_rows = [&](const Segment& w, uint32_t segment) {
-    const uint32_t buffer = segment % kBuffers;
-    if (segment >= kBuffers && !wait(&ctl, &ctl.q_empty[buffer], (segment / kBuffers - 1) & 1)) return false;
+    const uint32_t buffer = segment & buffers_log2;
+    if (segment >= buffers && !wait(&ctl, &ctl.q_empty[buffer], ((segment >> buffers_log2) - 1) & 1)) return false;
     const uint32_t to = buffer * q_size;
     const int rows0 = w.block * kRows, rows = min(kRows, w.nodes * a.group - rows0);  // rows that are there
     const bool tree = w.t0 == 0;
@@ -673,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
         bring(tk_at + at, k_from + node * a.k.node, j < w.nodes);
         bring(tv_at + at, v_from + node * a.v.node, j < w.nodes);
       }
-      if (me < w.nodes) sets[buffer].of[me] = seen & (w.nodes < 64 ? (1ull << w.nodes) - 1 : ~0ull);
+      if (me < w.nodes) sets[segment % kBuffers].of[me] = seen & (w.nodes < 64 ? (1ull << w.nodes) - 1 : ~0ull);
       // the page that the length ends in may be another row's too, forked and not yet copied
       if (lane == 0 && page >= 0 && in_page) holders = c.refs[page];
     }
@@ -781,7 +788,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
         if (!ok || ctl.seg[k.at].b < 0) break;
         const int t0 = ctl.seg[k.at].t0, t1 = ctl.seg[k.at].t1, len = ctl.seg[k.at].len, nodes = ctl.seg[k.at].nodes;
         const int n = (t1 - t0) * (kWide ? 2 : 1);
-        ok = wait_alone(&ctl, &ctl.q_full[segment % kBuffers], segment / kBuffers & 1);
+        ok = wait_alone(&ctl, &ctl.q_full[segment & buffers_log2], segment >> buffers_log2 & 1);
         tmem_after();
         bool k_ready = false;  // the next keys were seen in the ring
         // Step j, a tile for group s, makes the output of its tile, 64 keys as soon as their
@@ -824,7 +831,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
             }
             if (j == n - 1) {
               tmem_commit(smem_addr(&ctl.done));
-              if (n < kEarly) tmem_commit(smem_addr(&ctl.q_empty[segment % kBuffers]));
+              if (n < kEarly) tmem_commit(smem_addr(&ctl.q_empty[segment & buffers_log2]));
             }
           }
           if (j + 2 < n) {
@@ -840,7 +847,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
 #pragma unroll
             for (int i = 0; i < kDim / 16; i++) mma_ss(d, qd + (i >> 2) * q_step + (i & 3) * 2, kd + (i >> 2) * step + (i & 3) * 2, inst, i > 0);
             tmem_commit(smem_addr(&ctl.s_full[s]));
-            if (j == n - 3 && n >= kEarly) tmem_commit(smem_addr(&ctl.q_empty[segment % kBuffers]));
+            if (j == n - 3 && n >= kEarly) tmem_commit(smem_addr(&ctl.q_empty[segment & buffers_log2]));
             if (t > 0 && last_use) {
               tmem_commit(smem_addr(&ctl.empty[k_slot]));
               k_slot += 2;
@@ -849,7 +856,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
           }
         }
         segment++;
-        if (kBuffers == 2) {
+        if (buffers == 2) {
           const uint64_t to = segment & 1 ? q_size / 16 : -static_cast<uint64_t>(q_size / 16);  // the other buffer
           q_desc += to, tk_desc += to, tv_desc += to;
         }
@@ -905,7 +912,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
     if (warp == 10 && lane == 0) {
       a.cuts[blockIdx.x] = cut;
       if (a.q_box && *reinterpret_cast<volatile int32_t*>(&ctl.give_up))  // no copy may be under way when the block ends
-        for (uint32_t i = 0; i < kBuffers && i < segment; i++) wait_out(&ctl.q_full[i], (segment - 1 - i) / kBuffers & 1);
+        for (uint32_t i = 0; i < buffers && i < segment; i++) wait_out(&ctl.q_full[i], (segment - 1 - i) >> buffers_log2 & 1);
     }
   } else if (work && warp < 8) {
     // ---- softmax warps: a thread per row
@@ -1189,14 +1196,19 @@ cudaError_t launch(tg_cache* c, TreeArgs a, const CUtensorMap& q_map, cudaStream
   const int rows = a.nodes * a.group < L::kRows ? a.nodes * a.group : L::kRows;
   a.q_rows = kWide ? kTile : (rows + 7) & ~7;
   a.tree_rows = (a.nodes + 15) & ~15;
-  const int fixed = control_bytes<L::kBuffers>() + L::kBuffers * ((kWide ? 2 : 1) * a.q_rows + 2 * a.tree_rows) * kDim * 2;
+  constexpr int kRowBlocks = kWide ? 2 : 1, kRoom = kMaxSmem - control_bytes<L::kBuffers>();
+  static_assert((kRoom - (kRowBlocks * kTile + 2 * kTreeTile) * kDim * 2) / L::kSlot >= kMinSlots, "one buffer of any call leaves enough slots");
+  const int buffer = (kRowBlocks * a.q_rows + 2 * a.tree_rows) * kDim * 2;
+  a.buffers = L::kBuffers;
+  if (kRoom - a.buffers * buffer < kMinSlots * L::kSlot) a.buffers = 1;
+  const int fixed = control_bytes<L::kBuffers>() + a.buffers * buffer;
   a.slots = (kMaxSmem - fixed) / L::kSlot;
   const bool joined = c->view.head_dim == 128;  // as tree_setup's boxes
   a.ring_block = joined ? 1024 : kTile * 128;
   a.ring_group = joined ? 2048 : 1024;
   if (a.slots > kMaxSlots) a.slots = kMaxSlots;
   // the last row block's 128 rows, read from its start, end inside the block's memory:
-  // at least 4 slots of 128 rows follow it
+  // at least kMinSlots slots of 128 rows follow it
   cudaError_t e = launch_after(tree_kernel<kDim, kWide, kBf16>, dim3(c->sms), kThreads, fixed + a.slots * L::kSlot, st, 1, c->view, a, c->k_map, c->v_map, q_map);
   const dim3 grid(c->sms, (rows + 31) / 32, kDim / 32);
   if (e == cudaSuccess) e = launch_after(join_kernel<kDim, kWide, kBf16>, grid, 256, 0, st, 1, c->view, a);
