@@ -190,12 +190,15 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 }
 
 // sum 2^(x log2e - t), rescaled when a group exceeds t: t is a rounded x log2e, so
-// every term is at most about 1, and lse = t / log2e + ln(sum) has no error from the
-// rounding of t.
+// the largest term is 1 but for t's rounding, which lse = t / log2e + ln(sum) takes out
+// again.  From logits of about 2^30 on that rounding alone is a hundred binary orders and
+// more: the sum is then 0 or infinite, and the row is left to row_exact.
 struct Sum {
   float t = -INFINITY, l = 0.0f;
   __device__ __forceinline__ void raise(float top) {
-    const float at = top * kLog2e;
+    // finite for every finite logit: with t = -inf the terms of the lowest values, as masks
+    // have them, would be infinite and not 0 beside ordinary ones
+    const float at = top > -INFINITY ? fmaxf(top * kLog2e, -FLT_MAX) : top;
     if (at > t) {
       l *= exp2_fast(t - at);
       t = at;
@@ -385,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(BeamArgs a) {
     if (tid == 0) {
       a.heads[at].t = s.t;
       a.heads[at].l = s.l;
-      // NaN, +inf or logits beyond the range of x log2e in the part: its sum is not finite
+      // NaN, +inf or logits far beyond what t can tell apart in the part: its sum is not finite
       a.heads[at].count = n <= kListMax && s.l < INFINITY && s.t < INFINITY ? kept : -1;
     }
   }
@@ -517,6 +520,8 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(BeamArgs a) {
     if (lane == 0) lse[w] = top, row_sum[w] = sum;
   }
   __syncthreads();
+  // a sum that fp32 does not hold (see Sum): row_exact
+  if (tid < W && lse[tid] > -INFINITY && !(row_sum[tid] > 0.0f && row_sum[tid] < INFINITY)) exact[tid] = 1;
   if (tid < W && lse[tid] > -INFINITY)
     lse[tid] = static_cast<float>(static_cast<double>(lse[tid]) * (1.0 / static_cast<double>(kLog2e)) + log(static_cast<double>(row_sum[tid])));
   __syncthreads();
