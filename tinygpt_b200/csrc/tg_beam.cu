@@ -13,7 +13,7 @@
 //
 // Order is by score in fp32, then index, while a part's list is cut by logit.  The two
 // differ only where rounding gives two different logits one score; merge_kernel looks
-// for that at every list's cut and then, as for rows with NaN or +inf or with more ties
+// for that at every list's cut, among the kept logits and below the cut, and then, as for rows with NaN or +inf or with more ties
 // than a list holds, finds the row's list from the logits themselves (row_exact).
 //
 // Bound and figures (B200): HBM bytes for many rows, each logit once; 1024 rows of 128,256
@@ -111,6 +111,8 @@ struct Elem<TG_DTYPE_F32> {
     x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
   }
   static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+  // the next smaller value of the type
+  static __device__ __forceinline__ float below(float x) { return nextafterf(x, -INFINITY); }
   static __device__ __forceinline__ uint4 masked(const uint4& v, uint32_t bits) {
     return make_uint4(bits & 1 ? v.x : 0xff800000u, bits & 2 ? v.y : 0xff800000u, bits & 4 ? v.z : 0xff800000u, bits & 8 ? v.w : 0xff800000u);
   }
@@ -141,6 +143,10 @@ struct Elem<TG_DTYPE_BF16> {
     }
   }
   static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+  static __device__ __forceinline__ float below(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return __uint_as_float(x == 0.0f ? 0x80010000u : x > 0.0f ? b - 0x10000u : b + 0x10000u);
+  }
   static __device__ __forceinline__ uint32_t masked_word(uint32_t w, uint32_t bits) {
     return (bits & 1 ? w & 0xffffu : 0xff80u) | (bits & 2 ? w & 0xffff0000u : 0xff800000u);
   }
@@ -605,7 +611,9 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(BeamArgs a) {
     }
     __syncthreads();
     // A logit that a list left out matters only if it has the score of one that the
-    // list kept with a larger logit, and that score reaches the selection.
+    // list kept with a larger logit, and that score reaches the selection.  The largest
+    // left out has it then; beside kept ones of its own logit, which come before it, a
+    // smaller one may.
     const uint64_t last = best[W - 1];
     for (int i = tid; i < W * P; i += kMergeThreads) {
       const int w = i / P;
@@ -618,7 +626,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(BeamArgs a) {
         const uint64_t k = keys[i * W + r];
         if (k == 0 || score_of(k) != s) break;
         const Candidate c = a.candidates[(static_cast<int64_t>(row0) * P + i) * W + r];
-        if (c.x != h.cut) {
+        if (c.x != h.cut || score(Elem<DT>::below(h.cut), lse[w], beam[w]) == s) {
           exact[w] = 1;
           break;
         }
