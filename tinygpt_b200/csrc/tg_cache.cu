@@ -421,6 +421,14 @@ __global__ void __launch_bounds__(kCopyThreads) accept_kernel(CacheView c, int n
     tok[h] = in ? tokens[base + j] : 0;
     id[h] = in ? ids[base + j] : 0;
   }
+  int len = 0;
+  if (!bad) {
+    len = c.lens[s];
+    if (static_cast<int64_t>(len) + count > static_cast<int64_t>(c.counts[s]) << c.page_log2 || (count > 0 && !owns_end(c, s, len))) {
+      bad |= kNotReserved;
+      count = 0;
+    }
+  }
   // a child has a higher number than its parent, so the path ascends and ends
   int taken = 0, mine[2] = {-1, -1}, out[2] = {-1, -1};  // the path's entries l and l + 32, and their ids
   for (int at = count > 0 ? 0 : -1; at >= 0;) {
@@ -435,14 +443,7 @@ __global__ void __launch_bounds__(kCopyThreads) accept_kernel(CacheView c, int n
     at = lo ? __ffs(lo) - 1 : hi ? __ffs(hi) + 31 : -1;
   }
   int moved = 0;
-  if (!(bad & kBadSlot)) {
-    const int len = c.lens[s];
-    const int64_t room = static_cast<int64_t>(c.counts[s]) << c.page_log2;
-    if (len + static_cast<int64_t>(count) > room || (count > 0 && !owns_end(c, s, len))) {  // the tree was not reserved: nothing of it is kept
-      bad |= kNotReserved;
-      taken = 0;
-      mine[0] = mine[1] = out[0] = out[1] = -1;
-    }
+  if (!bad) {  // else the row stays as it is, what it has reserved included
     const int32_t* row = c.tables + static_cast<size_t>(s) * c.width;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
