@@ -457,7 +457,8 @@ int32_t tg_cache_device_status(tg_cache* c, uint32_t* out_bits);
 /* Reserves pages so that row i can store counts[i] tokens past its length.  Where
  * those would start in a page that other rows hold too, the row gets a copy of
  * its part of that page, in every layer (of several such rows in one call that
- * are the page's only holders, the first keeps the page).  seqs, counts: [n]. */
+ * are the page's only holders, the first keeps the page, and is served only if
+ * all the others are).  seqs, counts: [n]. */
 int32_t tg_cache_extend(tg_cache* c, int32_t n, const int32_t* seqs, const int32_t* counts, void* stream);
 
 /* Slot dst[i] becomes a copy of slot src[i] as it was before the call (src[i] = -1:

@@ -63,6 +63,9 @@ __device__ int block_prefix(int x, int* warp_sums, int* total) {
   return r;
 }
 
+constexpr int kShort = -1;               // in `first`: a row's copy of this page does not fit
+constexpr int kKeeperShort = 1 << 30;    // in `need`: the row would keep such a page (a table row has at most 2^28 pages)
+
 // One block, since rows take pages in order: two prefix sums over the block, one over the
 // rows' wishes and one over the bitmap, are all that orders them.  Pages for each row's next
 // counts[i] tokens.  Latency, about 6 us with 64 rows.
@@ -129,6 +132,19 @@ __global__ void __launch_bounds__(kBlock) extend_kernel(CacheView c, int n, cons
     for (int w = w0; w < w1 && rank < total; w++) {
       for (uint32_t m = __ldcg(&c.free_map[w]); m && rank < total; m &= m - 1) c.list[rank++] = (w << 5) + __ffs(m) - 1;
     }
+    if (total > avail) {
+      // the first of a shared page's only holders keeps it if the others copy it: where a copy
+      // does not fit, the page has two holders left and the first, who may not store, is not served either
+      for (int i = tid; i < n; i += kBlock) {
+        const int need = c.need[i], takes = (need >> 1) + (need & 1);
+        if (need > 0 && (need & 1) && c.start[i] + takes > avail) c.first[c.last[i]] = kShort;
+      }
+      __syncthreads();
+      for (int i = tid; i < n; i += kBlock) {
+        const int need = c.need[i], last = c.last[i];
+        if (need >= 0 && !(need & 1) && last >= 0 && c.first[last] == kShort) c.need[i] = need | kKeeperShort;
+      }
+    }
     __syncthreads();
     const int given = min(total, avail);
     for (int e = tid; e < given; e += kBlock) {
@@ -138,7 +154,7 @@ __global__ void __launch_bounds__(kBlock) extend_kernel(CacheView c, int n, cons
         if (c.start[mid] <= e) lo = mid; else hi = mid - 1;
       }
       const int need = c.need[lo], copy = need & 1, k = e - c.start[lo];
-      if (c.start[lo] + (need >> 1) + copy > avail) continue;  // the row does not fit
+      if ((need & kKeeperShort) || c.start[lo] + (need >> 1) + copy > avail) continue;  // the row is not served
       const int s = seqs[lo], p = c.list[e], len = c.lens[s];
       int32_t* row = c.tables + static_cast<size_t>(s) * c.width;
       c.refs[p] = 1;
@@ -157,12 +173,12 @@ __global__ void __launch_bounds__(kBlock) extend_kernel(CacheView c, int n, cons
   for (int i = tid; i < n; i += kBlock) {
     const int need = c.need[i];
     if (need < 0) continue;
-    const int s = seqs[i], last = c.last[i], takes = (need >> 1) + (need & 1);
+    const int s = seqs[i], last = c.last[i], takes = ((need & ~kKeeperShort) >> 1) + (need & 1);
     if (last >= 0) {
       c.shared[last] = 0;
       c.first[last] = INT_MAX;
     }
-    if (takes > 0 && c.start[i] + takes > avail) bad |= kNoPages;
+    if ((need & kKeeperShort) || (takes > 0 && c.start[i] + takes > avail)) bad |= kNoPages;
     else c.counts[s] += need >> 1;
     c.claim[s] = 0;
   }

@@ -28,7 +28,7 @@ struct CacheView {
   int32_t* shared;   // [num_pages] rows of the call that would write to this page
   int32_t* first;    // [num_pages] the first of them
   int32_t* start;    // [max_seqs]  row -> its first page in `list`
-  int32_t* need;     // [max_seqs]  row -> 2 * new pages + (1 if its last page is copied), -1: not served
+  int32_t* need;     // [max_seqs]  row -> 2 * new pages + (1 if its last page is copied), -1: not in the call
   int32_t* last;     // [max_seqs]  row -> its partly filled last page or -1
   int32_t* list;     // [num_pages] pages handed out by the call
   int4* copies;      // [max_seqs]  (from, to, tokens, -)
