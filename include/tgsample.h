@@ -473,7 +473,8 @@ int32_t tg_cache_fork(tg_cache* c, int32_t n, const int32_t* src, const int32_t*
  * reserved ones included. */
 int32_t tg_cache_truncate(tg_cache* c, int32_t n, const int32_t* seqs, const int32_t* lens, void* stream);
 
-/* Advances row i's length by counts[i] tokens, already stored in reserved pages. */
+/* Advances row i's length by counts[i] tokens, already stored in reserved pages (a
+ * slot that is given more than once, by each of its rows that still fits). */
 int32_t tg_cache_commit(tg_cache* c, int32_t n, const int32_t* seqs, const int32_t* counts, void* stream);
 
 /* Stores tokens' keys and values in one layer at row i's positions length ..

@@ -336,10 +336,26 @@ __global__ void __launch_bounds__(kCopyThreads) commit_kernel(CacheView c, int n
   after_previous_work();
   if (i >= n) return;
   const int s = seqs[i], more = counts[i];
-  if (s < 0 || s >= c.max_seqs) report(c, kBadSlot);
-  else if (more < 0) report(c, kBadLength);
-  else if (static_cast<int64_t>(c.lens[s]) + more > static_cast<int64_t>(c.counts[s]) << c.page_log2) report(c, kNotReserved);
-  else c.lens[s] += more;
+  if (s < 0 || s >= c.max_seqs) {
+    report(c, kBadSlot);
+    return;
+  }
+  if (more < 0) {
+    report(c, kBadLength);
+    return;
+  }
+  // checked and stored at once: a slot given twice must not pass its pages, whose ids later
+  // calls follow up to the length.  A failed exchange means that another row advanced.
+  const int64_t room = static_cast<int64_t>(c.counts[s]) << c.page_log2;
+  for (int len = __ldcg(&c.lens[s]);;) {
+    if (static_cast<int64_t>(len) + more > room) {
+      report(c, kNotReserved);
+      return;
+    }
+    const int now = atomicCAS(&c.lens[s], len, len + more);
+    if (now == len) return;
+    len = now;
+  }
 }
 
 struct Tokens {  // [n, tokens, kv_heads, head_dim]: strides in bytes
