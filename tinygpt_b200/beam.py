@@ -11,7 +11,7 @@ import ctypes
 from typing import NamedTuple
 
 from . import _lib
-from ._device import address, stream_address
+from ._device import address, on_its_stream, stream_address
 from ._lib import check
 from .sampler import _dtype_code
 
@@ -64,11 +64,13 @@ class BeamSearch:
         if t is not None and (t.dtype is not dtype or t.shape != shape or t.get_device() != self.device or not t.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on CUDA device {self.device}")
 
+    @on_its_stream
     def select(self, logits, scores, *, finished=None, eos_id: int = -1, pad_id: int = 0, mask_table=None, state_id=None,
                history=None, history_len=None, stream=None) -> Beams:
         """logits [batch * beams, vocab or more] fp32/bf16, scores float32 [batch, beams] (-inf: a beam that does not
         take part, as all but the first at the start), finished int32 [batch, beams], mask_table and state_id as
-        Sampler.sample, history int32 [batch * beams, stride] with history_len [batch * beams]."""
+        Sampler.sample, history int32 [batch * beams, stride] with history_len [batch * beams].  With `stream` given the
+        results are allocated for it, and inputs have to be ready on it."""
         B, W = scores.shape
         rows = B * W
         if W != self.beams or logits.dim() != 2 or logits.shape[0] != rows or logits.shape[1] < self.vocab:

@@ -11,7 +11,8 @@ nodes' logits -> accept.  A beam step:  BeamSearch.select -> fork -> extend ->
 tree_attention (every layer, one node) -> commit.
 
 Device arrays are torch CUDA tensors; every call goes through libtgsample.so on the
-current stream (or `stream`).
+current stream (or `stream`: results are allocated for it, inputs have to be ready on it
+and to be kept until it has run the call).
 """
 from __future__ import annotations
 
@@ -19,7 +20,7 @@ import ctypes
 import math
 
 from . import _lib
-from ._device import address, stream_address
+from ._device import address, on_its_stream, stream_address, stream_scope
 from ._lib import check
 
 try:
@@ -73,10 +74,10 @@ def tree_masks(parents, n_nodes=None, *, out=None, stream=None):
         raise ValueError("parents must be a CUDA tensor")
     _dense(parents, "parents", (n, nodes), dev, torch.int32)
     _rows(n_nodes, "n_nodes", n, dev)
-    if out is None:
-        out = torch.empty((n, nodes), dtype=torch.int64, device=parents.device)
-    _dense(out, "out", (n, nodes), dev, torch.int64)
-    with torch.cuda.device(dev):
+    with torch.cuda.device(dev), stream_scope(stream, dev):
+        if out is None:
+            out = torch.empty((n, nodes), dtype=torch.int64, device=parents.device)
+        _dense(out, "out", (n, nodes), dev, torch.int64)
         check(_lib.load().tg_tree_masks(n, nodes, address(n_nodes), address(parents), address(out), stream_address(stream, dev)))
     return out
 
@@ -184,6 +185,7 @@ class PagedCache:
         check(self._L.tg_cache_append(self._h, layer, n, seqs.data_ptr(), address(counts), shape[1], k.data_ptr(), ks[0], ks[1], ks[2],
                                       v.data_ptr(), vs[0], vs[1], vs[2], stream_address(stream, self.device)))
 
+    @on_its_stream
     def tree_attention(self, layer: int, seqs, q, k, v, masks=None, *, n_nodes=None, scale: float | None = None, out=None,
                        want_lse: bool = False, lse=None, stream=None):
         """tg_tree_attention: q [n, nodes, q_heads, head_dim] over the slots' cached tokens and the nodes' own k, v
@@ -213,6 +215,7 @@ class PagedCache:
                                         stream_address(stream, device)))
         return out if lse is None else (out, lse)
 
+    @on_its_stream
     def accept(self, seqs, parents, tokens, ids, *, n_nodes=None, out_ids=None, out_n=None, stream=None):
         """tg_cache_accept: walks each tree (parents, drafted tokens [n, nodes]) with the target's ids [n, nodes] and
         keeps the accepted path in the cache.  Returns (out_ids int32 [n, nodes], out_n int32 [n])."""
