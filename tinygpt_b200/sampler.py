@@ -10,7 +10,8 @@ Reference call sites this mirrors (sarthak-fleet/tinygpt):
       native-mac/Sources/TinyGPT/SpeculativeDecode.swift:41-210
 
 Device arrays are torch CUDA tensors (torch is only the allocator and stream
-provider here); every call goes through libtgsample.so.
+provider here); every call goes through libtgsample.so.  Results of a call that names
+a stream are allocated for that stream.
 """
 from __future__ import annotations
 
@@ -19,6 +20,7 @@ import ctypes
 import numpy as np
 
 from . import _lib
+from ._device import on_its_stream
 from ._lib import ROW_PARAMS_DTYPE, TGError, check  # noqa: F401
 
 try:
@@ -109,6 +111,7 @@ class Sampler:
         except Exception:  # noqa: BLE001
             pass
 
+    @on_its_stream
     def sample(self, logits, params, *, history=None, history_len=None, mask_table=None,
                state_id=None, uniforms=None, out=None, out_probs=None, stream=None):
         """tg_sample on device tensors.  logits [B, stride] fp32/bf16; params is a
@@ -164,6 +167,7 @@ class Sampler:
                                      p(state_id), p(uniforms), p(out), p(probs)))
         return out, probs
 
+    @on_its_stream
     def spec_verify(self, target_logits, draft_logits, draft_ids, temperature, u_accept, u_draw,
                     *, out=None, out_n=None, stream=None):
         """tg_spec_verify on device tensors.  target [B, K+1, V], draft [B, K, V]
@@ -185,6 +189,7 @@ class Sampler:
                                      _ptr(out_n), _stream_ptr(stream)))
         return out, out_n
 
+    @on_its_stream
     def spec_verify_masked(self, target_logits, draft_logits, draft_ids, temperature, u_accept,
                            u_draw, mask_table, state_ids, *, out=None, out_n=None, stream=None):
         """tg_spec_verify_masked: mask_table int32/uint32 [S, ceil(V/32)] and
@@ -205,6 +210,7 @@ class Sampler:
                                             _ptr(out), _ptr(out_n), _stream_ptr(stream)))
         return out, out_n
 
+    @on_its_stream
     def sample_shard_local(self, logits, params, vocab_offset: int, full_vocab: int, *,
                            history=None, history_len=None, mask_table=None, state_id=None,
                            out_records=None, stream=None):
@@ -225,6 +231,7 @@ class Sampler:
                                             _ptr(out_records), _stream_ptr(stream)))
         return out_records
 
+    @on_its_stream
     def sample_shard_merge(self, records, full_vocab: int, params, *, uniforms=None, out=None,
                            out_probs=None, stream=None):
         """tg_sample_shard_merge over gathered records uint8 [nshards, B, RECORD]."""
@@ -239,6 +246,7 @@ class Sampler:
                                             _ptr(out_probs), _stream_ptr(stream)))
         return out, out_probs
 
+    @on_its_stream
     def sample_sharded(self, nccl_comm, nranks: int, logits, params, vocab_offset: int, full_vocab: int, *,
                        history=None, history_len=None, mask_table=None, state_id=None, uniforms=None,
                        out=None, out_probs=None, stream=None):
