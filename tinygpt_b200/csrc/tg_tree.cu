@@ -44,8 +44,9 @@
 //
 // Rounding: S, the sums and O are fp32; P is rounded to the cache's type for the tensor
 // cores (the products with V take 16-bit operands), relative 2^-8 (bf16) or 2^-11
-// (f16) of a weight, and the output once.  t moves only when a row's maximum exceeds it
-// by more than 8, so P stays below 2^8 and O is rarely rescaled.
+// (f16, down to 2^-21 of the row's largest weight, below that to 2^-32 of it) of a weight, and
+// the output once.  t moves only when a row's maximum exceeds its first by more than 8, so P
+// stays below 2^8 (f16: 2^15) and O is rarely rescaled.
 #include "tg_cache.h"
 
 #include <cuda_bf16.h>
@@ -62,7 +63,12 @@ constexpr int kTile = 128;       // cached tokens of a tile, rows of a row block
 constexpr int kTreeTile = TG_MAX_TREE_NODES;
 constexpr int kWaitLimit = 1 << 24;
 constexpr long long kWaitCycles = 1ll << 31;
-constexpr float kSlack = 8.0f;   // log2 of how far P may exceed 1
+constexpr float kSlack = 8.0f;   // log2 of how far P may exceed its first maximum
+// log2 of that: f16 weights use the type's range, since those below 2^-14 lose bits and those
+// below 2^-25 are 0.  2^(7 + 8) is below its largest value; a row's largest weight is at
+// least 2^7, so bits are lost below 2^-21 of it, all of a weight below 2^-32.
+template <bool kBf16>
+constexpr float kFirst = kBf16 ? 0.0f : 7.0f;
 constexpr float kLog2e = 1.44269504f;
 
 // x / group by ceil(2^32 / group) (0: group 1): exact while x group^2 < 2^32, as rows below
@@ -978,10 +984,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
 #pragma unroll
             for (int e = 0; e < 64; e += 2) m[e >> 1 & 3] = max3(m[e >> 1 & 3], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
             const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * cs;
-            const bool move = top > t_ref + kSlack;
+            // the difference, not a sum with t: that would be rounded where scores are huge
+            const bool move = top - t_ref > kFirst<kBf16> + kSlack;
             if (__any_sync(~0u, move)) {
-              const float f = move ? exp2_fast(t_ref - top) : 1.0f;
-              if (move) t_ref = top;
+              const float to = top - kFirst<kBf16>, f = move ? exp2_fast(t_ref - to) : 1.0f;
+              if (move) t_ref = to;
               sum[0] = mul2(sum[0], two(f, f)), sum[1] = mul2(sum[1], two(f, f));
               if (half) {  // the products with the first half's weights are to end first; those
                            // of the tiles before had when this one's scores were made
