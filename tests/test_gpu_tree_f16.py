@@ -89,3 +89,14 @@ def test_values_at_the_ends_of_the_range(cuda_lib):
     out, _ = case.run()
     # the weights' sum and the sum of their rounded ones differ by 2^-11 at most
     assert (out.double() - 65504.0).abs().max() <= 65504.0 * 2.0 ** -10 and torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("nodes,heads", [(1, 1), (3, 4), (64, 4)])
+@pytest.mark.parametrize("tokens,weight_log2", [(1 << 20, -25.25), (1 << 20, -22.5), (1 << 18, -24.75), (70001, -19.3), (5000, -13.0), (5000, -3.0)])
+def test_sum_of_small_weights(cuda_lib, tokens, weight_log2, nodes, heads):
+    """The logarithm of a row's sum counts the small weights beside a large one: 64 of them meet it at a time."""
+    for at in (0, 127, tokens - 1):
+        _, lse = some_large(tokens, weight_log2, [at], nodes, heads)
+        total = 1 + (tokens - 1) * 2.0 ** weight_log2
+        move = 3 * 2.0 ** -23 * 18 + 2.0 ** -18
+        assert (lse - (-weight_log2 * np.log(2.0) + np.log(total))).abs().max() <= move + 2.0 ** -20 * 24

@@ -939,7 +939,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
       const int node = mine ? divide(rows0 + r, a.group_inverse) : 0, h = w.head * a.group + (mine ? rows0 + r - node * a.group : 0);
       uint64_t sees = 0;
       float t_ref = -INFINITY;
-      uint64_t sum[2] = {0, 0};
+      uint64_t sum = 0;
       bool clear = segment == 0;  // the last segment's O has been read
       const int step = kWide ? 1 : 2;
       for (int t = w.t0 + (kWide ? 0 : g); ok && t < w.t1; t += step) {
@@ -989,7 +989,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
             if (__any_sync(~0u, move)) {
               const float to = top - kFirst<kBf16>, f = move ? exp2_fast(t_ref - to) : 1.0f;
               if (move) t_ref = to;
-              sum[0] = mul2(sum[0], two(f, f)), sum[1] = mul2(sum[1], two(f, f));
+              sum = mul2(sum, two(f, f));
               if (half) {  // the products with the first half's weights are to end first; those
                            // of the tiles before had when this one's scores were made
                 ok = wait(&ctl, &ctl.half_done[g], s_turn & 1);
@@ -1000,13 +1000,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
             }
             const float t_use = t_ref == -INFINITY ? 0.0f : t_ref;
             const uint64_t scale = two(cs, cs), from = two(-t_use, -t_use);
+            uint64_t part[2] = {0, 0};  // small weights add up before they meet the row's sum
 #pragma unroll
             for (int e = 0; e < 64; e += 2) {
               const uint64_t x = fma2(two(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), scale, from);
               const float p0 = exp2_fast(low_of(x)), p1 = exp2_fast(high_of(x));
-              sum[e >> 1 & 1] = add2(sum[e >> 1 & 1], two(p0, p1));
+              part[e >> 1 & 1] = add2(part[e >> 1 & 1], two(p0, p1));
               v[e / 2] = pack<kBf16>(p0, p1);
             }
+            sum = add2(sum, add2(part[0], part[1]));
             tmem_store16(s_at + half * 32, v);
             tmem_store16(s_at + half * 32 + 16, v + 16);
             tmem_wait_st();
@@ -1025,7 +1027,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(CacheView c, TreeArgs
       if (!ok) break;
       loaded += 2 * (w.t1 - max(w.t0, 1));
       sums[segment % kBuffers].t[g][row] = t_ref;
-      sums[segment % kBuffers].sum[g][row] = (low_of(sum[0]) + high_of(sum[0])) + (low_of(sum[1]) + high_of(sum[1]));
+      sums[segment % kBuffers].sum[g][row] = low_of(sum) + high_of(sum);
       warp_arrive(&ctl.stats);
       segment++;
       warp_arrive(&ctl.seg_empty[k.at]);
