@@ -19,7 +19,9 @@
 // Bound and figures (B200): HBM bytes for many rows, each logit once; 1024 rows of 128,256
 // bf16 logits take 61 us (263 MB, 4.4 TB/s): the stream itself runs at 6.4 TB/s, the lists
 // at its blocks' ends and merge_kernel take a third of the time.  Latency for few: 4 rows
-// of 50,257 fp32 logits 10.5 us, half of it the merge.
+// of 50,257 fp32 logits 11 us, half of it the merge.  A batch row with rows for row_exact
+// takes far longer: 0.13 ms with one row of 50,257 and 4 beams, 0.7 ms with one of 128,256 and
+// 8 beams, 5 ms with all 8; 64 x 16 such rows 20 ms.
 //
 // One launch instead of two, the last block of a batch row merging it, was slower on the
 // device (66 and 12 us: every block waits for its fence and its arrival, and the merge

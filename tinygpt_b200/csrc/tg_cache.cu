@@ -12,7 +12,7 @@
 // layers: 12 us in 3 launches; 64 trees accepted in 32 layers, with truncate and extend:
 // 20 us in 5).  The copies are HBM bytes, 2 x (tokens x kv_heads x head_dim x 2 B x 2
 // pools x layers): 64 pages in 32 layers, 603 MB, 87 us for fork and extend together,
-// 6.9 TB/s.
+// 6.9 TB/s; 64 x 512 tokens of 8 heads appended, 268 MB, 43 us, 6.2 TB/s.
 #include "tg_cache.h"
 
 #include <climits>

@@ -28,16 +28,17 @@
 //           nodes of a segment ahead, the nodes also into the cache
 //   12-15   join a segment's two groups and write its rows, while the others go on
 //
-// Bound and figures (B200; 6.5 TB/s and 1.65 PFLOP/s by the card's own copy and GEMM):
-//   HBM for decoding: 64 sequences, 1 node, 114 us for 622 MB, 5.4 TB/s.  Pages below 64
-//   tokens cost more: the copy engine takes about 75 cycles a box and a box is a page's
+// Bound and figures (B200; 6.5 TB/s and 1.65 PFLOP/s by the card's own copy and GEMM; in
+// bursts of some ms, and in brackets over a second of calls, which the card runs slower):
+//   HBM for decoding: 64 sequences, 1 node, 115 (130) us for 622 MB, 5.4 TB/s (4.8).  Pages
+//   below 64 tokens cost more: the copy engine takes about 75 cycles a box and a box is a page's
 //   part of a tile (16,000 tokens, 32 sequences: 93 us, in pages of 16 118, of 8 153)
 //   the chain S -> P -> O -> S of a group for many rows: 4300 cycles a tile, of which the
 //   weights take 2400 (the exponentials' unit 1024 of them), the products 770, and the waits
-//   between warps the rest: 1 sequence, 64 nodes x 4 heads, 94 us, 0.73 PFLOP/s
-//   the card's power limit for the largest call (64 sequences, 16 nodes): 247 to 275 us, by
-//   the clock that the card holds, 1.66 to 1.75 GHz of 1.96
-//   latency for small calls: 14 us, of which join_kernel's launch takes 3
+//   between warps the rest: 1 sequence, 64 nodes x 4 heads, 95 (105) us, 0.72 PFLOP/s (0.66)
+//   the card's power limit for the largest call (64 sequences, 16 nodes): 240 to 267 (281) us,
+//   by the clock that the card holds, 1.66 to 1.78 GHz of 1.96
+//   latency for small calls: 15 us, of which join_kernel's launch takes 3
 // Tried and slower: exponentials of 32 scores beside the next 32's maxima (one vote more a
 // half tile: +5%), a tile's loop unrolled with more registers (the code left the
 // instruction caches: twice as slow), runs handed out in small pieces by a counter.
@@ -1208,6 +1209,8 @@ cudaError_t launch(tg_cache* c, TreeArgs a, const CUtensorMap& q_map, cudaStream
   constexpr int kRowBlocks = kWide ? 2 : 1, kRoom = kMaxSmem - control_bytes<L::kBuffers>();
   static_assert((kRoom - (kRowBlocks * kTile + 2 * kTreeTile) * kDim * 2) / L::kSlot >= kMinSlots, "one buffer of any call leaves enough slots");
   const int buffer = (kRowBlocks * a.q_rows + 2 * a.tree_rows) * kDim * 2;
+  // 16 sequences of 8192 tokens, 8 key heads: 64 nodes x 2 heads in one buffer beside 4 slots
+  // 121 us, the calls beside them (64 x 1, 48 x 2, 40 x 3, 32 x 4) in two beside 3 slots 146 to 153
   a.buffers = L::kBuffers;
   if (kRoom - a.buffers * buffer < kMinSlots * L::kSlot) a.buffers = 1;
   const int fixed = control_bytes<L::kBuffers>() + a.buffers * buffer;
